@@ -47,6 +47,7 @@ SOURCES = [
     "bindings.cpp",
     "gemm_bindings.cpp",
     "optim_bindings.cpp",
+    "attention_bindings.cpp",
     "comm.cpp",
     "segments.cpp",
     "collectives.cu",
@@ -59,6 +60,8 @@ SOURCES = [
     "gemm_sm100.cu",
     "optim.cu",
     "train_ops.cu",
+    "attention_fwd.cu",
+    "attention_bwd.cu",
     "noalloc.cu",
 ]
 
