@@ -48,6 +48,8 @@ SOURCES = [
     "gemm_bindings.cpp",
     "optim_bindings.cpp",
     "attention_bindings.cpp",
+    "rotary_bindings.cpp",
+    "adamw_multi_bindings.cpp",
     "comm.cpp",
     "segments.cpp",
     "collectives.cu",
@@ -62,6 +64,8 @@ SOURCES = [
     "train_ops.cu",
     "attention_fwd.cu",
     "attention_bwd.cu",
+    "rotary.cu",
+    "adamw_multi.cu",
     "noalloc.cu",
 ]
 

@@ -1,0 +1,372 @@
+// AdamW over a list of tensors in one launch, states in 32 or in 8 bits.
+//
+//   g = grad * clip,  m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2,
+//   p = p (1 - lr decay) - lr (m / (1 - b1^t)) / (sqrt(v / (1 - b2^t)) + eps)
+//
+// One warp takes a block of 256 elements of one tensor, eight neighbours per lane; which tensor it is, is looked up in
+// the table that comes with the launch's arguments, so nothing is copied to the device first and a captured launch carries
+// its own table.  Pure streaming: 28 bytes per parameter with states in 32 bits and a 16-bit parameter beside its 32-bit copy,
+// 16 bytes with states in 8 bits.
+//
+// 8-bit states.  A block keeps the size A of its largest value in 32 bits and a code c per element:
+//   m = sign * A (c / 127)^2,  v = A (c / 255)^4
+// Powers give small values finer steps than large ones: a v of 1e-9 of the largest still has a code of its own, which it needs,
+// because its root divides.  A value between two codes becomes one of them by chance, in proportion to its distances, so that
+// the mean is exact: rounding to the nearest code would stop an average whose change per step (1 - b2 of it) is below half a
+// step of the code, which at b2 = 0.999 is nearly always.  The chance is a hash of the element's place in the state, the
+// step and the seed: the same call gives the same bits.  Two rules keep the division harmless: a v that is not zero never gets
+// code 0, and a block whose largest size is below 2^-80 (whose root is far below any eps) is held as zeros.  A block that
+// holds a value that is not finite reads back as NaN throughout: a broken step does not hide.
+// The parameter is updated from the 32-bit m and v, before they are rounded.
+//
+// The products and sums that lead to a code are rounded one by one (no fused multiply-add): what a code is does not hang on what
+// a compiler makes of the expression.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+#include <string.h>
+
+#include "adamw_multi.h"
+#include "pdl.cuh"
+
+namespace pccl {
+
+namespace {
+
+constexpr int kThreads = 256;
+
+template <int MAX>
+struct Table {
+  AdamTensor t[MAX];
+  int count;
+};
+
+// Two rounds of multiply and xor-shift.  The multipliers are the leading bits of the fractional parts of the square roots
+// of 2 and 3, both odd.
+__host__ __device__ __forceinline__ uint32_t mix(uint32_t x) {
+  x ^= x >> 16;
+  x *= 0x6A09E667u;
+  x ^= x >> 15;
+  x *= 0xBB67AE85u;
+  return x ^ (x >> 16);
+}
+
+// 8-bit pieces of the state and 16- or 32-bit elements, eight at a time.
+struct Raw8 {
+  uint4 a, b;                              // fp32: both; 16 bits: a
+};
+template <int TYPE>
+__device__ __forceinline__ void widen(const Raw8& r, float* f) {
+  const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+  if constexpr (TYPE == kAdamF32) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(w[i]);
+  } else if constexpr (TYPE == kAdamBf16) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] = __uint_as_float(w[i] << 16);
+      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 x = __half22float2(*reinterpret_cast<const __half2*>(w + i));
+      f[2 * i] = x.x;
+      f[2 * i + 1] = x.y;
+    }
+  }
+}
+// 32 bytes in one access.
+__device__ __forceinline__ void load32(const void* p, Raw8& r) {
+  asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r.a.x), "=r"(r.a.y), "=r"(r.a.z), "=r"(r.a.w), "=r"(r.b.x), "=r"(r.b.y), "=r"(r.b.z), "=r"(r.b.w)
+               : "l"(p));
+}
+__device__ __forceinline__ void store32(void* p, const float* f) {
+  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]), "f"(f[4]),
+               "f"(f[5]), "f"(f[6]), "f"(f[7])
+               : "memory");
+}
+template <int TYPE>
+__device__ __forceinline__ void load8(const void* base, int64_t i, Raw8& r) {
+  if constexpr (TYPE == kAdamF32) load32(static_cast<const float*>(base) + i, r);
+  else r.a = __ldcs(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + i));
+}
+template <int TYPE>
+__device__ __forceinline__ float load1(const void* base, int64_t i) {
+  if constexpr (TYPE == kAdamF32) return static_cast<const float*>(base)[i];
+  else if constexpr (TYPE == kAdamBf16) return __bfloat162float(static_cast<const __nv_bfloat16*>(base)[i]);
+  else return __half2float(static_cast<const __half*>(base)[i]);
+}
+template <int TYPE>
+__device__ __forceinline__ uint32_t narrow2(float a, float b) {
+  if constexpr (TYPE == kAdamBf16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+template <int TYPE>
+__device__ __forceinline__ void store1(void* base, int64_t i, float x) {
+  if constexpr (TYPE == kAdamF32) static_cast<float*>(base)[i] = x;
+  else if constexpr (TYPE == kAdamBf16) static_cast<__nv_bfloat16*>(base)[i] = __float2bfloat16_rn(x);
+  else static_cast<__half*>(base)[i] = __float2half_rn(x);
+}
+
+// ---- codes
+constexpr float kSigned = 16129.f, kUnsigned = 4228250625.f;      // 127^2, 255^4 (rounded to 32 bits)
+constexpr float kSignedUnit = (float)(1.0 / 16129.0), kUnsignedUnit = (float)(1.0 / 4228250625.0);
+constexpr float kLeast = 8.271806125530277e-25f;                  // 2^-80
+
+template <bool SIGNED>
+__device__ __forceinline__ float power(float c) {
+  const float c2 = __fmul_rn(c, c);
+  return SIGNED ? c2 : __fmul_rn(c2, c2);
+}
+template <bool SIGNED>
+__device__ __forceinline__ float decode(uint32_t byte, float unit) {
+  if constexpr (SIGNED) {
+    const float c = (float)(int)(int8_t)byte;
+    return __fmul_rn(unit, __fmul_rn(fabsf(c), c));
+  } else {
+    return __fmul_rn(unit, power<false>((float)byte));
+  }
+}
+// x: the value, inv: 1 / A (0: the block holds zeros), noise: 16 bits.
+template <bool SIGNED>
+__device__ __forceinline__ uint32_t encode(float x, float inv, uint32_t noise) {
+  constexpr float top = SIGNED ? 127.f : 255.f;
+  const float y = __fmul_rn(__fmul_rn(fabsf(x), inv), SIGNED ? kSigned : kUnsigned);
+  // the largest c with c^power <= y: the hardware's root, put right by one where it is off
+  float r;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(y));
+  if constexpr (!SIGNED) asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(r));
+  float c = fminf(floorf(r), top);
+  float lo = power<SIGNED>(c), hi = power<SIGNED>(c + 1.f);
+  if (hi <= y) {
+    c += 1.f;
+    lo = hi;
+    hi = power<SIGNED>(c + 1.f);
+  } else if (lo > y) {
+    c -= 1.f;
+    hi = lo;
+    lo = power<SIGNED>(c);
+  }
+  const float u = (float)noise * 0x1p-16f + 0x1p-17f;
+  if (__fmul_rn(u, __fsub_rn(hi, lo)) < __fsub_rn(y, lo)) c += 1.f;
+  c = fminf(c, top);
+  if constexpr (SIGNED) {
+    const int i = (int)c;
+    return (uint32_t)(x < 0.f ? -i : i) & 0xffu;
+  } else {
+    return (uint32_t)(x > 0.f && inv > 0.f ? fmaxf(c, 1.f) : c);
+  }
+}
+// The block's largest size: sizes are not negative, so their bits are in the order of their values, infinities and NaN on top.
+__device__ __forceinline__ float block_max(const float* x) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(fabsf(x[i])));
+  m = __reduce_max_sync(0xffffffffu, m);
+  const float f = __uint_as_float(m);
+  return m >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : (f < kLeast ? 0.f : f);
+}
+
+template <int PT, int GT, bool BITS8, int MAX>
+__global__ void __launch_bounds__(kThreads) adamw_multi_kernel(const __grid_constant__ AdamMultiArgs a,
+                                                               const __grid_constant__ Table<MAX> table) {
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x & 31;
+  float gs = a.grad_scale;
+  if (a.total_sq_norm != nullptr) {
+    const float norm = sqrtf(*a.total_sq_norm) * a.grad_scale;
+    const float clip = a.max_grad_norm / (norm + 1e-6f);
+    gs = clip >= 1.f ? gs : gs * clip;                   // a norm that is NaN makes every gradient NaN
+  }
+  const uint32_t warps = gridDim.x * (kThreads / 32);
+  int k = 0;
+  for (uint32_t blk = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); blk < a.blocks; blk += warps) {
+    // the last tensor that starts at or before this block: its tensor is at or behind the last block's
+    int hi = table.count;
+    while (hi - k > 1) {
+      const int mid = (k + hi) >> 1;
+      if (table.t[mid].first <= blk) k = mid;
+      else hi = mid;
+    }
+    const AdamTensor& t = table.t[k];
+    const int64_t at = (int64_t)(blk - t.first) * kAdamBlock + lane * 8;       // place within the tensor
+    const uint64_t sblk = a.first_block + blk;
+    const uint64_t si = sblk * kAdamBlock + (uint64_t)lane * 8;                // place within the state
+    void* weights = PT == kAdamF32 ? t.param : static_cast<void*>(t.master);
+    const uintptr_t bad = (reinterpret_cast<uintptr_t>(weights) & 31u) | (reinterpret_cast<uintptr_t>(t.grad) & (GT == kAdamF32 ? 31u : 15u)) |
+                          (PT == kAdamF32 ? 0u : reinterpret_cast<uintptr_t>(t.param) & 15u);
+    const bool whole = bad == 0 && at - lane * 8 + kAdamBlock <= t.n;          // the same for the whole warp
+    // ---- loads
+    float g[8], p[8], m[8], v[8];
+    float m_unit = 0.f, v_unit = 0.f;
+    if (whole) {
+      Raw8 rg, rp, rm, rv;
+      load8<GT>(t.grad, at, rg);
+      load8<kAdamF32>(weights, at, rp);
+      if constexpr (BITS8) {
+        const uint2 cm = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.m) + si));
+        const uint2 cv = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.v) + si));
+        m_unit = __fmul_rn(a.m_scale[sblk], kSignedUnit);
+        v_unit = __fmul_rn(a.v_scale[sblk], kUnsignedUnit);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          m[i] = decode<true>(((i < 4 ? cm.x : cm.y) >> (8 * (i & 3))) & 0xffu, m_unit);
+          v[i] = decode<false>(((i < 4 ? cv.x : cv.y) >> (8 * (i & 3))) & 0xffu, v_unit);
+        }
+      } else {
+        load8<kAdamF32>(a.m, (int64_t)si, rm);
+        load8<kAdamF32>(a.v, (int64_t)si, rv);
+        widen<kAdamF32>(rm, m);
+        widen<kAdamF32>(rv, v);
+      }
+      widen<GT>(rg, g);
+      widen<kAdamF32>(rp, p);
+    } else {
+      if constexpr (BITS8) {
+        m_unit = __fmul_rn(a.m_scale[sblk], kSignedUnit);
+        v_unit = __fmul_rn(a.v_scale[sblk], kUnsignedUnit);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const bool on = at + i < t.n;
+        g[i] = on ? load1<GT>(t.grad, at + i) : 0.f;
+        p[i] = on ? static_cast<const float*>(weights)[at + i] : 0.f;
+        if constexpr (BITS8) {
+          m[i] = on ? decode<true>(static_cast<const uint8_t*>(a.m)[si + i], m_unit) : 0.f;
+          v[i] = on ? decode<false>(static_cast<const uint8_t*>(a.v)[si + i], v_unit) : 0.f;
+        } else {
+          m[i] = on ? static_cast<const float*>(a.m)[si + i] : 0.f;
+          v[i] = on ? static_cast<const float*>(a.v)[si + i] : 0.f;
+        }
+      }
+    }
+    // ---- the step
+    const float keep = 1.f - a.lr * t.decay;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float x = __fmul_rn(g[i], gs);
+      m[i] = __fadd_rn(__fmul_rn(a.beta1, m[i]), __fmul_rn(a.one_minus_beta1, x));
+      v[i] = __fadd_rn(__fmul_rn(a.beta2, v[i]), __fmul_rn(a.one_minus_beta2, __fmul_rn(x, x)));
+      p[i] = p[i] * keep - a.lr * (m[i] * a.bias1) / (sqrtf(v[i] * a.bias2) + a.eps);
+    }
+    // ---- states
+    uint32_t cm[2] = {0u, 0u}, cv[2] = {0u, 0u};
+    if constexpr (BITS8) {
+      const float am = block_max(m), av = block_max(v);
+      const float im = am > 0.f ? __fdiv_rn(1.f, am) : 0.f, iv = av > 0.f ? __fdiv_rn(1.f, av) : 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint64_t e = si + i;
+        const uint32_t noise = mix((uint32_t)e + (uint32_t)(e >> 32) * 0x9E3779B1u + a.key);
+        cm[i >> 2] |= encode<true>(m[i], im, noise >> 16) << (8 * (i & 3));
+        cv[i >> 2] |= encode<false>(v[i], iv, noise & 0xffffu) << (8 * (i & 3));
+      }
+      if (lane == 0) {
+        a.m_scale[sblk] = am;
+        a.v_scale[sblk] = av;
+      }
+      // padding is in the state's last block of a tensor too: its codes are 0
+      __stcs(reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.m) + si), make_uint2(cm[0], cm[1]));
+      __stcs(reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.v) + si), make_uint2(cv[0], cv[1]));
+    }
+    // ---- stores
+    if (whole) {
+      if constexpr (!BITS8) {
+        store32(static_cast<float*>(a.m) + si, m);
+        store32(static_cast<float*>(a.v) + si, v);
+      }
+      store32(static_cast<float*>(weights) + at, p);
+      if constexpr (PT != kAdamF32)
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(t.param) + at) =
+            make_uint4(narrow2<PT>(p[0], p[1]), narrow2<PT>(p[2], p[3]), narrow2<PT>(p[4], p[5]), narrow2<PT>(p[6], p[7]));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (at + i < t.n) {
+          if constexpr (!BITS8) {
+            static_cast<float*>(a.m)[si + i] = m[i];
+            static_cast<float*>(a.v)[si + i] = v[i];
+          }
+          static_cast<float*>(weights)[at + i] = p[i];
+          if constexpr (PT != kAdamF32) store1<PT>(t.param, at + i, p[i]);
+        }
+      }
+    }
+  }
+}
+
+// 2 bytes in, 8 out per element; a lane takes eight neighbours of one block.
+__global__ void __launch_bounds__(kThreads) adamw_dequantize_kernel(const uint8_t* m, const float* m_scale, const uint8_t* v,
+                                                                    const float* v_scale, float* m_out, float* v_out, int64_t n) {
+  pdl_wait();
+  pdl_trigger();
+  const int64_t stride = (int64_t)gridDim.x * kThreads * 8;
+  for (int64_t i = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * 8; i < n; i += stride) {
+    const uint2 cm = *reinterpret_cast<const uint2*>(m + i), cv = *reinterpret_cast<const uint2*>(v + i);
+    const float um = __fmul_rn(m_scale[i / kAdamBlock], kSignedUnit), uv = __fmul_rn(v_scale[i / kAdamBlock], kUnsignedUnit);
+    float x[8], y[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      x[e] = decode<true>(((e < 4 ? cm.x : cm.y) >> (8 * (e & 3))) & 0xffu, um);
+      y[e] = decode<false>(((e < 4 ? cv.x : cv.y) >> (8 * (e & 3))) & 0xffu, uv);
+    }
+    store32(m_out + i, x);
+    store32(v_out + i, y);
+  }
+}
+
+template <int PT, int GT, bool BITS8, int MAX>
+cudaError_t launch(const AdamMultiArgs& a, const AdamTensor* tensors, int count, int sm_count, cudaStream_t s) {
+  Table<MAX> table;
+  memcpy(table.t, tensors, sizeof(AdamTensor) * (size_t)count);
+  table.count = count;
+  const uint32_t need = (a.blocks + kThreads / 32 - 1) / (kThreads / 32), most = (uint32_t)sm_count * 8;
+  return launch_pdl(adamw_multi_kernel<PT, GT, BITS8, MAX>, dim3(need < most ? need : most), dim3(kThreads), 0, s, a, table);
+}
+template <int PT, int GT>
+cudaError_t launch_bits(const AdamMultiArgs& a, const AdamTensor* tensors, int count, bool bits8, int sm_count, cudaStream_t s) {
+  // a short list does not carry the long table with it
+  if (count <= 64)
+    return bits8 ? launch<PT, GT, true, 64>(a, tensors, count, sm_count, s) : launch<PT, GT, false, 64>(a, tensors, count, sm_count, s);
+  return bits8 ? launch<PT, GT, true, kAdamTensors>(a, tensors, count, sm_count, s)
+               : launch<PT, GT, false, kAdamTensors>(a, tensors, count, sm_count, s);
+}
+template <int PT>
+cudaError_t launch_grad(const AdamMultiArgs& a, const AdamTensor* t, int count, int gt, bool bits8, int sm_count, cudaStream_t s) {
+  if (gt == kAdamBf16) return launch_bits<PT, kAdamBf16>(a, t, count, bits8, sm_count, s);
+  if (gt == kAdamF16) return launch_bits<PT, kAdamF16>(a, t, count, bits8, sm_count, s);
+  return launch_bits<PT, kAdamF32>(a, t, count, bits8, sm_count, s);
+}
+
+}  // namespace
+
+uint32_t adamw_noise_key(uint64_t seed, int64_t step) { return mix(mix((uint32_t)seed) + (uint32_t)step); }
+
+cudaError_t launch_adamw_multi(const AdamMultiArgs& a, const AdamTensor* tensors, int count, int pt, int gt, bool bits8, int sm_count,
+                               cudaStream_t s) {
+  if (count <= 0 || a.blocks == 0) return cudaSuccess;
+  if (count > kAdamTensors) return cudaErrorInvalidValue;
+  if (pt == kAdamBf16) return launch_grad<kAdamBf16>(a, tensors, count, gt, bits8, sm_count, s);
+  if (pt == kAdamF16) return launch_grad<kAdamF16>(a, tensors, count, gt, bits8, sm_count, s);
+  return launch_grad<kAdamF32>(a, tensors, count, gt, bits8, sm_count, s);
+}
+
+cudaError_t launch_adamw_dequantize(const int8_t* m, const float* m_scale, const uint8_t* v, const float* v_scale, float* m_out,
+                                    float* v_out, int64_t n, cudaStream_t s) {
+  if (n <= 0) return cudaSuccess;
+  const int64_t blocks = (n / 8 + kThreads - 1) / kThreads;
+  return launch_pdl(adamw_dequantize_kernel, dim3((unsigned)(blocks < (1 << 20) ? blocks : (1 << 20))), dim3(kThreads), 0, s,
+                    reinterpret_cast<const uint8_t*>(m), m_scale, v, v_scale, m_out, v_out, n);
+}
+
+}  // namespace pccl

@@ -625,6 +625,8 @@ py::dict status_dict(Comm& c, int li) {
 void bind_gemm(py::module_& m);   // gemm_bindings.cpp
 void bind_optim(py::module_& m);  // optim_bindings.cpp
 void bind_attention(py::module_& m);  // attention_bindings.cpp
+void bind_rotary(py::module_& m);  // rotary_bindings.cpp
+void bind_adamw_multi(py::module_& m);  // adamw_multi_bindings.cpp
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "pccl native layer: sm_100a collective kernels, symmetric heap, tcgen05 GEMMs";
@@ -772,4 +774,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   bind_gemm(m);
   bind_optim(m);
   bind_attention(m);
+  bind_rotary(m);
+  bind_adamw_multi(m);
 }

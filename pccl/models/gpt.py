@@ -18,7 +18,9 @@ data gradients read their operands as they lie in memory (``pccl.ops.gemm.matmul
 kernel does not take, the same products go to cuBLAS through ``torch`` (the baseline arm).  The
 two GEMMs that directly consume a freshly gathered weight (QKV and FC1) can be replaced by the
 fused all-gather+GEMM kernel through the ``linear_fwd`` hook.  The attention core uses
-``scaled_dot_product_attention`` under a local autograd scope.
+``scaled_dot_product_attention`` under a local autograd scope, or, with ``native_attention`` on, this library's
+attention kernels (``pccl.ops.attention``).  A configuration with ``qk_norm_rope`` norms the queries and keys of each
+head and turns them by their positions (``pccl.ops.rotary``) in the place of learned position embeddings.
 """
 from __future__ import annotations
 
@@ -41,6 +43,9 @@ class GPTConfig:
     init_std: float = 0.02
     ln_eps: float = 1e-5
     name: str = "gpt"
+    qk_norm_rope: bool = False     # queries and keys normed per head and rotated; no position embedding
+    rope_theta: float = 10000.0
+    qk_eps: float = 1e-6
 
     @property
     def head_dim(self) -> int:
@@ -100,9 +105,11 @@ def unit_specs(cfg: GPTConfig) -> List[UnitSpec]:
     """Unit 0 holds the embeddings and the final layer norm (the head needs both and the
     token embedding is tied to the output projection); units 1..L are the blocks."""
     d, f = cfg.d_model, cfg.d_ff
+    positions = [] if cfg.qk_norm_rope else [ParamSpec("wpe", (cfg.seq_len, d), "normal")]
+    qk = [ParamSpec("qn_w", (cfg.head_dim,), "ones"), ParamSpec("kn_w", (cfg.head_dim,), "ones")] if cfg.qk_norm_rope else []
     units = [_layout("embed", [
         ParamSpec("wte", (cfg.vocab, d), "normal"),
-        ParamSpec("wpe", (cfg.seq_len, d), "normal"),
+        *[ParamSpec(p.name, p.shape, p.init) for p in positions],
         ParamSpec("lnf_w", (d,), "ones"),
         ParamSpec("lnf_b", (d,), "zeros"),
     ])]
@@ -120,6 +127,7 @@ def unit_specs(cfg: GPTConfig) -> List[UnitSpec]:
             ParamSpec("ln1_b", (d,), "zeros"),
             ParamSpec("ln2_w", (d,), "ones"),
             ParamSpec("ln2_b", (d,), "zeros"),
+            *[ParamSpec(p.name, p.shape, p.init) for p in qk],
         ]))
     return units
 
@@ -202,6 +210,7 @@ _native = None
 native_launches = 0     # kernels of this library launched by the functions below
 native_gemm = True       # dense products on the library's tcgen05 GEMM (off: cuBLAS through torch; set by the engine)
 fused_gelu_gemm = False  # FC1 on the tcgen05 GEMM with the GELU in its epilogue (set by the engine)
+native_attention = False  # the attention core on the library's kernels (off: scaled_dot_product_attention; set by the engine)
 fused_gelu_bwd_gemm = False  # the GELU backward as the epilogue of the data-gradient GEMM in front of it (with native_gemm)
 
 
@@ -280,34 +289,142 @@ def _gelu_bwd(dg: torch.Tensor, u: torch.Tensor, gb: torch.Tensor) -> torch.Tens
     return du
 
 
+@dataclass
+class Positions:
+    """Where the tokens of a batch stand, for a configuration with ``qk_norm_rope``: the tables of angles and, where each row
+    of the batch is not one sequence, the starts of the packed documents (int32, with the end of the last) and each token's
+    place in its own."""
+
+    cos: torch.Tensor
+    sin: torch.Tensor
+    cu_seqlens: Optional[torch.Tensor] = None
+    place: Optional[torch.Tensor] = None
+
+
+def positions_of(cfg: GPTConfig, batch: int, seq: int, device, tables=None, cu_seqlens: Optional[torch.Tensor] = None) -> Positions:
+    """The positions of a batch; ``cu_seqlens`` (int32, on the device) packs documents of any length into its batch * seq
+    tokens, one behind the other.  ``tables``: cos and sin of an earlier call."""
+    if tables is None:
+        from ..ops.rotary import rotary_table
+
+        tables = rotary_table(cfg.seq_len, cfg.head_dim, cfg.rope_theta, device)
+    pos = Positions(*tables)
+    if cu_seqlens is not None:
+        # tokens behind the last document count on from its end, within the table
+        t = torch.arange(batch * seq, dtype=torch.int32, device=device)
+        which = torch.bucketize(t, cu_seqlens[1:], right=True).clamp_(max=cu_seqlens.numel() - 1)
+        pos.cu_seqlens, pos.place = cu_seqlens, (t - cu_seqlens[which]).remainder_(pos.cos.shape[0])
+    return pos
+
+
+def native_attention_takes(cfg: GPTConfig) -> bool:
+    return cfg.head_dim % 8 == 0 and cfg.head_dim <= 128
+
+
+def _qk(qkv: torch.Tensor, p: Dict[str, torch.Tensor], cfg: GPTConfig, batch: int, pos: Positions):
+    """Normed and rotated queries and keys, [batch, rows, heads, dim]."""
+    global native_launches
+    from ..ops.rotary import qk_norm_rope_forward
+
+    T = qkv.shape[0]
+    q, k, _v = qkv.view(batch, T // batch, 3, cfg.n_head, cfg.head_dim).unbind(2)
+    native_launches += 1
+    return qk_norm_rope_forward(q, k, p["qn_w"], p["kn_w"], pos.cos, pos.sin,
+                                None if pos.place is None else pos.place.view(batch, T // batch), cfg.qk_eps)
+
+
+def _attention(qkv: torch.Tensor, p: Dict[str, torch.Tensor], cfg: GPTConfig, batch: int, pos: Optional[Positions]):
+    """Causal attention of a block from its packed projection: [T, d] and what the backward pass wants."""
+    T, d = qkv.shape[0], cfg.d_model
+    S, H, dh = T // batch, cfg.n_head, cfg.head_dim
+    q, k, v = qkv.view(batch, S, 3, H, dh).unbind(2)
+    if cfg.qk_norm_rope:
+        if pos is None:
+            raise ValueError("a configuration with qk_norm_rope needs the positions of its tokens (positions_of)")
+        q, k = _qk(qkv, p, cfg, batch, pos)
+    cu = pos.cu_seqlens if pos is not None else None
+    if native_attention and _fast(qkv):
+        global native_launches
+        from ..ops.attention import attention_forward
+
+        native_launches += 1
+        if cu is not None:
+            q, k, v = (t.reshape(T, H, dh) if t.is_contiguous() else t.view(T, H, dh) for t in (q, k, v))
+        out, lse = attention_forward(q, k, v, causal=True, cu_seqlens_q=cu)
+        return out.view(T, d), (qkv, q, k, v, out, lse)
+    if cu is not None:
+        raise ValueError("packed documents need native_attention")
+    qd, kd, vd = (t.transpose(1, 2).detach().requires_grad_() for t in (q, k, v))            # [B, H, S, dh] views
+    with torch.enable_grad():
+        att = F.scaled_dot_product_attention(qd, kd, vd, is_causal=True)                      # [B, H, S, dh]
+    return att.detach().transpose(1, 2).reshape(T, d), (qkv if cfg.qk_norm_rope else None, qd, kd, vd, att, None)
+
+
+def _attention_backward(da: torch.Tensor, saved, p: Dict[str, torch.Tensor], gr: Dict[str, torch.Tensor], cfg: GPTConfig, batch: int,
+                        pos: Optional[Positions]) -> torch.Tensor:
+    """[T, 3d] gradient of the packed projection; writes the bias gradient of the projection (its column sums) and those of
+    the query and key norms."""
+    global native_launches
+    T, d = da.shape
+    S, H, dh = T // batch, cfg.n_head, cfg.head_dim
+    qkv, q, k, v, att, lse = saved
+    if lse is None:
+        datt = da.view(batch, S, H, dh).transpose(1, 2)
+        dq, dk, dv = torch.autograd.grad(att, (q, k, v), datt)
+        if not cfg.qk_norm_rope:
+            return _cat_qkv_grads(dq, dk, dv, T, d, gr["qkv_b"])
+        dqkv = torch.empty(T, 3 * d, dtype=da.dtype, device=da.device)
+        parts = dqkv.view(batch, S, 3, H, dh).unbind(2)
+        dq, dk = (t.transpose(1, 2).contiguous() for t in (dq, dk))
+        parts[2].copy_(dv.transpose(1, 2))
+    else:
+        from ..ops.attention import attention_backward
+
+        native_launches += 3
+        dqkv = torch.empty_like(qkv)
+        parts = dqkv.view(batch, S, 3, H, dh).unbind(2)
+        grads = parts
+        if pos is not None and pos.cu_seqlens is not None:
+            grads = dqkv.view(T, 3, H, dh).unbind(1)
+            dqkv.zero_()                            # tokens behind the last document have no gradient
+        attention_backward(da.view(att.shape), q, k, v, att, lse, causal=True,
+                           cu_seqlens_q=pos.cu_seqlens if pos is not None else None, dq=grads[0], dk=grads[1], dv=grads[2])
+        dq, dk = parts[0], parts[1]
+    if cfg.qk_norm_rope:
+        from ..ops.rotary import qk_norm_rope_backward
+
+        native_launches += 2
+        q0, k0, _v0 = qkv.view(batch, S, 3, H, dh).unbind(2)
+        qk_norm_rope_backward(dq, dk, q0, k0, p["qn_w"], p["kn_w"], pos.cos, pos.sin,
+                              None if pos.place is None else pos.place.view(batch, S), cfg.qk_eps, dq_in=parts[0], dk_in=parts[1],
+                              dq_weight=gr["qn_w"], dk_weight=gr["kn_w"])
+    _bias_grad(dqkv, gr["qkv_b"])
+    return dqkv
+
+
 def layer_forward_deferred(x: torch.Tensor, branch: Optional[torch.Tensor], p: Dict[str, torch.Tensor], cfg: GPTConfig,
-                           batch: int, linear_fwd: LinearFwd = _default_linear):
-    """One transformer block whose residual adds ride on the layer norms.
+                           batch: int, linear_fwd: LinearFwd = _default_linear, pos: Optional[Positions] = None):
+    """One transformer block whose residual adds ride on the layer norms.  ``pos``: where its tokens stand, for a
+    configuration with ``qk_norm_rope`` (``positions_of``).
 
     The block's input is ``x + branch`` (``branch``: the previous block's MLP output, not yet
     added; None for the first block).  Returns ``(x2, mlp_out, ctx)``: the block's output is
     ``x2 + mlp_out``, left unsummed so the next layer norm adds it in its own pass."""
-    T, d = x.shape
-    S, H, dh = T // batch, cfg.n_head, cfg.head_dim
     h1, mean1, rstd1, x = _ln_fwd(x, p["ln1_w"], p["ln1_b"], cfg.ln_eps, branch)
     qkv = linear_fwd(h1, p["qkv_w"], p["qkv_b"], "qkv")                  # [T, 3d]
-    q, k, v = (t.transpose(1, 2) for t in qkv.view(batch, S, 3, H, dh).unbind(2))   # [B, H, S, dh] views
-    qd, kd, vd = (t.detach().requires_grad_() for t in (q, k, v))
-    with torch.enable_grad():
-        att = F.scaled_dot_product_attention(qd, kd, vd, is_causal=True)            # [B, H, S, dh]
-    a = att.detach().transpose(1, 2).reshape(T, d)
+    a, att = _attention(qkv, p, cfg, batch, pos)                         # [T, d]
     o = mm_nt(a, p["proj_w"], p["proj_b"])
     h2, mean2, rstd2, x2 = _ln_fwd(x, p["ln2_w"], p["ln2_b"], cfg.ln_eps, o)       # x2 = x + o, in o's memory
     u, g = _fc1_gelu(h2, p, linear_fwd)                                  # [T, f]
     m = mm_nt(g, p["fc2_w"], p["fc2_b"])
-    ctx = (x, mean1, rstd1, h1, qd, kd, vd, att, a, x2, mean2, rstd2, h2, u, g)
+    ctx = (x, mean1, rstd1, h1, att, a, x2, mean2, rstd2, h2, u, g, pos)
     return x2, m, ctx
 
 
 def layer_forward(x: torch.Tensor, p: Dict[str, torch.Tensor], cfg: GPTConfig, batch: int,
-                  linear_fwd: LinearFwd = _default_linear):
+                  linear_fwd: LinearFwd = _default_linear, pos: Optional[Positions] = None):
     """x: [T, d] with T = batch * seq.  Returns (y, ctx)."""
-    x2, m, ctx = layer_forward_deferred(x, None, p, cfg, batch, linear_fwd)
+    x2, m, ctx = layer_forward_deferred(x, None, p, cfg, batch, linear_fwd, pos)
     return m.add_(x2), ctx
 
 
@@ -338,9 +455,7 @@ def layer_backward(dy: torch.Tensor, ctx, p: Dict[str, torch.Tensor], gr: Dict[s
     q/k/v packing) instead of between them.  The current stream waits for ``side`` before the
     function returns, and every tensor a side-stream GEMM reads stays referenced until then."""
     global native_launches
-    x, mean1, rstd1, h1, qd, kd, vd, att, a, x2, mean2, rstd2, h2, u, g = ctx
-    T, d = x.shape
-    S, H, dh = T // batch, cfg.n_head, cfg.head_dim
+    x, mean1, rstd1, h1, att, a, x2, mean2, rstd2, h2, u, g, pos = ctx
     main = torch.cuda.current_stream(dy.device) if side is not None else None
 
     def wgrad(dy_, x_, gw):
@@ -371,9 +486,7 @@ def layer_backward(dy: torch.Tensor, ctx, p: Dict[str, torch.Tensor], gr: Dict[s
     dx2 = _ln_bwd(dh2, x2, mean2, rstd2, p["ln2_w"], p["ln2_b"], gr["ln2_w"], gr["ln2_b"], resid=dy, dx_sum=gr["proj_b"])
     wgrad(dx2, a, gr["proj_w"])
     da = mm_nn(dx2, p["proj_w"])
-    datt = da.view(batch, S, H, dh).transpose(1, 2)
-    dq, dk, dv = torch.autograd.grad(att, (qd, kd, vd), datt)
-    dqkv = _cat_qkv_grads(dq, dk, dv, T, d, gr["qkv_b"])
+    dqkv = _attention_backward(da, att, p, gr, cfg, batch, pos)
     wgrad(dqkv, h1, gr["qkv_w"])
     dh1 = mm_nn(dqkv, p["qkv_w"])
     dx = _ln_bwd(dh1, x, mean1, rstd1, p["ln1_w"], p["ln1_b"], gr["ln1_w"], gr["ln1_b"], resid=dx2, dx_sum=dx_sum)
@@ -386,14 +499,17 @@ def embed_forward(tokens: torch.Tensor, p: Dict[str, torch.Tensor]) -> torch.Ten
     """tokens: [B, S] int64 -> [B*S, d]."""
     B, S = tokens.shape
     x = F.embedding(tokens, p["wte"])
-    x = x + p["wpe"][:S].unsqueeze(0)
+    if "wpe" in p:
+        x = x + p["wpe"][:S].unsqueeze(0)
     return x.view(B * S, -1)
 
 
 def embed_backward(dx: torch.Tensor, tokens: torch.Tensor, gr: Dict[str, torch.Tensor]) -> None:
-    """Accumulates into gr["wte"] (the head already wrote its share) and writes gr["wpe"]."""
+    """Accumulates into gr["wte"] (the head already wrote its share) and writes gr["wpe"] where the model has it."""
     B, S = tokens.shape
     gr["wte"].index_add_(0, tokens.reshape(-1), dx)
+    if "wpe" not in gr:
+        return
     gw = gr["wpe"]
     gw.zero_()
     gw[:S].copy_(dx.view(B, S, -1).sum(0))

@@ -8,7 +8,7 @@ NCCL (the baseline arm); after ``pccl.patch_deepspeed.patch_deepspeed`` the very
 engine gathers parameters and reduces gradients through this library's kernels.
 
 Memory plan (per rank, P ranks, N parameters):
-  bf16 parameter shard N/P, fp32 master + Adam moments 12 N/P, gradient shard 2-4 N/P,
+  bf16 parameter shard N/P, fp32 master + Adam moments 12 N/P (6 N/P with moments in 8 bits), gradient shard 2-4 N/P,
   two rotating gathered-parameter buffers and two rotating gradient buffers of the
   largest unit (bf16), one dedicated gradient buffer for the embedding unit.
 With the patched backend all communication buffers live in the symmetric heap, so
@@ -97,7 +97,7 @@ class Zero3Engine:
                  linear_fwd: Optional[Callable] = None, micro_batch: int = 1, fused_ag_gemm: bool = False,
                  gather_ctas: int = 16, fused_gelu_gemm: bool = False, overlap_wgrad: bool = False,
                  native_gemm: bool = False, copy_engine_gather: bool = False, fused_gelu_bwd_gemm: bool = False,
-                 dynamic_tiles: Optional[bool] = None):
+                 dynamic_tiles: Optional[bool] = None, native_attention: bool = False, optim_bits: int = 32):
         from .. import build_kernels
 
         self.C = build_kernels.load()
@@ -120,6 +120,15 @@ class Zero3Engine:
         self.dynamic_tiles = (self.world > 1) if dynamic_tiles is None else bool(dynamic_tiles)
         # GELU backward as the epilogue of the data-gradient GEMM of FC2 (needs native_gemm)
         self.fused_gelu_bwd_gemm = bool(fused_gelu_bwd_gemm) and self.native_gemm
+        # the attention core on the library's kernels instead of scaled_dot_product_attention
+        if cfg.qk_norm_rope and cfg.head_dim % 8 != 0:
+            raise ValueError("qk_norm_rope wants a head size that is a multiple of 8")
+        self.native_attention = bool(native_attention) and gpt.native_attention_takes(cfg)
+        self._rope_tables = None
+        # both Adam moments in 32 bits, or in 8 with a scale for each 256 (pccl.ops.optim)
+        if optim_bits not in (8, 32):
+            raise ValueError("optim_bits must be 8 or 32")
+        self.optim_bits = optim_bits
         # parameter gathers by the GPU's copy engines instead of gather kernels (no SM is taken from
         # the GEMMs they overlap); needs symmetric parameter shards
         self.copy_engine_gather = bool(copy_engine_gather)
@@ -180,8 +189,14 @@ class Zero3Engine:
             for b in self.gradbuf + [self.gradbuf0]:
                 b.zero_()
         self.master = torch.empty(total_shard, dtype=torch.float32, device=self.device)
-        self.exp_avg = torch.zeros(total_shard, dtype=torch.float32, device=self.device)
-        self.exp_avg_sq = torch.zeros(total_shard, dtype=torch.float32, device=self.device)
+        self.exp_avg = self.exp_avg_sq = self.adam8 = None
+        if optim_bits == 32:
+            self.exp_avg = torch.zeros(total_shard, dtype=torch.float32, device=self.device)
+            self.exp_avg_sq = torch.zeros(total_shard, dtype=torch.float32, device=self.device)
+        else:
+            from ..ops.optim import adamw_state
+
+            self.adam8 = adamw_state([self.master], bits=8)
         self.sq_norm = torch.zeros(1, dtype=torch.float32, device=self.device)
         self.loss_sum = torch.zeros(1, dtype=torch.float32, device=self.device)
         # rows whose target was neither the ignore index nor a valid class (the loss kernel skips them)
@@ -292,11 +307,18 @@ class Zero3Engine:
 
     # ------------------------------------------------------------------ one training step
     @torch.no_grad()
-    def train_step(self, tokens: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
+    def train_step(self, tokens: torch.Tensor, targets: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None) -> torch.Tensor:
         """tokens, targets: [B, S] int64, on the host (pinned) or on the device.  Runs
         forward, backward, gradient reduction and the optimizer; returns the mean loss of
-        this rank's micro-batch as a one-element device tensor."""
+        this rank's micro-batch as a one-element device tensor.
+
+        ``cu_seqlens`` (int32, on the device) packs documents of any length into the B * S tokens, one behind the other: the
+        starts of the documents and the end of the last.  Attention and positions then keep to each document.  Needs
+        ``native_attention`` and a configuration with ``qk_norm_rope``; documents are at most ``cfg.seq_len`` long (what
+        lies behind starts again at position 0)."""
         cfg, C = self.cfg, self.C
+        if cu_seqlens is not None and not (self.native_attention and cfg.qk_norm_rope):
+            raise ValueError("packed documents need native_attention and a configuration with qk_norm_rope")
         if tokens.device.type != "cuda":
             if self._tokens_dev is None or self._tokens_dev.shape != tokens.shape:
                 self._tokens_dev = torch.empty(tokens.shape, dtype=torch.int64, device=self.device)
@@ -324,6 +346,11 @@ class Zero3Engine:
         gpt.native_gemm = self.native_gemm
         C.gemm_set_dynamic_tiles(self.dynamic_tiles)
         gpt.fused_gelu_bwd_gemm = self.fused_gelu_bwd_gemm
+        gpt.native_attention = self.native_attention
+        pos = None
+        if cfg.qk_norm_rope:
+            pos = gpt.positions_of(cfg, B, S, self.device, self._rope_tables, cu_seqlens)
+            self._rope_tables = (pos.cos, pos.sin)
         saved = []
         for li in range(1, L + 1):
             slot = li % 2
@@ -333,7 +360,7 @@ class Zero3Engine:
             skip = (0, 1) if self.fused_ag_gemm else ()
             nxt = self._gather(li + 1, 1 - slot, skip) if li < L else self._gather(0, 1 - slot)
             self._cur = (li, slot)
-            x, branch, ctx = gpt.layer_forward_deferred(x, branch, self.pviews[li][slot], cfg, B, self.linear_fwd)
+            x, branch, ctx = gpt.layer_forward_deferred(x, branch, self.pviews[li][slot], cfg, B, self.linear_fwd, pos)
             self._cur = None
             saved.append(ctx)
         # ---- head: final norm, tied projection, loss; forward and backward together
@@ -376,9 +403,16 @@ class Zero3Engine:
             C.sq_norm(self.grad_shard, self.sq_norm)
             if self.world > 1:
                 _wait(self.backend.all_reduce(self.sq_norm, group=self.group, async_op=False))
-        C.adamw(self.master, self.exp_avg, self.exp_avg_sq, self.grad_shard, self.param_shard, o.lr, o.beta1, o.beta2,
-                o.eps, o.weight_decay, self.step_count, 1.0, o.max_grad_norm,
-                self.sq_norm if o.max_grad_norm > 0 else None)
+        if self.adam8 is not None:
+            from ..ops.optim import adamw_step
+
+            adamw_step([self.param_shard], [self.grad_shard], self.adam8, step=self.step_count, lr=o.lr, beta1=o.beta1, beta2=o.beta2,
+                       eps=o.eps, weight_decay=o.weight_decay, masters=[self.master], max_grad_norm=o.max_grad_norm,
+                       total_sq_norm=self.sq_norm if o.max_grad_norm > 0 else None, seed=self.rank)
+        else:
+            C.adamw(self.master, self.exp_avg, self.exp_avg_sq, self.grad_shard, self.param_shard, o.lr, o.beta1, o.beta2,
+                    o.eps, o.weight_decay, self.step_count, 1.0, o.max_grad_norm,
+                    self.sq_norm if o.max_grad_norm > 0 else None)
         if self.copy_engine_gather:
             # the next step's copy-engine gathers read the peers' shards without a handshake: nobody
             # may start them before every rank's optimizer has written its shard (device barrier
@@ -397,6 +431,10 @@ class Zero3Engine:
         from ..ops.gemm import check_errors as check_gemm_errors
 
         check_gemm_errors(self.device)
+        if self.native_attention:
+            from ..ops.attention import check_errors as check_attention_errors
+
+            check_attention_errors(self.device)
         bad = int(self.bad_targets.item())
         if bad:
             self.bad_targets.zero_()
@@ -415,14 +453,22 @@ class Zero3Engine:
 
     # ------------------------------------------------------------------ checkpoint (sharded)
     def state_dict(self) -> Dict[str, torch.Tensor]:
-        return {"master": self.master, "exp_avg": self.exp_avg, "exp_avg_sq": self.exp_avg_sq,
-                "step": torch.tensor(self.step_count), "world": torch.tensor(self.world)}
+        sd = {"master": self.master, "step": torch.tensor(self.step_count), "world": torch.tensor(self.world)}
+        if self.adam8 is None:
+            sd.update(exp_avg=self.exp_avg, exp_avg_sq=self.exp_avg_sq)
+        else:
+            sd.update(exp_avg=self.adam8.exp_avg, exp_avg_sq=self.adam8.exp_avg_sq, exp_avg_scale=self.adam8.exp_avg_scale,
+                      exp_avg_sq_scale=self.adam8.exp_avg_sq_scale)
+        return sd
 
     def load_state_dict(self, sd: Dict[str, torch.Tensor]) -> None:
         if int(sd["world"]) != self.world:
             raise ValueError("sharded checkpoint was written with a different world size")
-        self.master.copy_(sd["master"])
-        self.exp_avg.copy_(sd["exp_avg"])
-        self.exp_avg_sq.copy_(sd["exp_avg_sq"])
+        if ("exp_avg_scale" in sd) != (self.adam8 is not None):
+            raise ValueError("checkpoint was written with a different optim_bits")
+        own = self.state_dict()
+        for name in own:
+            if name not in ("step", "world"):
+                own[name].copy_(sd[name])
         self.param_shard.copy_(self.master)
         self.step_count = int(sd["step"])

@@ -17,8 +17,10 @@ def _oracle(q, k, v, see, scale, dout=None, out=None, lse=None):
     """One sequence, [rows, heads, dim]; returns values and how far each may be off.
 
     u: half a step of the 16-bit type.  Probabilities and score gradients are rounded to it before a product, results once at
-    the end.  Everything else is 32-bit: a sum of D products is off by at most D + 2 roundings of the sum of their sizes."""
-    u, f = torch.finfo(q.dtype).eps / 2, 2.0 ** -23
+    the end.  Everything else is 32-bit: a sum of D products is off by at most D + 2 roundings of the sum of their sizes.
+    ``ftz``: the exponential and the tensor cores' sums flush what is below 2^-126 to zero, so a probability and each partial sum may
+    be off by that much, whatever its size."""
+    u, f, ftz = torch.finfo(q.dtype).eps / 2, 2.0 ** -23, 2.0 ** -126
     G = q.shape[1] // k.shape[1]
     D = q.shape[2]
     up = lambda x: x.double().transpose(0, 1)                                    # noqa: E731
@@ -34,19 +36,19 @@ def _oracle(q, k, v, see, scale, dout=None, out=None, lse=None):
         a = p @ V.abs()
         # a probability of a 16-bit type below its normal range is off by half of its smallest step; the running maximum
         # may be below the true one by 2^8, never above
-        tiny = torch.finfo(q.dtype).tiny * u * V.abs().sum(1, keepdim=True)
         n = max(s.shape[-1], 1)
+        tiny = (torch.finfo(q.dtype).tiny * u + ftz) * V.abs().sum(1, keepdim=True) + n * ftz
         return (o.transpose(0, 1), ((u + 2 * e_s + n * 2.0 ** -24) * a + u * o.abs() + tiny).transpose(0, 1) + torch.finfo(q.dtype).tiny * u,
                 L, e_s + n * 2.0 ** -24 + f * L.nan_to_num(neginf=0.0).abs())
     L, dO, O = lse.double(), up(dout), up(out)
     p = torch.exp(s - L.nan_to_num(neginf=0.0)[..., None])
     dp, delta = dO @ V.transpose(1, 2), (dO * O).sum(-1, keepdim=True)
     ds = p * (dp - delta)
-    e_p = (D + 4) * f * (size.amax() if size.numel() else 0.0) + f * L.nan_to_num(neginf=0.0).abs().max() + 2.0 ** -20
+    e_p = (D + 4) * f * (size.amax() if size.numel() else 0.0) + f * (L.nan_to_num(neginf=0.0).abs().max() if L.numel() else 0.0) + 2.0 ** -20
     e_dp = (D + 4) * f * (dO.abs() @ V.abs().transpose(1, 2) + (dO * O).abs().sum(-1, keepdim=True))
     small = torch.finfo(q.dtype).tiny * u
-    e_ds = (u + 2 * e_p) * ds.abs() + p * e_dp + small
-    e_pr = (u + 2 * e_p) * p + small
+    e_ds = (u + 2 * e_p) * ds.abs() + p * e_dp + small + ftz * (1 + (dp - delta).abs())
+    e_pr = (u + 2 * e_p) * p + small + ftz
     share = lambda x: x.unflatten(0, (k.shape[1], G)).sum(1)                      # noqa: E731
     n = G * max(s.shape[1], s.shape[2])
     dq, dk, dv = (ds @ K) * scale, share(ds.transpose(1, 2) @ Q) * scale, share(p.transpose(1, 2) @ dO)
@@ -55,7 +57,7 @@ def _oracle(q, k, v, see, scale, dout=None, out=None, lse=None):
     t_k = share(ads.transpose(1, 2) @ Q.abs()) * scale + u * dk.abs()
     t_v = share((e_pr + n * f * p).transpose(1, 2) @ dO.abs()) + u * dv.abs()
     down = lambda x: x.transpose(0, 1)                                           # noqa: E731
-    return [(down(x), down(t) + small) for x, t in ((dq, t_q), (dk, t_k), (dv, t_v))]
+    return [(down(x), down(t) + small + (n + 1) * ftz * max(scale, 1.0)) for x, t in ((dq, t_q), (dk, t_k), (dv, t_v))]
 
 
 def _close(got, want, tol, what):
@@ -131,3 +133,242 @@ def test_backward_matches_formula(case):
         want = _oracle(q[b], k[b], v[b], _visible(Sq, Sk, causal), D ** -0.5, dout[b], out[b], lse[b])
         for x, (w, t), what in zip(got, want, ("dq", "dk", "dv")):
             _close(x[b], w, t, what)
+
+
+# queries and keys of each packed sequence, rows behind the last one, heads, key heads, dim, causal
+PACKED = [
+    ([(1, 1)], 0, 1, 1, 64, True), ([(5, 5), (0, 0), (130, 130), (1, 1), (128, 128), (257, 257)], 7, 4, 2, 128, True),
+    ([(300, 300), (0, 40), (40, 0), (77, 500), (129, 64)], 130, 2, 1, 64, True), ([(33, 33)] * 40, 3, 2, 2, 80, False),
+    ([(0, 0), (0, 0)], 300, 2, 2, 128, True), ([(700, 300), (300, 700)], 1, 4, 4, 128, True), ([(7, 7), (2, 2)] * 37, 0, 3, 1, 40, True),
+]
+
+
+def _pack(lens, tail, H, Hk, D, dtype, seed, poison):
+    """Packed inputs whose rows behind the last sequence are ``poison``."""
+    q, _k, _v, dout = _inputs(1, sum(a for a, _ in lens) + tail, sum(b for _, b in lens) + tail + 1, H, Hk, D, dtype, seed)
+    k, v = _k, _v
+    q, k, v, dout = (x[0].clone() for x in (q, k, v, dout))
+    cu = [torch.tensor([0] + [sum(x[i] for x in lens[:n + 1]) for n in range(len(lens))], dtype=torch.int32, device=DEV) for i in (0, 1)]
+    for x, c in ((q, cu[0]), (dout, cu[0]), (k, cu[1]), (v, cu[1])):
+        x[int(c[-1]):] = poison
+    return q, k, v, dout, cu
+
+
+@pytest.mark.parametrize("poison", [0.0, math.nan, math.inf])
+@pytest.mark.parametrize("case", PACKED, ids=str)
+def test_packed_sequences_stay_apart(case, poison):
+    from pccl.ops.attention import attention_backward, attention_forward, check_errors
+
+    lens, tail, H, Hk, D, causal = case
+    q, k, v, dout, (cq, ck) = _pack(lens, tail, H, Hk, D, BF, 3, poison)
+    out, lse = attention_forward(q, k, v, causal=causal, cu_seqlens_q=cq, cu_seqlens_k=ck)
+    dq, dk, dv = attention_backward(dout, q, k, v, out, lse, causal=causal, cu_seqlens_q=cq, cu_seqlens_k=ck)
+    check_errors()
+    for i, (n, m) in enumerate(lens):
+        a, b = int(cq[i]), int(ck[i])
+        sq, sk, sv, sd = q[a:a + n], k[b:b + m], v[b:b + m], dout[a:a + n]
+        see = _visible(n, m, causal)
+        o, to, L, tl = _oracle(sq, sk, sv, see, D ** -0.5)
+        _close(out[a:a + n], o, to, "out")
+        got = lse[:, a:a + n]
+        assert torch.equal(got == -math.inf, L == -math.inf)
+        _close(got.masked_fill(L == -math.inf, 0), L.masked_fill(L == -math.inf, 0), tl, "lse")
+        want = _oracle(sq, sk, sv, see, D ** -0.5, sd, out[a:a + n], got.contiguous())
+        for x, (w, t), what in zip((dq[a:a + n], dk[b:b + m], dv[b:b + m]), want, ("dq", "dk", "dv")):
+            _close(x, w, t, what)
+    # what is allocated here holds zeros behind the last sequence
+    for x, c in ((out, cq), (dq, cq), (dk, ck), (dv, ck)):
+        assert torch.all(x[int(c[-1]):] == 0)
+    assert torch.all(lse[:, int(cq[-1]):] == -math.inf)
+
+
+def test_packed_outputs_of_the_caller_keep_the_rows_behind():
+    from pccl.ops.attention import attention_backward, attention_forward
+
+    q, k, v, dout, (cq, ck) = _pack([(50, 50), (90, 90)], 20, 2, 2, 64, BF, 4, 0.0)
+    k, v = k[:160], v[:160]
+    new = [torch.full_like(t, 7.0) for t in (q, q, k, v)]
+    _out, lse = attention_forward(q, k, v, cu_seqlens_q=cq, out=new[0])
+    attention_backward(dout, q, k, v, new[0], lse, cu_seqlens_q=cq, dq=new[1], dk=new[2], dv=new[3])
+    ref, _ = attention_forward(q, k, v, cu_seqlens_q=cq)
+    assert torch.equal(new[0][:140], ref[:140])
+    for x in new:
+        assert torch.all(x[140:] == 7.0) and not torch.any(x[:140] == 7.0)
+
+
+def test_neighbouring_sequences_may_hold_nan():
+    from pccl.ops.attention import attention_backward, attention_forward
+
+    lens = [(70, 70), (60, 60), (200, 200)]
+    q, k, v, dout, (cq, ck) = _pack(lens, 0, 2, 1, 128, BF, 5, 0.0)
+    k, v = k[:330], v[:330]
+    good = attention_forward(q, k, v, cu_seqlens_q=cq)
+    grads = attention_backward(dout, q, k, v, *good, cu_seqlens_q=cq)
+    for x in (q, k, v, dout):
+        x[70:130] = math.nan
+    bad = attention_forward(q, k, v, cu_seqlens_q=cq)
+    bgrads = attention_backward(dout, q, k, v, *bad, cu_seqlens_q=cq)
+    for a, b in ((good[0], bad[0]), (good[1].t(), bad[1].t()), *zip(grads, bgrads)):
+        assert torch.equal(a[:70], b[:70]) and torch.equal(a[130:], b[130:])
+        assert torch.isnan(b[70:130]).all()
+
+
+def test_large_scores_and_rising_maxima():
+    """Scores of hundreds, rising along the keys, so that the running maximum is followed again and again."""
+    from pccl.ops.attention import attention_backward, attention_forward, check_errors
+
+    for dtype in (BF, FP):
+        q, k, v, dout = _inputs(1, 600, 600, 2, 2, 64, dtype, 6)
+        q, v = q * 4, v.contiguous()
+        k = k * torch.linspace(0.1, 8, 600, device=DEV).view(1, -1, 1, 1).to(dtype)
+        for causal in (True, False):
+            out, lse = attention_forward(q, k, v, causal=causal)
+            _check_forward(out, lse, q, k, v, causal, 64 ** -0.5)
+            o, L = _given(q, k, v, causal, 64 ** -0.5)
+            got = attention_backward(dout, q, k, v, o, L, causal=causal)
+            check_errors()
+            for x, (w, t), what in zip(got, _oracle(q[0], k[0], v[0], _visible(600, 600, causal), 64 ** -0.5, dout[0], o[0], L[0]),
+                                       ("dq", "dk", "dv")):
+                _close(x[0], w, t, what)
+
+
+def test_other_scales_strides_and_outputs():
+    from pccl.ops.attention import attention_backward, attention_forward
+
+    g = torch.Generator(device=DEV).manual_seed(7)
+    B, S, H, Hk, D = 2, 200, 4, 2, 64
+    base = torch.randn(B, H, S, 72, device=DEV, generator=g).to(BF)              # heads before rows, gaps behind columns
+    q = base[..., :D].transpose(1, 2)
+    kv = torch.randn(S, B, 2 * Hk, D, device=DEV, generator=g).to(BF)            # rows before the batch
+    k, v = kv[:, :, :Hk].transpose(0, 1), kv[:, :, Hk:].transpose(0, 1)
+    out = torch.empty(B, S, 2 * H, D, device=DEV, dtype=BF)[:, :, ::2]
+    got, lse = attention_forward(q, k, v, causal=True, scale=0.3, out=out)
+    assert got.data_ptr() == out.data_ptr()
+    _check_forward(out, lse, q, k, v, True, 0.3)
+    dout = torch.randn(B, S, H, D, device=DEV, generator=g).to(BF)
+    pack = torch.full((B, S, H + 2 * Hk, D), 9.0, device=DEV, dtype=BF)
+    grads = (pack[:, :, :H], pack[:, :, H:H + Hk], pack[:, :, H + Hk:])
+    attention_backward(dout, q, k, v, out, lse, causal=True, scale=0.3, dq=grads[0], dk=grads[1], dv=grads[2])
+    plain = attention_backward(dout, q.contiguous(), k.contiguous(), v.contiguous(), out.contiguous(), lse, causal=True, scale=0.3)
+    for a, b in zip(grads, plain):
+        assert torch.equal(a, b)
+
+
+def test_results_do_not_change_from_call_to_call():
+    from pccl.ops.attention import attention_backward, attention_forward
+
+    q, k, v, dout = _inputs(2, 500, 500, 8, 2, 64, BF, 8)
+    first = attention_forward(q, k, v)
+    grads = attention_backward(dout, q, k, v, *first)
+    for _ in range(3):
+        again = attention_forward(q, k, v)
+        for a, b in zip((*first, *grads), (*again, *attention_backward(dout, q, k, v, *again))):
+            assert torch.equal(a, b)
+
+
+def test_captured_calls_and_other_streams():
+    """Two captured graphs and eager calls on two streams at once: nothing is shared between them."""
+    from pccl.ops.attention import attention_backward, attention_forward, check_errors
+
+    data = [_inputs(1, 300, 300, 4, 4, 128, BF, s) for s in (20, 21, 22, 23)]
+    run = lambda d: (lambda f: (*f, *attention_backward(d[3], *d[:3], *f)))(attention_forward(*d[:3]))      # noqa: E731
+    want = [run(d) for d in data]
+    graphs = []
+    for d in data[:2]:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            res = run(d)
+        graphs.append((g, res))
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        eager = []
+        for s, (g, _r) in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        for s, d in zip(streams[2:], data[2:]):
+            with torch.cuda.stream(s):
+                eager.append(run(d))
+        torch.cuda.synchronize()
+        for w, got in zip(want, [r for _g, r in graphs] + eager):
+            for a, b in zip(w, got):
+                assert torch.equal(a, b)
+    check_errors()
+
+
+def test_empty_calls():
+    from pccl.ops.attention import attention_backward, attention_forward
+
+    z = lambda *s: torch.zeros(*s, device=DEV, dtype=BF)                          # noqa: E731
+    out, lse = attention_forward(z(1, 5, 2, 64) + 1, z(1, 0, 2, 64), z(1, 0, 2, 64))
+    assert torch.all(out == 0) and torch.all(lse == -math.inf)
+    dq, dk, dv = attention_backward(z(1, 5, 2, 64) + 1, z(1, 5, 2, 64) + 1, z(1, 0, 2, 64), z(1, 0, 2, 64), out, lse)
+    assert torch.all(dq == 0) and dk.numel() == 0 and dv.numel() == 0
+    out, lse = attention_forward(z(1, 0, 2, 64), z(1, 5, 2, 64), z(1, 5, 2, 64))
+    assert out.numel() == 0 and lse.numel() == 0
+    dq, dk, dv = attention_backward(z(1, 0, 2, 64), z(1, 0, 2, 64), z(1, 5, 2, 64), z(1, 5, 2, 64), out, lse)
+    assert torch.all(dk == 0) and torch.all(dv == 0)
+    assert attention_forward(z(0, 5, 2, 64), z(0, 5, 2, 64), z(0, 5, 2, 64))[0].shape == (0, 5, 2, 64)
+
+
+def test_starts_out_of_order_or_range_touch_nothing_outside():
+    """Broken starts give results that mean nothing, within the tensors: rows of guard around them keep their values."""
+    from pccl.ops.attention import attention_backward, attention_forward, check_errors
+
+    q, k, v, dout, _ = _pack([(300, 300)], 0, 2, 2, 64, BF, 9, 0.0)
+    k, v = k[:300], v[:300]
+    for starts in ([0, 1000], [-50, 200], [200, 100, 300], [300, 0], [2 ** 31 - 1, -2 ** 31, 5], [0, 300, 0, 300]):
+        cu = torch.tensor(starts, dtype=torch.int32, device=DEV)
+        guards = [torch.full((500, 2, 64), 3.0, device=DEV, dtype=BF) for _ in range(4)]
+        outs = [g[100:400] for g in guards]
+        _o, lse = attention_forward(q, k, v, cu_seqlens_q=cu, out=outs[0])
+        attention_backward(dout, q, k, v, outs[0], lse.nan_to_num(0, 0, 0), cu_seqlens_q=cu, dq=outs[1], dk=outs[2], dv=outs[3])
+        check_errors()
+        for g in guards:
+            assert torch.all(g[:100] == 3.0) and torch.all(g[400:] == 3.0)
+
+
+def test_refusals():
+    from pccl.ops.attention import attention_backward, attention_forward
+
+    mk = lambda *s, dt=BF: torch.zeros(*s, device=DEV, dtype=dt)                  # noqa: E731
+    q, k = mk(1, 8, 4, 64), mk(1, 8, 2, 64)
+    cu = torch.tensor([0, 8], dtype=torch.int32, device=DEV)
+    bad = [
+        lambda: attention_forward(q.float(), k.float(), k.float()),
+        lambda: attention_forward(q, k.half(), k),
+        lambda: attention_forward(q, mk(1, 8, 3, 64), mk(1, 8, 3, 64)),            # 4 query heads on 3 key heads
+        lambda: attention_forward(q, k, mk(1, 9, 2, 64)),
+        lambda: attention_forward(mk(1, 8, 4, 136), mk(1, 8, 2, 136), mk(1, 8, 2, 136)),
+        lambda: attention_forward(mk(1, 8, 4, 60), mk(1, 8, 2, 60), mk(1, 8, 2, 60)),
+        lambda: attention_forward(q.cpu(), k, k),
+        lambda: attention_forward(q, k.cpu(), k),
+        lambda: attention_forward(q, mk(1, 8, 1, 64).expand(1, 8, 2, 64), k),      # expanded heads
+        lambda: attention_forward(mk(1, 8, 4, 65)[..., 1:], k, k),                 # strides and start off the boundary
+        lambda: attention_forward(mk(1, 8, 64, 4).transpose(2, 3), k, k),          # columns not contiguous
+        lambda: attention_forward(q, k, k, scale=0.0),
+        lambda: attention_forward(q, k, k, scale=-1.0),
+        lambda: attention_forward(q, k, k, scale=math.nan),
+        lambda: attention_forward(q, k, k, cu_seqlens_q=cu),                       # packed wants [rows, heads, dim]
+        lambda: attention_forward(q[0], k[0], k[0]),                               # not packed wants a batch
+        lambda: attention_forward(q[0], k[0], k[0], cu_seqlens_q=cu.long()),
+        lambda: attention_forward(q[0], k[0], k[0], cu_seqlens_q=cu.cpu()),
+        lambda: attention_forward(q[0], k[0], k[0], cu_seqlens_q=cu[:1]),
+        lambda: attention_forward(q[0], mk(9, 2, 64), mk(9, 2, 64), cu_seqlens_q=cu),
+        lambda: attention_forward(q[0], k[0], k[0], cu_seqlens_k=cu),
+        lambda: attention_forward(q[0], k[0], k[0], cu_seqlens_q=cu, cu_seqlens_k=torch.zeros(3, dtype=torch.int32, device=DEV)),
+        lambda: attention_forward(q, k, k, out=mk(1, 8, 4, 32)),
+        lambda: attention_forward(q, k, k, out=q),
+        lambda: attention_forward(q, k, k, out=mk(1, 8, 1, 64).expand(1, 8, 4, 64)),
+    ]
+    lse = torch.zeros(1, 4, 8, device=DEV)
+    bad += [
+        lambda: attention_backward(q, q, k, k, q, lse[:, :, :7]),
+        lambda: attention_backward(q, q, k, k, q, lse.double()),
+        lambda: attention_backward(q[:, :, :2], q, k, k, q, lse),
+        lambda: attention_backward(q, q, k, k, q, lse, dq=torch.empty_like(q)),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(RuntimeError):
+            call()
+            pytest.fail(f"call {i} was taken")

@@ -548,3 +548,118 @@ def test_engine_fused_kernels_match_autograd_at_width_1024(fused_gelu_gemm, over
             gr, rf = got[name].float(), ref.grad
             err = (gr - rf).norm() / (rf.norm() + 1e-12)
             assert err < 6e-2, f"unit {u.name} grad {name}: relative error {float(err):.3e}"
+
+
+# ---------------------------------------------------------------- native attention, query/key norms with rotation, 8-bit moments
+def _plain_step(cfg, params, tokens, targets, docs=None):
+    """Loss and gradients of the model in 64 bits, by autograd; ``docs``: which document each token belongs to, and its place."""
+    P = [{k: v.double().requires_grad_() for k, v in u.items()} for u in params]
+    B, S = tokens.shape
+    d, H, dh = cfg.d_model, cfg.n_head, cfg.head_dim
+    F = torch.nn.functional
+    x = F.embedding(tokens, P[0]["wte"])
+    if not cfg.qk_norm_rope:
+        x = x + P[0]["wpe"][:S]
+    i = torch.arange(S, device=DEV)
+    see, place = (i[None] <= i[:, None]).expand(B, S, S), i.expand(B, S)
+    if docs is not None:
+        which, place = docs
+        x = x.reshape(1, B * S, d)
+        i = torch.arange(B * S, device=DEV)
+        see, place = ((i[None] <= i[:, None]) & (which[:, None] == which[None]))[None], place[None]
+    ang = place.double()[..., None] * 10000.0 ** (-torch.arange(0, dh, 2, dtype=torch.float64, device=DEV) / dh)
+
+    def turn(t, w):
+        t = t * (t.square().mean(-1, keepdim=True) + cfg.qk_eps).rsqrt() * w
+        a, b = t[..., :dh // 2], t[..., dh // 2:]
+        c, s = ang.cos()[:, :, None], ang.sin()[:, :, None]
+        return torch.cat((a * c - b * s, b * c + a * s), -1)
+
+    for p in P[1:]:
+        h = F.layer_norm(x, (d,), p["ln1_w"], p["ln1_b"], cfg.ln_eps)
+        q, k, v = (h @ p["qkv_w"].t() + p["qkv_b"]).view(*h.shape[:2], 3, H, dh).unbind(2)
+        if cfg.qk_norm_rope:
+            q, k = turn(q, p["qn_w"]), turn(k, p["kn_w"])
+        s = torch.einsum("bihd,bjhd->bhij", q, k) / math.sqrt(dh)
+        a = torch.softmax(s.masked_fill(~see[:, None], -math.inf), -1)
+        o = torch.einsum("bhij,bjhd->bihd", a, v).reshape(h.shape)
+        x = x + o @ p["proj_w"].t() + p["proj_b"]
+        h = F.layer_norm(x, (d,), p["ln2_w"], p["ln2_b"], cfg.ln_eps)
+        x = x + F.gelu(h @ p["fc1_w"].t() + p["fc1_b"], approximate="tanh") @ p["fc2_w"].t() + p["fc2_b"]
+    x = F.layer_norm(x, (d,), P[0]["lnf_w"], P[0]["lnf_b"], cfg.ln_eps)
+    loss = F.cross_entropy((x @ P[0]["wte"].t()).view(-1, cfg.vocab), targets.reshape(-1))
+    loss.backward()
+    return loss.detach(), [{k: v.grad for k, v in u.items()} for u in P]
+
+
+@pytest.mark.parametrize("what", ["native", "rope", "rope_native", "packed"])
+def test_engine_gradients_with_native_attention(what):
+    """Every gradient of a step against the model in 64 bits.  The engine keeps activations in bf16, so that is what bounds
+    it: per product the operands are off by half a step (2^-8), about a dozen roundings one after the other through the two
+    blocks and back, which add up in squares: 2^-8 * sqrt(2 * 12) = 1.9 %, with as much again for the softmax's slope."""
+    from pccl.models.gpt import GPTConfig
+    from pccl.parallel.backend import TorchBackend
+    from pccl.parallel.zero3 import OptimConfig, Zero3Engine
+
+    rope = what != "native"
+    cfg = GPTConfig(2, 256, 4, 512, vocab=512, seq_len=160, init_std=0.08, qk_norm_rope=rope)
+    eng = Zero3Engine(cfg, TorchBackend(), OptimConfig(lr=0.0, max_grad_norm=0.0), native_gemm=True, native_attention=what != "rope")
+    g = torch.Generator(device=DEV).manual_seed(3)
+    tok = torch.randint(0, cfg.vocab, (2, 161), device=DEV, generator=g)
+    cu = docs = None
+    if what == "packed":
+        cu = torch.tensor([0, 1, 100, 230, 320], dtype=torch.int32, device=DEV)
+        i = torch.arange(320, device=DEV)
+        which = (i[:, None] >= cu[None, 1:]).sum(1)
+        docs = (which, i - cu.long()[which])
+    params = [{k: v.clone() for k, v in u[0].items()} for u in eng.pviews]
+    assert ("qn_w" in params[1]) == rope and ("wpe" in params[0]) != rope
+    loss = eng.train_step(tok[:, :-1], tok[:, 1:], cu) if cu is not None else eng.train_step(tok[:, :-1], tok[:, 1:])
+    eng.check_errors()
+    want, grads = _plain_step(cfg, params, tok[:, :-1], tok[:, 1:], docs)
+    assert abs(float(loss) - float(want)) <= 2e-2 * float(want)
+    for gv, ref in zip([eng.gviews0] + [u[0] for u in eng.gviews[1:]], grads):
+        for name, r in ref.items():
+            rel = float((gv[name].double() - r).norm() / r.norm().clamp(min=1e-12))
+            # the key bias moves all of a query's scores alike: without the norm its true gradient is zero
+            if name == "qkv_b" and not rope:
+                d = cfg.d_model
+                keep = torch.cat((torch.arange(d), torch.arange(2 * d, 3 * d))).to(DEV)
+                rel = float((gv[name].double() - r)[keep].norm() / r[keep].norm())
+            assert rel <= 0.04, (name, rel)
+
+
+def test_engine_with_8_bit_moments_steps_and_resumes():
+    """The run of all of it: rotation, native attention, 8-bit moments, clipping, a checkpoint in the middle."""
+    from pccl.models.gpt import GPTConfig
+    from pccl.parallel.backend import TorchBackend
+    from pccl.parallel.zero3 import OptimConfig, Zero3Engine
+
+    cfg = GPTConfig(2, 256, 4, 512, vocab=512, seq_len=128, qk_norm_rope=True)
+    mk = lambda **kw: Zero3Engine(cfg, TorchBackend(), OptimConfig(lr=1e-3), native_gemm=True, native_attention=True, **kw)     # noqa: E731
+    a, full = mk(optim_bits=8), mk()
+    g = torch.Generator(device=DEV).manual_seed(4)
+    toks = [torch.randint(0, cfg.vocab, (2, 129), device=DEV, generator=g) for _ in range(4)]
+    for t in toks[:2]:
+        a.train_step(t[:, :-1], t[:, 1:])
+        full.train_step(t[:, :-1], t[:, 1:])
+    # the first step of both is the same; later ones differ by the rounding of the moments only.  A parameter moves by at
+    # most lr / (1 - beta1) or so each step
+    assert float((a.master - full.master).abs().max()) <= 4 * 1e-3
+    sd = {k: v.clone() for k, v in a.state_dict().items()}
+    b = mk(optim_bits=8)
+    b.load_state_dict(sd)
+    for t in toks[2:]:
+        la, lb = a.train_step(t[:, :-1], t[:, 1:]), b.train_step(t[:, :-1], t[:, 1:])
+        assert torch.isfinite(la).all() and torch.allclose(la, lb, rtol=1e-4)
+    a.check_errors()
+    assert a.adam8.bits == 8 and a.exp_avg is None and a.launches > 0
+    with pytest.raises(ValueError):
+        full.load_state_dict(sd)
+    with pytest.raises(ValueError):
+        a.load_state_dict(full.state_dict())
+    with pytest.raises(ValueError):
+        mk(optim_bits=16)
+    with pytest.raises(ValueError):
+        Zero3Engine(GPTConfig(1, 256, 4, 512, vocab=512, seq_len=128), TorchBackend()).train_step(
+            toks[0][:, :-1], toks[0][:, 1:], torch.tensor([0, 256], dtype=torch.int32, device=DEV))
