@@ -28,6 +28,7 @@
 #include <stdint.h>
 #include <string.h>
 
+#include "act.cuh"
 #include "adamw_multi.h"
 #include "pdl.cuh"
 
@@ -117,67 +118,116 @@ __device__ __forceinline__ void store1(void* base, int64_t i, float x) {
   else static_cast<__half*>(base)[i] = __float2half_rn(x);
 }
 
+__device__ __forceinline__ void unpair(const F2* a, float* f) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) split(a[i], f[2 * i], f[2 * i + 1]);
+}
+
 // ---- codes
 constexpr float kSigned = 16129.f, kUnsigned = 4228250625.f;      // 127^2, 255^4 (rounded to 32 bits)
 constexpr float kSignedUnit = (float)(1.0 / 16129.0), kUnsignedUnit = (float)(1.0 / 4228250625.0);
 constexpr float kLeast = 8.271806125530277e-25f;                  // 2^-80
 
+// Four codes as fp32, two and two: the byte becomes the last mantissa byte of 2^23 + c, which is exact (conversions between
+// integers and floats run at a quarter of the rate of additions).
 template <bool SIGNED>
-__device__ __forceinline__ float power(float c) {
-  const float c2 = __fmul_rn(c, c);
-  return SIGNED ? c2 : __fmul_rn(c2, c2);
+__device__ __forceinline__ void codes4(uint32_t w, F2& a, F2& b) {
+  if constexpr (SIGNED) w ^= 0x80808080u;                       // c + 128
+  const F2 off = f2(SIGNED ? -8388736.f : -8388608.f);
+  a = f2(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7540)), __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7541))) + off;
+  b = f2(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7542)), __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7543))) + off;
 }
 template <bool SIGNED>
-__device__ __forceinline__ float decode(uint32_t byte, float unit) {
+__device__ __forceinline__ F2 decode2(const F2& c, const F2& unit) {
   if constexpr (SIGNED) {
-    const float c = (float)(int)(int8_t)byte;
-    return __fmul_rn(unit, __fmul_rn(fabsf(c), c));
+    float x, y;
+    split(c, x, y);
+    return unit * (f2(fabsf(x), fabsf(y)) * c);
   } else {
-    return __fmul_rn(unit, power<false>((float)byte));
+    const F2 c2 = c * c;
+    return unit * (c2 * c2);
   }
 }
-// x: the value, inv: 1 / A (0: the block holds zeros), noise: 16 bits.
+// Eight values.
 template <bool SIGNED>
-__device__ __forceinline__ uint32_t encode(float x, float inv, uint32_t noise) {
-  constexpr float top = SIGNED ? 127.f : 255.f;
-  const float y = __fmul_rn(__fmul_rn(fabsf(x), inv), SIGNED ? kSigned : kUnsigned);
-  // the largest c with c^power <= y: the hardware's root, put right by one where it is off
+__device__ __forceinline__ void decode8(const uint2& w, float unit, F2* x) {
+  codes4<SIGNED>(w.x, x[0], x[1]);
+  codes4<SIGNED>(w.y, x[2], x[3]);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = decode2<SIGNED>(x[i], f2(unit));
+}
+template <bool SIGNED>
+__device__ __forceinline__ F2 power2(const F2& c) {
+  const F2 c2 = c * c;
+  return SIGNED ? c2 : c2 * c2;
+}
+__device__ __forceinline__ float root_hw(float x) {
   float r;
-  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(y));
-  if constexpr (!SIGNED) asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(r));
-  float c = fminf(floorf(r), top);
-  float lo = power<SIGNED>(c), hi = power<SIGNED>(c + 1.f);
-  if (hi <= y) {
-    c += 1.f;
-    lo = hi;
-    hi = power<SIGNED>(c + 1.f);
-  } else if (lo > y) {
-    c -= 1.f;
-    hi = lo;
-    lo = power<SIGNED>(c);
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// Codes of two values, as floats 2^23 + c (unsigned) or 1.5 * 2^23 + c (signed), whose last byte is the code.  inv: 1 / A (0: the
+// block holds zeros); u: noise in (0, 1).  c starts as the whole part of the hardware's root.  Where that is off by one, because
+// the root lies within 2^-16 of a whole number, the comparison moves it to the right neighbour all the same, but for noise
+// within 2^-16 of 0 or 1.
+template <bool SIGNED>
+__device__ __forceinline__ void encode2(const F2& x, const F2& inv, const F2& u, float& r0, float& r1) {
+  constexpr float top = SIGNED ? 127.f : 255.f;
+  float x0, x1, y0, y1;
+  split(x, x0, x1);
+  const F2 y = (f2(fabsf(x0), fabsf(x1)) * inv) * f2(SIGNED ? kSigned : kUnsigned);
+  split(y, y0, y1);
+  y0 = root_hw(y0);
+  y1 = root_hw(y1);
+  if constexpr (!SIGNED) {
+    y0 = root_hw(y0);
+    y1 = root_hw(y1);
   }
-  const float u = (float)noise * 0x1p-16f + 0x1p-17f;
-  if (__fmul_rn(u, __fsub_rn(hi, lo)) < __fsub_rn(y, lo)) c += 1.f;
-  c = fminf(c, top);
+  const F2 c = f2(__fadd_rz(y0, 8388608.f), __fadd_rz(y1, 8388608.f)) + f2(-8388608.f);
+  const F2 c1 = c + f2(1.f), lo = power2<SIGNED>(c);
+  const F2 minus = f2(-1.f);
+  const F2 step = u * fma2(lo, minus, power2<SIGNED>(c1)), part = fma2(lo, minus, y);     // times -1 is exact: a subtraction
+  float s0, s1, p0, p1, a0, a1, b0, b1;
+  split(step, s0, s1);
+  split(part, p0, p1);
+  split(c, a0, a1);
+  split(c1, b0, b1);
+  a0 = fminf(s0 < p0 ? b0 : a0, top);
+  a1 = fminf(s1 < p1 ? b1 : a1, top);
   if constexpr (SIGNED) {
-    const int i = (int)c;
-    return (uint32_t)(x < 0.f ? -i : i) & 0xffu;
+    r0 = copysignf(a0, x0) + 12582912.f;
+    r1 = copysignf(a1, x1) + 12582912.f;
   } else {
-    return (uint32_t)(x > 0.f && inv > 0.f ? fmaxf(c, 1.f) : c);
+    float i0, i1;
+    split(inv, i0, i1);                                          // both halves are the block's
+    r0 = (x0 > 0.f && i0 > 0.f ? fmaxf(a0, 1.f) : a0) + 8388608.f;
+    r1 = (x1 > 0.f && i0 > 0.f ? fmaxf(a1, 1.f) : a1) + 8388608.f;
   }
 }
+__device__ __forceinline__ uint32_t bytes4(float a, float b, float c, float d) {
+  const uint32_t lo = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0040), hi = __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0040);
+  return __byte_perm(lo, hi, 0x5410);
+}
+// 16 bits of noise n as (n + 1/2) / 2^16, exactly: the bits of 1 + that, less 1.
+__device__ __forceinline__ float noise_hi(uint32_t h) { return __uint_as_float(((h >> 9) & 0x007fff80u) | 0x3f800040u); }
+__device__ __forceinline__ float noise_lo(uint32_t h) { return __uint_as_float(((h << 7) & 0x007fff80u) | 0x3f800040u); }
+
 // The block's largest size: sizes are not negative, so their bits are in the order of their values, infinities and NaN on top.
-__device__ __forceinline__ float block_max(const float* x) {
+__device__ __forceinline__ float block_max(const F2* x) {
   uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(fabsf(x[i])));
+  for (int i = 0; i < 4; ++i) {
+    float a, b;
+    split(x[i], a, b);
+    m = max(m, max(__float_as_uint(fabsf(a)), __float_as_uint(fabsf(b))));
+  }
   m = __reduce_max_sync(0xffffffffu, m);
   const float f = __uint_as_float(m);
   return m >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : (f < kLeast ? 0.f : f);
 }
 
 template <int PT, int GT, bool BITS8, int MAX>
-__global__ void __launch_bounds__(kThreads) adamw_multi_kernel(const __grid_constant__ AdamMultiArgs a,
+__global__ void __launch_bounds__(kThreads, 4) adamw_multi_kernel(const __grid_constant__ AdamMultiArgs a,
                                                                const __grid_constant__ Table<MAX> table) {
   pdl_wait();
   pdl_trigger();
@@ -207,7 +257,8 @@ __global__ void __launch_bounds__(kThreads) adamw_multi_kernel(const __grid_cons
                           (PT == kAdamF32 ? 0u : reinterpret_cast<uintptr_t>(t.param) & 15u);
     const bool whole = bad == 0 && at - lane * 8 + kAdamBlock <= t.n;          // the same for the whole warp
     // ---- loads
-    float g[8], p[8], m[8], v[8];
+    float g[8], p[8];
+    F2 m[4], v[4];                                                             // pairs of neighbours
     float m_unit = 0.f, v_unit = 0.f;
     if (whole) {
       Raw8 rg, rp, rm, rv;
@@ -218,58 +269,79 @@ __global__ void __launch_bounds__(kThreads) adamw_multi_kernel(const __grid_cons
         const uint2 cv = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.v) + si));
         m_unit = __fmul_rn(a.m_scale[sblk], kSignedUnit);
         v_unit = __fmul_rn(a.v_scale[sblk], kUnsignedUnit);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          m[i] = decode<true>(((i < 4 ? cm.x : cm.y) >> (8 * (i & 3))) & 0xffu, m_unit);
-          v[i] = decode<false>(((i < 4 ? cv.x : cv.y) >> (8 * (i & 3))) & 0xffu, v_unit);
-        }
+        decode8<true>(cm, m_unit, m);
+        decode8<false>(cv, v_unit, v);
       } else {
         load8<kAdamF32>(a.m, (int64_t)si, rm);
         load8<kAdamF32>(a.v, (int64_t)si, rv);
-        widen<kAdamF32>(rm, m);
-        widen<kAdamF32>(rv, v);
+        float x[8], y[8];
+        widen<kAdamF32>(rm, x);
+        widen<kAdamF32>(rv, y);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          m[i] = f2(x[2 * i], x[2 * i + 1]);
+          v[i] = f2(y[2 * i], y[2 * i + 1]);
+        }
       }
       widen<GT>(rg, g);
       widen<kAdamF32>(rp, p);
     } else {
-      if constexpr (BITS8) {
-        m_unit = __fmul_rn(a.m_scale[sblk], kSignedUnit);
-        v_unit = __fmul_rn(a.v_scale[sblk], kUnsignedUnit);
-      }
+      float x[8], y[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const bool on = at + i < t.n;
         g[i] = on ? load1<GT>(t.grad, at + i) : 0.f;
         p[i] = on ? static_cast<const float*>(weights)[at + i] : 0.f;
-        if constexpr (BITS8) {
-          m[i] = on ? decode<true>(static_cast<const uint8_t*>(a.m)[si + i], m_unit) : 0.f;
-          v[i] = on ? decode<false>(static_cast<const uint8_t*>(a.v)[si + i], v_unit) : 0.f;
-        } else {
-          m[i] = on ? static_cast<const float*>(a.m)[si + i] : 0.f;
-          v[i] = on ? static_cast<const float*>(a.v)[si + i] : 0.f;
+        if constexpr (!BITS8) {
+          x[i] = on ? static_cast<const float*>(a.m)[si + i] : 0.f;
+          y[i] = on ? static_cast<const float*>(a.v)[si + i] : 0.f;
+        }
+      }
+      if constexpr (BITS8) {                                     // the state's blocks are whole: behind a tensor's end they hold zeros
+        m_unit = __fmul_rn(a.m_scale[sblk], kSignedUnit);
+        v_unit = __fmul_rn(a.v_scale[sblk], kUnsignedUnit);
+        decode8<true>(*reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.m) + si), m_unit, m);
+        decode8<false>(*reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.v) + si), v_unit, v);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          m[i] = f2(x[2 * i], x[2 * i + 1]);
+          v[i] = f2(y[2 * i], y[2 * i + 1]);
         }
       }
     }
     // ---- the step
-    const float keep = 1.f - a.lr * t.decay;
+    const F2 keep = f2(1.f - a.lr * t.decay);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float x = __fmul_rn(g[i], gs);
-      m[i] = __fadd_rn(__fmul_rn(a.beta1, m[i]), __fmul_rn(a.one_minus_beta1, x));
-      v[i] = __fadd_rn(__fmul_rn(a.beta2, v[i]), __fmul_rn(a.one_minus_beta2, __fmul_rn(x, x)));
-      p[i] = p[i] * keep - a.lr * (m[i] * a.bias1) / (sqrtf(v[i] * a.bias2) + a.eps);
+    for (int i = 0; i < 4; ++i) {
+      const F2 x = f2(g[2 * i], g[2 * i + 1]) * f2(gs);
+      m[i] = f2(a.beta1) * m[i] + f2(a.one_minus_beta1) * x;
+      v[i] = f2(a.beta2) * v[i] + f2(a.one_minus_beta2) * (x * x);
+      // the update's root and quotient are the hardware's (a few units in the last place of the update, not of the parameter)
+      float a0, a1;
+      split(v[i] * f2(a.bias2), a0, a1);
+      asm("sqrt.approx.f32 %0, %0;" : "+f"(a0));                 // v may be below 2^-126 where eps is 0
+      asm("sqrt.approx.f32 %0, %0;" : "+f"(a1));
+      split(f2(a0, a1) + f2(a.eps), a0, a1);
+      const F2 q = m[i] * f2(a.lr * a.bias1) * f2(rcp_hw(a0), rcp_hw(a1));
+      split(fma2(f2(p[2 * i], p[2 * i + 1]), keep, q * f2(-1.f)), p[2 * i], p[2 * i + 1]);
     }
     // ---- states
     uint32_t cm[2] = {0u, 0u}, cv[2] = {0u, 0u};
     if constexpr (BITS8) {
       const float am = block_max(m), av = block_max(v);
       const float im = am > 0.f ? __fdiv_rn(1.f, am) : 0.f, iv = av > 0.f ? __fdiv_rn(1.f, av) : 0.f;
+      const uint32_t base = (uint32_t)si + (uint32_t)(si >> 32) * 0x9E3779B1u + a.key;    // blocks do not straddle 2^32
+      float km[8], kv[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint64_t e = si + i;
-        const uint32_t noise = mix((uint32_t)e + (uint32_t)(e >> 32) * 0x9E3779B1u + a.key);
-        cm[i >> 2] |= encode<true>(m[i], im, noise >> 16) << (8 * (i & 3));
-        cv[i >> 2] |= encode<false>(v[i], iv, noise & 0xffffu) << (8 * (i & 3));
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t n0 = mix(base + 2 * i), n1 = mix(base + 2 * i + 1);
+        encode2<true>(m[i], f2(im), f2(noise_hi(n0), noise_hi(n1)) + f2(-1.f), km[2 * i], km[2 * i + 1]);
+        encode2<false>(v[i], f2(iv), f2(noise_lo(n0), noise_lo(n1)) + f2(-1.f), kv[2 * i], kv[2 * i + 1]);
+      }
+      for (int i = 0; i < 2; ++i) {
+        cm[i] = bytes4(km[4 * i], km[4 * i + 1], km[4 * i + 2], km[4 * i + 3]);
+        cv[i] = bytes4(kv[4 * i], kv[4 * i + 1], kv[4 * i + 2], kv[4 * i + 3]);
       }
       if (lane == 0) {
         a.m_scale[sblk] = am;
@@ -282,20 +354,26 @@ __global__ void __launch_bounds__(kThreads) adamw_multi_kernel(const __grid_cons
     // ---- stores
     if (whole) {
       if constexpr (!BITS8) {
-        store32(static_cast<float*>(a.m) + si, m);
-        store32(static_cast<float*>(a.v) + si, v);
+        float x[8], y[8];
+        unpair(m, x);
+        unpair(v, y);
+        store32(static_cast<float*>(a.m) + si, x);
+        store32(static_cast<float*>(a.v) + si, y);
       }
       store32(static_cast<float*>(weights) + at, p);
       if constexpr (PT != kAdamF32)
         *reinterpret_cast<uint4*>(static_cast<uint16_t*>(t.param) + at) =
             make_uint4(narrow2<PT>(p[0], p[1]), narrow2<PT>(p[2], p[3]), narrow2<PT>(p[4], p[5]), narrow2<PT>(p[6], p[7]));
     } else {
+      float x[8], y[8];
+      unpair(m, x);
+      unpair(v, y);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         if (at + i < t.n) {
           if constexpr (!BITS8) {
-            static_cast<float*>(a.m)[si + i] = m[i];
-            static_cast<float*>(a.v)[si + i] = v[i];
+            static_cast<float*>(a.m)[si + i] = x[i];
+            static_cast<float*>(a.v)[si + i] = y[i];
           }
           static_cast<float*>(weights)[at + i] = p[i];
           if constexpr (PT != kAdamF32) store1<PT>(t.param, at + i, p[i]);
@@ -314,12 +392,12 @@ __global__ void __launch_bounds__(kThreads) adamw_dequantize_kernel(const uint8_
   for (int64_t i = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * 8; i < n; i += stride) {
     const uint2 cm = *reinterpret_cast<const uint2*>(m + i), cv = *reinterpret_cast<const uint2*>(v + i);
     const float um = __fmul_rn(m_scale[i / kAdamBlock], kSignedUnit), uv = __fmul_rn(v_scale[i / kAdamBlock], kUnsignedUnit);
+    F2 p[4], q[4];
     float x[8], y[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      x[e] = decode<true>(((e < 4 ? cm.x : cm.y) >> (8 * (e & 3))) & 0xffu, um);
-      y[e] = decode<false>(((e < 4 ? cv.x : cv.y) >> (8 * (e & 3))) & 0xffu, uv);
-    }
+    decode8<true>(cm, um, p);
+    decode8<false>(cv, uv, q);
+    unpair(p, x);
+    unpair(q, y);
     store32(m_out + i, x);
     store32(v_out + i, y);
   }
@@ -330,7 +408,7 @@ cudaError_t launch(const AdamMultiArgs& a, const AdamTensor* tensors, int count,
   Table<MAX> table;
   memcpy(table.t, tensors, sizeof(AdamTensor) * (size_t)count);
   table.count = count;
-  const uint32_t need = (a.blocks + kThreads / 32 - 1) / (kThreads / 32), most = (uint32_t)sm_count * 8;
+  const uint32_t need = (a.blocks + kThreads / 32 - 1) / (kThreads / 32), most = (uint32_t)sm_count * 4;
   return launch_pdl(adamw_multi_kernel<PT, GT, BITS8, MAX>, dim3(need < most ? need : most), dim3(kThreads), 0, s, a, table);
 }
 template <int PT, int GT>

@@ -31,11 +31,12 @@ struct RotaryArgs {
   int half, interleaved;
   int B, S, D, H[2];
   int heads_per_item, chunks[2];   // a thread group works on so many heads of one row at a time
+  int q_blocks;                    // the first blocks work on queries, the others on keys
   float eps;
-  float* partial;                  // backward: rotary_blocks(...) * 2 * D floats
+  float* partial;                  // backward: rotary_blocks(...) * D floats
 };
 
-// How the work is cut; sets heads_per_item and chunks, returns the number of blocks.
+// How the work is cut; sets heads_per_item, chunks and q_blocks, returns the number of blocks.
 int rotary_blocks(RotaryArgs& a, bool backward, int sm_count);
 cudaError_t launch_rotary_forward(const RotaryArgs& a, int blocks, cudaStream_t s);
 cudaError_t launch_rotary_backward(const RotaryArgs& a, int blocks, cudaStream_t s);

@@ -144,7 +144,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> qk_norm_rope_backward
     return {qo, ko, dqw, dkw};
   }
   const int blocks = rotary_blocks(a, true, at::cuda::getCurrentDeviceProperties()->multiProcessorCount);
-  at::Tensor partial = at::empty({(int64_t)blocks * 2 * s.D}, q.options().dtype(at::kFloat));
+  at::Tensor partial = at::empty({(int64_t)blocks * s.D}, q.options().dtype(at::kFloat));
   a.partial = partial.data_ptr<float>();
   PCCL_CUDA(launch_rotary_backward(a, blocks, at::cuda::getCurrentCUDAStream().stream()));
   return {qo, ko, dqw, dkw};
