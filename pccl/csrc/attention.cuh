@@ -112,20 +112,23 @@ __device__ __forceinline__ void commit(uint64_t* bar) {
 // d[128, 128] = a b^T, both tiles contracted along their DP columns.
 template <int DP>
 __device__ __forceinline__ void mma_columns(uint32_t d, uint32_t a_addr, uint32_t b_addr, uint32_t id) {
-  const uint32_t a = desc_k(a_addr), b = desc_k(b_addr);
+  uint32_t a = desc_k(a_addr), b = desc_k(b_addr);
+  asm volatile("" : "+r"(a), "+r"(b));                       // the steps' descriptors are formed here, not kept in registers over the loop
 #pragma unroll
   for (int k = 0; k < DP / 16; ++k) {
     const uint32_t off = (k >> 2) * (kBlockBytes >> 4) + (k & 3) * (32 >> 4);
     mma_ss(d, a + off, b + off, id, k > 0 ? 1u : 0u);
   }
 }
-// d[128, DP] (+)= a b, a: 128 x 128 of 16 bits in tensor memory, b: a tile contracted along its 128 rows.  The 64 columns of
-// a's first half start at a0, those of the second at a1.
+// d[128, DP] (+)= a b, a: 128 x 128 of 16 bits in tensor memory, b: a tile contracted along its 128 rows, in steps of 16 of
+// which this takes [FROM, TO).  The columns of a's first four steps start at a0, those of the last four at a1.
+template <int FROM, int TO>
 __device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a0, uint32_t a1, uint32_t b_addr, uint32_t id, bool accumulate) {
-  const uint32_t b = desc_mn(b_addr);
+  uint32_t b = desc_mn(b_addr);
+  asm volatile("" : "+r"(a0), "+r"(a1), "+r"(b));
 #pragma unroll
-  for (int k = 0; k < 8; ++k)
-    mma_ts(d, (k < 4 ? a0 : a1) + (k & 3) * 8, b + k * (2048 >> 4), id, (accumulate || k > 0) ? 1u : 0u);
+  for (int k = FROM; k < TO; ++k)
+    mma_ts(d, (k < 4 ? a0 : a1) + (k & 3) * 8, b + k * (2048 >> 4), id, (accumulate || k > FROM) ? 1u : 0u);
 }
 
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
@@ -188,6 +191,35 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return r;
 }
 
+// ---- work that is taken over at run time.  A grid has one CTA per tile; a CTA that is done with its tile takes the place of one
+// that has not started yet (cluster launch control), so that loads of its next tile overlap the end of the last and
+// the hardware's order of CTAs, which is the order in which tiles are listed, is kept.
+struct alignas(16) Handle {
+  uint32_t w[4];
+};
+__device__ __forceinline__ void ask_for_work(Handle* slot, uint64_t* bar) {
+  mbar_expect_tx(bar, 16);
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(smem_u32(slot)),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+// The number of the CTA whose place was taken, or -1: there is none left.
+__device__ __forceinline__ int work_taken(const Handle* slot) {
+  int taken, x;
+  asm volatile(
+      "{\n\t.reg .b128 h;\n\t.reg .pred p;\n\t"
+      "ld.shared.b128 h, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+      "selp.s32 %0, 1, 0, p;\n\t"
+      "mov.s32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n\t}"
+      : "=r"(taken), "=r"(x)
+      : "r"(smem_u32(slot))
+      : "memory");
+  fence_proxy_async_smem();              // the slot is written again through the other proxy
+  return taken ? x : -1;
+}
+
 // ---- which rows a CTA works on.  Packed sequences are cut into tiles of `rows` each on its own; tile numbers run through
 // them in order.  The starts are clamped into [0, limit], so that starts that are out of order or out of range make tiles
 // fewer, shorter or equal, never out of range.
@@ -242,30 +274,39 @@ __device__ __forceinline__ Span find_span(const AttnArgs& a, int t, int rows, bo
   return sp;
 }
 
-// Rows [first, min(first + rows, limit)) of one head to zero, by the whole CTA.
-__device__ __forceinline__ void zero_rows(const AttnTensor& t, int head, int first, int rows, int limit, int D) {
+// Rows [first, min(first + rows, limit)) of one head to zero, by `threads` threads.
+__device__ __forceinline__ void zero_rows(const AttnTensor& t, int head, int first, int rows, int limit, int D, int tid, int threads) {
   const int n = limit - first < rows ? limit - first : rows;
   const int vecs = D >> 3;
-  for (int i = threadIdx.x; i < n * vecs; i += blockDim.x) {
+  for (int i = tid; i < n * vecs; i += threads) {
     const int r = i / vecs, c = i - r * vecs;
     *reinterpret_cast<uint4*>(reinterpret_cast<char*>(const_cast<void*>(t.p)) +
                               2 * ((int64_t)(first + r) * t.ss + (int64_t)head * t.sh + c * 8)) = make_uint4(0, 0, 0, 0);
   }
 }
 
-// 32 accumulator columns of one row, times f, as 16-bit elements; only columns below D exist.
+// 32 accumulator columns of one row, times f, as 16-bit elements; only columns below D exist.  wide: the row starts on a
+// 32-byte boundary, and a store of 32 bytes writes one whole sector.
 template <bool BF16>
-__device__ __forceinline__ void store32(uint16_t* row, int col0, int D, const uint32_t* r, float f) {
+__device__ __forceinline__ void store32(uint16_t* row, int col0, int D, const uint32_t* r, float f, bool wide) {
 #pragma unroll
-  for (int v = 0; v < 4; ++v) {
-    if (col0 + v * 8 < D) {
-      uint32_t w[4];
+  for (int v = 0; v < 2; ++v) {
+    uint32_t w[8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        w[e] = pack2<BF16>(__uint_as_float(r[v * 8 + 2 * e]) * f, __uint_as_float(r[v * 8 + 2 * e + 1]) * f);
-      *reinterpret_cast<uint4*>(row + col0 + v * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+    for (int e = 0; e < 8; ++e) w[e] = pack2<BF16>(__uint_as_float(r[v * 16 + 2 * e]) * f, __uint_as_float(r[v * 16 + 2 * e + 1]) * f);
+    const int col = col0 + v * 16;
+    if (wide && col + 16 <= D) {
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(row + col), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+                   "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                   : "memory");
+    } else {
+      if (col < D) *reinterpret_cast<uint4*>(row + col) = make_uint4(w[0], w[1], w[2], w[3]);
+      if (col + 8 < D) *reinterpret_cast<uint4*>(row + col + 8) = make_uint4(w[4], w[5], w[6], w[7]);
     }
   }
+}
+__device__ __forceinline__ bool rows_are_wide(const AttnTensor& t) {
+  return ((reinterpret_cast<uintptr_t>(t.p) | (uintptr_t)(t.sb * 2) | (uintptr_t)(t.ss * 2) | (uintptr_t)(t.sh * 2)) & 31u) == 0;
 }
 __device__ __forceinline__ uint16_t* row_ptr(const AttnTensor& t, int batch, int head, int row) {
   return reinterpret_cast<uint16_t*>(const_cast<void*>(t.p)) + (int64_t)batch * t.sb + (int64_t)row * t.ss + (int64_t)head * t.sh;

@@ -96,8 +96,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     sp = find_span(a, (int)(blockIdx.x / (unsigned)a.Hk), 128, true);
     if (sp.tile < 0) {
       if (a.zero_tail) {
-        zero_rows(a.dk, kv_head, sp.first_k, 128, a.Sk, a.D);
-        zero_rows(a.dv, kv_head, sp.first_k, 128, a.Sk, a.D);
+        zero_rows(a.dk, kv_head, sp.first_k, 128, a.Sk, a.D, threadIdx.x, kThreads);
+        zero_rows(a.dv, kv_head, sp.first_k, 128, a.Sk, a.D, threadIdx.x, kThreads);
       }
       return;
     }
@@ -215,12 +215,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int it = 0; it < total && ok; ++it) {
         if (!(ok = wait(&b.p_ready, it & 1u, abort_flag))) break;
         fence_after();
-        mma_rows(tmem + C::kDv, tmem + C::kS, tmem + C::kS + 64, at(do_ring, it), id_o, it > 0);
+        mma_rows<0, 8>(tmem + C::kDv, tmem + C::kS, tmem + C::kS + 64, at(do_ring, it), id_o, it > 0);
         commit(b.do_empty + it % C::kStages);
         if (it + 1 < total && !(ok = scores(it + 1))) break;
         if (!(ok = wait(&b.ds_ready, it & 1u, abort_flag))) break;
         fence_after();
-        mma_rows(tmem + C::kDk, tmem + C::kDp, tmem + C::kDp + 64, at(q_ring, it), id_o, it > 0);
+        mma_rows<0, 8>(tmem + C::kDk, tmem + C::kDp, tmem + C::kDp + 64, at(q_ring, it), id_o, it > 0);
         commit(b.q_empty + it % C::kStages);
         if (it + 1 < total) ok = dprobs(it + 1);
       }
@@ -351,7 +351,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int e = 0; e < 32; ++e) o[e] = 0;
         }
-        if (exists) store32<BF16>(out, c * 32, a.D, o, g == 0 ? 1.f : a.scale);
+        if (exists) store32<BF16>(out, c * 32, a.D, o, g == 0 ? 1.f : a.scale, rows_are_wide(g == 0 ? a.dv : a.dk));
       }
     }
   }
@@ -398,7 +398,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     head = (int)(blockIdx.x % (unsigned)a.H);
     sp = find_span(a, (int)(blockIdx.x / (unsigned)a.H), 128, false);
     if (sp.tile < 0) {
-      if (a.zero_tail) zero_rows(a.dq, head, sp.first_q, 128, a.Sq, a.D);
+      if (a.zero_tail) zero_rows(a.dq, head, sp.first_q, 128, a.Sq, a.D, threadIdx.x, kThreads);
       return;
     }
   } else {
@@ -517,7 +517,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!(ok = wait(b.ds_ready + (j & 1), (j >> 1) & 1u, abort_flag))) break;
         fence_after();
         const uint32_t ds = tmem + C::kS + (j & 1) * 128;
-        mma_rows(tmem + C::kDq, ds, ds + 64, k_ring + ((uint32_t)j % C::kK) * C::kTile, id_o, j > 0);
+        mma_rows<0, 8>(tmem + C::kDq, ds, ds + 64, k_ring + ((uint32_t)j % C::kK) * C::kTile, id_o, j > 0);
         commit(b.k_empty + j % C::kK);
         if (j + 2 < n) ok = scores(j + 2);
       }
@@ -621,7 +621,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int e = 0; e < 32; ++e) o[e] = 0;
         }
-        if (exists) store32<BF16>(out, col, a.D, o, a.scale);
+        if (exists) store32<BF16>(out, col, a.D, o, a.scale, rows_are_wide(a.dq));
       }
     }
   }

@@ -3,12 +3,21 @@
 //
 //   warps 0-3   softmax of queries 0-127: one query per thread, its 128 scores of a key tile in registers
 //   warps 4-7   the same for queries 128-255
-//   warp 8      TMA: the query tiles once, then key and value tiles into a ring
+//   warp 8      TMA: the query tiles, then key and value tiles into a ring; asks for the next tile of the grid
 //   warp 9      tensor memory; one thread issues the products
 // The products of one half run while the other half is in its softmax:
 //   S0(j)  S1(j) | P0(j) V -> O0, S0(j+1) | P1(j) V -> O1, S1(j+1) | ...
 // Tensor memory: S0, S1 (128 columns each, P over the first 64 of them), O0, O1 (DP columns each).  Products of one CTA run in
 // the order of issue, so S0(j+1) may be written over P0(j), and a finished S0(j+1) says that O0 holds the sum up to j.
+// P is handed over in two halves, so that its product begins while the other half is still in its exponentials.
+//
+// What bounds it.  With the softmax left out, the products alone run at 1373 TFLOP/s on 16 heads of 16384 causal (0.84 of the
+// measured rate: both operands of Q K^T come from shared memory, 128 bytes per cycle for 128 x 128 tiles); with it 1171.  The exponentials
+// are not the limit: without them the same call takes as long, and moving a quarter of them to the multiply-add units as a
+// polynomial made it slower (939 -> 997 us).  The chain product - maximum - exponentials - product is.
+// Shorter sequences pay for the start and the end of each tile: 4 x 2048 x 16 heads of 128 causal 86.6 us (794 TFLOP/s), 70 without
+// softmax.  The grid's tiles are taken over at run time (attention.cuh), so that the loads of the next tile overlap the end of
+// the last: 97.8 -> 87.1 us there; one CTA per tile and two passes over the scores in tensor memory: 105.
 //
 // The running maximum only follows the true one when it has fallen behind by a factor of 2^8: sums and products are then at
 // most 2^8 times larger than with the true maximum, far inside fp32 and inside the range of 16-bit probabilities, and O, which
@@ -22,8 +31,9 @@ namespace {
 
 using namespace attn;
 
-constexpr int kThreads = 320;
+constexpr int kThreads = 384;                   // warps 10 and 11 only complete the third warpgroup
 constexpr float kBehind = 8.f;                  // binary orders of magnitude that the running maximum may fall behind
+constexpr int kReaders = 10;                    // of the next tile's number: eight softmax warps, loads, products
 
 template <int DP>
 struct Fwd {
@@ -31,22 +41,56 @@ struct Fwd {
   static constexpr uint32_t kTile = (DP / 64) * kBlockBytes;
   static constexpr uint32_t kRing = 2 * kTile;
   static constexpr uint32_t kBars = kRing + kStages * kTile;
-  static constexpr uint32_t kSmem = kBars + 256 + 1024;     // barriers, slack for the alignment of the swizzled tiles
+  static constexpr uint32_t kSmem = kBars + 512 + 1024;     // barriers, slack for the alignment of the swizzled tiles
   static constexpr uint32_t kS = 0, kO = 256;               // tensor memory columns
   static constexpr uint32_t kCols = 512;
 };
 
 struct Bars {
-  uint64_t full[8], empty[8], q[2], s[2], p[2], o[2], fix, drain;
+  Handle next[2];
+  uint64_t next_full[2], next_empty[2];
+  uint64_t full[8], empty[8], q_full[2], q_empty[2], s[2], p0[2], p1[2], o_full[2], o_empty[2], fix, drain;
   uint32_t tmem;
   int abort;
 };
-static_assert(sizeof(Bars) <= 256, "the barriers' part of shared memory");
+static_assert(sizeof(Bars) <= 512, "the barriers' part of shared memory");
 
 // Scores from place `left` on become -inf.
 __device__ __forceinline__ void mask32(uint32_t* r, int left) {
 #pragma unroll
   for (int e = 0; e < 32; ++e) r[e] = e < left ? r[e] : 0xff800000u;
+}
+
+// The queries of one tile number, and how many key tiles each half of them sees.
+struct Work {
+  Span sp;
+  int head, row0, offset, n[2];
+};
+__device__ __forceinline__ Work work_at(const AttnArgs& a, unsigned id, int tiles) {
+  Work w;
+  if (a.cu_q != nullptr) {
+    w.head = (int)(id % (unsigned)a.H);
+    w.sp = find_span(a, (int)(id / (unsigned)a.H), 256, false);
+  } else {
+    // with a causal mask the last tiles have the most keys: they come first
+    const unsigned heads = (unsigned)(a.B * a.H), bh = id % heads, t = id / heads;
+    w.head = (int)(bh % (unsigned)a.H);
+    w.sp.batch = (int)(bh / (unsigned)a.H);
+    w.sp.first_q = w.sp.first_k = 0;
+    w.sp.len_q = a.Sq;
+    w.sp.len_k = a.Sk;
+    w.sp.tile = a.causal ? tiles - 1 - (int)t : (int)t;
+  }
+  w.row0 = w.sp.tile * 256;
+  w.offset = w.sp.len_k - w.sp.len_q;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int first = w.row0 + h * 128;
+    const int last = first + 127 < w.sp.len_q - 1 ? first + 127 : w.sp.len_q - 1;
+    const int keys = !a.causal ? w.sp.len_k : (last + w.offset + 1 < w.sp.len_k ? last + w.offset + 1 : w.sp.len_k);
+    w.n[h] = w.sp.tile >= 0 && first < w.sp.len_q && keys > 0 ? (keys + 127) / 128 : 0;
+  }
+  return w;
 }
 
 template <int DP, bool BF16>
@@ -60,51 +104,21 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* abort_flag = &b.abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  // ---- this CTA's queries.  With a causal mask the last tiles have the most keys: they come first.
-  Span sp;
-  int head;
-  if (a.cu_q != nullptr) {
-    head = (int)(blockIdx.x % (unsigned)a.H);
-    sp = find_span(a, (int)(blockIdx.x / (unsigned)a.H), 256, false);
-    if (sp.tile < 0) {                                       // behind the last sequence
-      if (a.zero_tail) {
-        zero_rows(a.o, head, sp.first_q, 256, a.Sq, a.D);
-        const int r = sp.first_q + (int)threadIdx.x;
-        if (threadIdx.x < 256 && r < a.Sq) a.lse[stat_row(a, 0, head) + r] = -INFINITY;
-      }
-      return;
-    }
-  } else {
-    const unsigned bh = blockIdx.x % (unsigned)(a.B * a.H), t = blockIdx.x / (unsigned)(a.B * a.H);
-    head = (int)(bh % (unsigned)a.H);
-    sp.batch = (int)(bh / (unsigned)a.H);
-    sp.first_q = sp.first_k = 0;
-    sp.len_q = a.Sq;
-    sp.len_k = a.Sk;
-    sp.tile = a.causal ? tiles - 1 - (int)t : (int)t;
-  }
-  const int kv_head = head / (a.H / a.Hk);
-  const int row0 = sp.tile * 256, offset = sp.len_k - sp.len_q;
-  int n[2];                                                  // key tiles that each half sees
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int first = row0 + h * 128;
-    const int last = first + 127 < sp.len_q - 1 ? first + 127 : sp.len_q - 1;
-    const int keys = !a.causal ? sp.len_k : (last + offset + 1 < sp.len_k ? last + offset + 1 : sp.len_k);
-    n[h] = first < sp.len_q && keys > 0 ? (keys + 127) / 128 : 0;
-  }
-  const int nmax = n[0] > n[1] ? n[0] : n[1];
-
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::kStages; ++i) {
       mbar_init(b.full + i, 1);
       mbar_init(b.empty + i, 1);
     }
     for (int h = 0; h < 2; ++h) {
-      mbar_init(b.q + h, 1);
+      mbar_init(b.next_full + h, 1);
+      mbar_init(b.next_empty + h, kReaders);
+      mbar_init(b.q_full + h, 1);
+      mbar_init(b.q_empty + h, 1);
       mbar_init(b.s + h, 1);
-      mbar_init(b.p + h, 4);
-      mbar_init(b.o + h, 1);
+      mbar_init(b.p0 + h, 4);
+      mbar_init(b.p1 + h, 4);
+      mbar_init(b.o_full + h, 1);
+      mbar_init(b.o_empty + h, 4);
     }
     mbar_init(&b.fix, 1);
     mbar_init(&b.drain, 1);
@@ -117,201 +131,290 @@ __global__ void __launch_bounds__(kThreads, 1)
   fence_after();
   const uint32_t tmem = b.tmem;
 
-  if (warp == 8) {
-    // ------------------------------------------------------------ loads
-    bool ok = true;
-    if (lane == 0) {
-      for (int h = 0; h < 2; ++h)
-        if (n[h] > 0) {
-          mbar_expect_tx(b.q + h, C::kTile);
-          load_tile<DP>(smem + h * C::kTile, &map_q, head, sp.first_q + row0 + h * 128, sp.batch, b.q + h);
+  // The tile after the k-th, for every role alike: -1 none, -2 a wait gave up.  Whole warps.
+  auto next_tile = [&](int k) {
+    if (!wait_warp(b.next_full + (k & 1), (k >> 1) & 1u, abort_flag)) return -2;
+    const int id = work_taken(b.next + (k & 1));
+    __syncwarp();
+    if (lane == 0) mbar_arrive(b.next_empty + (k & 1));
+    return id;
+  };
+
+  // Registers: 384 threads start with 168 each, 64,512 together.  A thread that holds 128 scores wants more, the issuing warps
+  // less: 256 x 224 + 128 x 56 = 64,512.
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 8) {
+      // ---------------------------------------------------------- loads, and the tiles to come
+      bool ok = true;
+      uint32_t it = 0, fixes = 0, q_count[2] = {0, 0};
+      int k = 0;
+      for (int id = (int)blockIdx.x;; ++k) {
+        if (k >= 2 && !wait_warp(b.next_empty + (k & 1), ((k >> 1) - 1) & 1u, abort_flag)) {
+          ok = false;
+          break;
         }
-    }
-    uint32_t it = 0;
-    for (; (int)it < 2 * nmax; ++it) {                       // K0, V0, K1, V1, ...
-      const uint32_t st = it % C::kStages, ph = (it / C::kStages) & 1u;
-      if (!wait_warp(b.empty + st, ph ^ 1u, abort_flag)) {
-        ok = false;
-        break;
+        if (lane == 0) ask_for_work(b.next + (k & 1), b.next_full + (k & 1));
+        const Work w = work_at(a, (unsigned)id, tiles);
+        const int kv_head = w.head / (a.H / a.Hk), nmax = w.n[0] > w.n[1] ? w.n[0] : w.n[1];
+        for (int i = 0; i < 2 * nmax && ok; ++i, ++it) {     // K0, V0, K1, V1, ...
+          const uint32_t st = it % C::kStages, ph = (it / C::kStages) & 1u;
+          if (!(ok = wait_warp(b.empty + st, ph ^ 1u, abort_flag))) break;
+          const int row = (i >> 1) * 128;
+          const bool value = (i & 1) != 0;
+          unsigned char* dst = smem + C::kRing + st * C::kTile;
+          // the rows behind a packed sequence are its neighbour's
+          const bool ragged = value && a.cu_q != nullptr && row + 128 > w.sp.len_k;
+          uint64_t* bar = ragged ? &b.fix : b.full + st;
+          if (lane == 0) {
+            mbar_expect_tx(bar, C::kTile);
+            load_tile<DP>(dst, value ? &map_v : &map_k, kv_head, w.sp.first_k + row, w.sp.batch, bar);
+          }
+          if (ragged) {
+            ok = wait_warp(&b.fix, fixes++ & 1u, abort_flag);
+            clear_rows<DP>(dst, w.sp.len_k - row);
+            if (lane == 0) mbar_arrive(b.full + st);
+          }
+          if (i == 0) {                                      // behind the first key tile: the queries of the last tile may still be in use
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if (w.n[h] == 0 || !ok) continue;
+              if (!(ok = wait_warp(b.q_empty + h, (q_count[h] & 1u) ^ 1u, abort_flag))) continue;
+              ++q_count[h];
+              if (lane == 0) {
+                mbar_expect_tx(b.q_full + h, C::kTile);
+                load_tile<DP>(smem + h * C::kTile, &map_q, w.head, w.sp.first_q + w.row0 + h * 128, w.sp.batch, b.q_full + h);
+              }
+            }
+          }
+        }
+        if (!ok) break;
+        id = next_tile(k);
+        if (id < 0) {
+          ok = id == -1;
+          break;
+        }
       }
-      const int j = (int)(it >> 1), row = j * 128;
-      const bool value = (it & 1u) != 0;
-      unsigned char* dst = smem + C::kRing + st * C::kTile;
-      // the rows behind a packed sequence are its neighbour's
-      const bool ragged = value && a.cu_q != nullptr && row + 128 > sp.len_k;
-      uint64_t* bar = ragged ? &b.fix : b.full + st;
-      if (lane == 0) {
-        mbar_expect_tx(bar, C::kTile);
-        load_tile<DP>(dst, value ? &map_v : &map_k, kv_head, sp.first_k + row, sp.batch, bar);
+      if (!ok) {
+        if (lane == 0) {
+          atomicCAS(a.error, 0, kErrLoad);
+          *abort_flag = 1;
+        }
+        for (int i = 0; i < 1000; ++i) __nanosleep(1000);    // which copies are on their way is not known: the time that they can take
       }
-      if (ragged) {                                          // at most once: the last tile of the sequence
-        if (!wait_warp(&b.fix, 0, abort_flag)) ok = false;
-        clear_rows<DP>(dst, sp.len_k - row);
-        if (lane == 0) mbar_arrive(b.full + st);
-      }
-    }
-    if (!ok && lane == 0) {
-      atomicCAS(a.error, 0, kErrLoad);
-      *abort_flag = 1;
-    }
-    // what was asked for has to land before the CTA leaves its shared memory
-    for (uint32_t m = it > (uint32_t)C::kStages ? it - C::kStages : 0; m < it; ++m)
-      mbar_wait(b.full + m % C::kStages, (m / C::kStages) & 1u, kWaitNs / C::kStages);
-    for (int h = 0; h < 2; ++h)
-      if (n[h] > 0) mbar_wait(b.q + h, 0, kWaitNs);
-  } else if (warp == 9) {
-    // ------------------------------------------------------------ products
-    if (lane == 0) {
+    } else if (warp == 9) {
+      // ---------------------------------------------------------- products
       constexpr uint32_t id_s = idesc(BF16, 128, false), id_o = idesc(BF16, DP, true);
       const uint32_t q_addr = smem_u32(smem), ring = smem_u32(smem + C::kRing);
       bool ok = true;
-      auto tile_at = [&](uint32_t it) { return ring + (it % C::kStages) * C::kTile; };
-      auto loaded = [&](uint32_t it) { return wait(b.full + it % C::kStages, (it / C::kStages) & 1u, abort_flag); };
-      auto scores = [&](int h, int j) {
-        mma_columns<DP>(tmem + C::kS + h * 128, q_addr + h * C::kTile, tile_at(2 * j), id_s);
-        commit(b.s + h);
-      };
-      if (nmax > 0) {
-        ok = loaded(0);
-        for (int h = 0; h < 2 && ok; ++h)
-          if (n[h] > 0) {
-            ok = wait(b.q + h, 0, abort_flag);
-            if (ok) scores(h, 0);
+      uint32_t it = 0, s_count[2] = {0, 0}, items[2] = {0, 0};     // ring position; tiles and work items of each half
+      int id = (int)blockIdx.x;
+      for (int k = 0;; ++k) {
+        const Work w = work_at(a, (unsigned)id, tiles);
+        const int nmax = w.n[0] > w.n[1] ? w.n[0] : w.n[1];
+        if (lane == 0 && nmax > 0) {
+          auto tile_at = [&](uint32_t i) { return ring + (i % C::kStages) * C::kTile; };
+          auto loaded = [&](uint32_t i) { return wait(b.full + i % C::kStages, (i / C::kStages) & 1u, abort_flag); };
+          auto scores = [&](int h, int j) {
+            mma_columns<DP>(tmem + C::kS + h * 128, q_addr + h * C::kTile, tile_at(it + 2 * j), id_s);
+            commit(b.s + h);
+            if (j + 1 == w.n[h]) commit(b.q_empty + h);      // the queries are not read again
+          };
+          ok = loaded(it);
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (ok && w.n[h] > 0) {
+              ok = wait(b.q_full + h, items[h] & 1u, abort_flag);
+              if (ok) scores(h, 0);
+            }
+          if (ok) commit(b.empty + it % C::kStages);
+          for (int j = 0; j < nmax && ok; ++j) {
+            if (!(ok = loaded(it + 2 * j + 1))) break;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if (!ok) break;
+              if (j < w.n[h]) {
+                // the last tile's sums have been read out of O before this one's are begun
+                if (j == 0 && !(ok = wait(b.o_empty + h, (items[h] & 1u) ^ 1u, abort_flag))) break;
+                const uint32_t ph = (s_count[h] + (uint32_t)j) & 1u, p = tmem + C::kS + h * 128, v = tile_at(it + 2 * j + 1);
+                if (!(ok = wait(b.p0 + h, ph, abort_flag))) break;
+                fence_after();
+                mma_rows<0, 4>(tmem + C::kO + h * 128, p, p + 32, v, id_o, j > 0);
+                if (!(ok = wait(b.p1 + h, ph, abort_flag))) break;
+                fence_after();
+                mma_rows<4, 8>(tmem + C::kO + h * 128, p, p + 32, v, id_o, true);
+                if (j + 1 == w.n[h]) commit(b.o_full + h);
+              }
+              if (h == 0 && j + 1 < nmax) ok = loaded(it + 2 * j + 2);
+              if (ok && j + 1 < w.n[h]) scores(h, j + 1);
+            }
+            if (!ok) break;
+            commit(b.empty + (it + 2 * j + 1) % C::kStages);
+            if (j + 1 < nmax) commit(b.empty + (it + 2 * j + 2) % C::kStages);
           }
-        if (ok) commit(b.empty + 0);
-      }
-      for (int j = 0; j < nmax && ok; ++j) {
-        ok = loaded(2 * j + 1);
-        for (int h = 0; h < 2 && ok; ++h) {
-          if (j < n[h]) {
-            if (!(ok = wait(b.p + h, j & 1u, abort_flag))) break;
-            fence_after();
-            const uint32_t p = tmem + C::kS + h * 128;
-            mma_rows(tmem + C::kO + h * 128, p, p + 32, tile_at(2 * j + 1), id_o, j > 0);
-            if (j + 1 == n[h]) commit(b.o + h);
-          }
-          if (h == 0 && j + 1 < nmax) ok = loaded(2 * j + 2);
-          if (ok && j + 1 < n[h]) scores(h, j + 1);
+          it += 2 * (uint32_t)nmax;
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (w.n[h] > 0) {
+              s_count[h] += (uint32_t)w.n[h];
+              ++items[h];
+            }
         }
-        if (!ok) break;
-        commit(b.empty + (2 * j + 1) % C::kStages);
-        if (j + 1 < nmax) commit(b.empty + (2 * j + 2) % C::kStages);
+        __syncwarp();
+        if (__any_sync(0xffffffffu, !ok)) {
+          ok = false;
+          break;
+        }
+        id = next_tile(k);
+        if (id < 0) {
+          ok = id == -1;
+          break;
+        }
       }
-      if (!ok) {
-        atomicCAS(a.error, 0, kErrMma);
-        *abort_flag = 1;
+      if (lane == 0) {
+        if (!ok) {
+          atomicCAS(a.error, 0, kErrMma);
+          *abort_flag = 1;
+        }
+        commit(&b.drain);
+        mbar_wait(&b.drain, 0, kWaitNs);
       }
-      commit(&b.drain);
-      mbar_wait(&b.drain, 0, kWaitNs);
+      __syncwarp();
     }
-    __syncwarp();
   } else {
     // ------------------------------------------------------------ softmax: thread = query
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     const int h = warp >> 2;
-    const int row = row0 + h * 128 + (warp & 3) * 32 + lane;          // within the sequence
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem + C::kS + h * 128 + lanes, t_o = tmem + C::kO + h * 128 + lanes;
     const float sl2 = a.scale * kLog2e;
     const float behind = kBehind / sl2;
-    const int keys = !a.causal ? sp.len_k : (row + offset + 1 < sp.len_k ? row + offset + 1 : sp.len_k);   // that this query sees
-    const int keys_all = __shfl_sync(0xffffffffu, keys, 0);           // that every query of the warp sees
-    float m = -INFINITY, l = 0.f;
     bool ok = true;
-    for (int j = 0; j < n[h]; ++j) {
-      if (!(ok = wait_warp(b.s + h, j & 1u, abort_flag))) break;
-      fence_after();
-      const bool masked = keys_all < (j + 1) * 128;
-      const int left = keys - j * 128;                                // keys of this tile that this query sees
-      uint32_t s[2][32];                                              // two quarters of the row, the next one on its way
-      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-      tmem_ld32(t_s, s[0]);
+    uint32_t s_count = 0, items = 0;
+    int id = (int)blockIdx.x;
+    for (int k = 0;; ++k) {
+      const Work w = work_at(a, (unsigned)id, tiles);
+      const int n = h == 0 ? w.n[0] : w.n[1];
+      const int row = w.row0 + h * 128 + (warp & 3) * 32 + lane;         // within the sequence
+      const int keys = !a.causal ? w.sp.len_k : (row + w.offset + 1 < w.sp.len_k ? row + w.offset + 1 : w.sp.len_k);   // that this query sees
+      const int keys_all = __shfl_sync(0xffffffffu, keys, 0);           // that every query of the warp sees
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < n; ++j, ++s_count) {
+        if (!(ok = wait_warp(b.s + h, s_count & 1u, abort_flag))) break;
+        fence_after();
+        uint32_t s[4][32];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        tmem_wait_ld(s[c & 1]);
-        tmem_ld32(t_s + ((c + 1) & 3) * 32, s[(c + 1) & 1]);          // behind the last quarter the first one again
-        uint32_t* r = s[c & 1];
-        if (masked) mask32(r, left - c * 32);
+        for (int c = 0; c < 4; ++c) tmem_ld32(t_s + c * 32, s[c]);
 #pragma unroll
-        for (int e = 0; e < 32; e += 8)
+        for (int c = 0; c < 4; ++c) tmem_wait_ld(s[c]);
+        const bool masked = keys_all < (j + 1) * 128;
+        if (masked) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) top[i] = fmaxf(fmaxf(top[i], __uint_as_float(r[e + i])), __uint_as_float(r[e + 4 + i]));
-      }
-      const float m_new = fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), m);
-      if (__any_sync(0xffffffffu, m_new > m + behind)) {
-        const float f = m_new == m ? 1.f : ex2_hw((m - m_new) * sl2);
-        m = m_new;
-        l *= f;
-        if (j > 0) {
+          for (int c = 0; c < 4; ++c) mask32(s[c], keys - j * 128 - c * 32);
+        }
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int c = 0; c < DP / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld32(t_o + c * 32, o);
-            tmem_wait_ld(o);
+        for (int c = 0; c < 4; ++c)
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-            tmem_st32(t_o + c * 32, o);
+          for (int e = 0; e < 32; e += 8)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top[i] = fmaxf(fmaxf(top[i], __uint_as_float(s[c][e + i])), __uint_as_float(s[c][e + 4 + i]));
+        const float m_new = fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), m);
+        if (__any_sync(0xffffffffu, m_new > m + behind)) {
+          const float f = m_new == m ? 1.f : ex2_hw((m - m_new) * sl2);
+          m = m_new;
+          l *= f;
+          if (j > 0) {
+#pragma unroll
+            for (int c = 0; c < DP / 32; ++c) {
+              uint32_t o[32];
+              tmem_ld32(t_o + c * 32, o);
+              tmem_wait_ld(o);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tmem_st32(t_o + c * 32, o);
+            }
           }
         }
-      }
-      const F2 scale2 = f2(sl2), base2 = f2(m == -INFINITY ? 0.f : -m * sl2);
-      F2 sum2[2] = {f2(0.f), f2(0.f)};
+        const F2 scale2 = f2(sl2), base2 = f2(m == -INFINITY ? 0.f : -m * sl2);
+        F2 sum2[2] = {f2(0.f), f2(0.f)};
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        tmem_wait_ld(s[c & 1]);
-        if (c < 3) tmem_ld32(t_s + (c + 1) * 32, s[(c + 1) & 1]);
-        uint32_t* r = s[c & 1];
-        if (masked) mask32(r, left - c * 32);
-        uint32_t w[16];
+        for (int c = 0; c < 4; ++c) {
+          uint32_t wd[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const F2 x = fma2(f2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), scale2, base2);
-          float x0, x1;
-          split(x, x0, x1);
-          x0 = ex2_hw(x0);
-          x1 = ex2_hw(x1);
-          sum2[e & 1] = sum2[e & 1] + f2(x0, x1);
-          w[e] = pack2<BF16>(x0, x1);
+          for (int e = 0; e < 16; ++e) {
+            const F2 x = fma2(f2(__uint_as_float(s[c][2 * e]), __uint_as_float(s[c][2 * e + 1])), scale2, base2);
+            float x0, x1;
+            split(x, x0, x1);
+            x0 = ex2_hw(x0);
+            x1 = ex2_hw(x1);
+            sum2[e & 1] = sum2[e & 1] + f2(x0, x1);
+            wd[e] = pack2<BF16>(x0, x1);
+          }
+          tmem_st16(t_s + c * 16, wd);
+          if (c == 1) {                                                // the product may begin with the first half
+            tmem_wait_st();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(b.p0 + h);
+          }
         }
-        tmem_st16(t_s + c * 16, w);
+        float a0, a1;
+        split(sum2[0] + sum2[1], a0, a1);
+        l += a0 + a1;
+        tmem_wait_st();
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(b.p1 + h);
       }
-      float a0, a1;
-      split(sum2[0] + sum2[1], a0, a1);
-      l += a0 + a1;
-      tmem_wait_st();
-      fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(b.p + h);
-    }
-    if (ok && n[h] > 0) {
-      ok = wait_warp(b.o + h, 0, abort_flag);
-      fence_after();
-    }
-    if (!ok) {
-      if (lane == 0) {
-        atomicCAS(a.error, 0, kErrCompute);
-        *abort_flag = 1;
+      if (ok && n > 0) {
+        ok = wait_warp(b.o_full + h, items & 1u, abort_flag);
+        ++items;
+        fence_after();
       }
-    } else {
-      const bool exists = row < sp.len_q;
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      uint16_t* out = row_ptr(a.o, sp.batch, head, sp.first_q + row);
+      if (!ok) break;
+      if (w.sp.tile < 0) {                                             // behind the last sequence
+        if (a.zero_tail) {
+          zero_rows(a.o, w.head, w.sp.first_q, 256, a.Sq, a.D, threadIdx.x, 256);
+          const int r = w.sp.first_q + (int)threadIdx.x;
+          if (r < a.Sq) a.lse[stat_row(a, 0, w.head) + r] = -INFINITY;
+        }
+      } else {
+        const bool exists = row < w.sp.len_q, wide = rows_are_wide(a.o);
+        const bool none = m == -INFINITY;                              // no key is seen
+        const float inv = none ? 0.f : 1.f / l;
+        uint16_t* out = row_ptr(a.o, w.sp.batch, w.head, w.sp.first_q + row);
 #pragma unroll
-      for (int c = 0; c < DP / 32; ++c) {
-        uint32_t o[32];
-        if (n[h] > 0) {
-          tmem_ld32(t_o + c * 32, o);
-          tmem_wait_ld(o);
-        } else {
+        for (int c = 0; c < DP / 32; ++c) {
+          uint32_t o[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) o[e] = 0;
-        }
-        if (l == 0.f) {
+          if (n > 0) {
+            tmem_ld32(t_o + c * 32, o);
+            tmem_wait_ld(o);
+            if (c == DP / 32 - 1) {                                    // O may be written again
+              fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(b.o_empty + h);
+            }
+          }
+          if (none) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = 0;
+            for (int e = 0; e < 32; ++e) o[e] = 0;
+          }
+          if (exists) store32<BF16>(out, c * 32, a.D, o, inv, wide);
         }
-        if (exists) store32<BF16>(out, c * 32, a.D, o, inv);
+        if (exists) a.lse[stat_row(a, w.sp.batch, w.head) + w.sp.first_q + row] = none ? -INFINITY : m * a.scale + logf(l);
       }
-      if (exists) a.lse[stat_row(a, sp.batch, head) + sp.first_q + row] = l == 0.f ? -INFINITY : m * a.scale + logf(l);
+      id = next_tile(k);
+      if (id < 0) {
+        ok = id == -1;
+        break;
+      }
+    }
+    if (!ok && lane == 0) {
+      atomicCAS(a.error, 0, kErrCompute);
+      *abort_flag = 1;
     }
   }
   fence_before();
