@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       } else {
         const bool exists = row < w.sp.len_q, wide = rows_are_wide(a.o);
-        const bool none = m == -INFINITY;                              // no key is seen
+        const bool none = l == 0.f;                                    // no key is seen (scores that are NaN leave l NaN)
         const float inv = none ? 0.f : 1.f / l;
         uint16_t* out = row_ptr(a.o, w.sp.batch, w.head, w.sp.first_q + row);
 #pragma unroll
