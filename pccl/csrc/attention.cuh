@@ -33,16 +33,17 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// Bounded wait that also gives up when another role has failed.
+// Bounded wait that also gives up when another role has failed.  The clock is first read after some polls: reading the
+// global timer takes longer than most waits here.
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const uint64_t t0 = global_timer_ns();
-  uint32_t it = 0;
-  for (;;) {
+  uint64_t t0 = 0;
+  for (uint32_t it = 0;; ++it) {
     if (mbar_try_wait(bar, parity)) return true;
-    if ((++it & 255u) == 0u) {
+    if ((it & 255u) == 255u) {
       if (*abort_flag != 0) return false;
-      if (global_timer_ns() - t0 > kWaitNs) return false;
+      const uint64_t now = global_timer_ns();
+      if (t0 == 0) t0 = now;
+      else if (now - t0 > kWaitNs) return false;
     }
   }
 }
@@ -105,6 +106,14 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint32_t b_l
       ::"r"(d), "r"(a_tmem), "r"(b_lo), "r"(id), "r"(accumulate), "r"(kDescHi)
       : "memory");
 }
+// True in one lane of a converged warp, the same one every time.  The issuing warp runs as a whole and only its products and commits
+// stand behind this: in a branch on the lane number every operand of every product is moved into the
+// uniform registers anew (128 x 16 x 16 products back to back: 57 against 42-46 cycles each).
+__device__ __forceinline__ bool elect() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(r));
+  return r != 0;
+}
 __device__ __forceinline__ void commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
@@ -112,8 +121,7 @@ __device__ __forceinline__ void commit(uint64_t* bar) {
 // d[128, 128] = a b^T, both tiles contracted along their DP columns.
 template <int DP>
 __device__ __forceinline__ void mma_columns(uint32_t d, uint32_t a_addr, uint32_t b_addr, uint32_t id) {
-  uint32_t a = desc_k(a_addr), b = desc_k(b_addr);
-  asm volatile("" : "+r"(a), "+r"(b));                       // the steps' descriptors are formed here, not kept in registers over the loop
+  const uint32_t a = desc_k(a_addr), b = desc_k(b_addr);
 #pragma unroll
   for (int k = 0; k < DP / 16; ++k) {
     const uint32_t off = (k >> 2) * (kBlockBytes >> 4) + (k & 3) * (32 >> 4);
@@ -121,14 +129,13 @@ __device__ __forceinline__ void mma_columns(uint32_t d, uint32_t a_addr, uint32_
   }
 }
 // d[128, DP] (+)= a b, a: 128 x 128 of 16 bits in tensor memory, b: a tile contracted along its 128 rows, in steps of 16 of
-// which this takes [FROM, TO).  The columns of a's first four steps start at a0, those of the last four at a1.
-template <int FROM, int TO>
-__device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a0, uint32_t a1, uint32_t b_addr, uint32_t id, bool accumulate) {
-  uint32_t b = desc_mn(b_addr);
-  asm volatile("" : "+r"(a0), "+r"(a1), "+r"(b));
+// which this takes [FROM, TO).  GROUP steps of a lie side by side (8 columns each), the next GROUP from STRIDE columns further on.
+template <int FROM, int TO, int GROUP, int STRIDE>
+__device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a, uint32_t b_addr, uint32_t id, bool accumulate) {
+  const uint32_t b = desc_mn(b_addr);
 #pragma unroll
   for (int k = FROM; k < TO; ++k)
-    mma_ts(d, (k < 4 ? a0 : a1) + (k & 3) * 8, b + k * (2048 >> 4), id, (accumulate || k > FROM) ? 1u : 0u);
+    mma_ts(d, a + (k / GROUP) * STRIDE + (k % GROUP) * 8, b + k * (2048 >> 4), id, (accumulate || k > FROM) ? 1u : 0u);
 }
 
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {

@@ -24,7 +24,9 @@ namespace {
 
 using namespace attn;
 
-constexpr int kThreads = 384;
+constexpr int kCompute = 8;                     // warps that make probabilities and score gradients, 512 / kCompute columns each
+constexpr int kCols = 512 / kCompute;
+constexpr int kThreads = kCompute * 32 + 128;
 
 // ---------------------------------------------------------------- row sums
 // delta_i = <do_i, o_i>: sixteen lanes per row.  One read of both tensors.
@@ -73,14 +75,17 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(const __grid_const
 // ---------------------------------------------------------------- dk, dv
 template <int DP>
 struct Dkv {
-  static constexpr int kStages = DP == 128 ? 2 : 4;          // of each of the two rings
+  // Stages of the two rings.  A query tile is last read by the fourth product of its step and wanted again by the first, two
+  // products later with two stages: less than a load takes.
+  static constexpr int kNq = DP == 128 ? 3 : 4, kNdo = DP == 128 ? 2 : 4;
   static constexpr uint32_t kTile = (DP / 64) * kBlockBytes;
-  static constexpr uint32_t kQ = 2 * kTile, kDo = kQ + kStages * kTile;
-  static constexpr uint32_t kStat = kDo + kStages * kTile;   // [2][lse, delta][128] floats
+  static constexpr uint32_t kQ = 2 * kTile, kDo = kQ + kNq * kTile;
+  static constexpr uint32_t kStat = kDo + kNdo * kTile;      // [2][lse, delta][128] floats
   static constexpr uint32_t kBars = kStat + 2 * 2 * 128 * 4;
-  static constexpr uint32_t kSmem = kBars + 512 + 1024;
+  static constexpr uint32_t kSmem = kBars + 512;              // 231,936 of 232,448: no room to move the base to a boundary
   static constexpr uint32_t kS = 0, kDp = 128, kDv = 256, kDk = 256 + DP;      // tensor memory columns
-  static constexpr int kReaders = 11;                        // of the next tile's number: warps 0-10
+  static constexpr int kOutWarps = kCompute;                 // that read the finished sums
+  static constexpr int kReaders = kCompute + 3;              // of the next tile's number: all warps but the last
 };
 struct DkvBars {
   Handle next[2];
@@ -128,17 +133,22 @@ __global__ void __launch_bounds__(kThreads, 1)
                          const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do,
                          const __grid_constant__ AttnArgs a) {
   using C = Dkv<DP>;
-  extern __shared__ unsigned char smem_raw[];
-  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  extern __shared__ __align__(1024) unsigned char smem[];   // the swizzled tiles want 1024 bytes; without static variables it starts there
+  if ((smem_u32(smem) & 1023u) != 0u) {
+    if (threadIdx.x == 0) atomicCAS(a.error, 0, kErrLoad);
+    return;
+  }
   DkvBars& b = *reinterpret_cast<DkvBars*>(smem + C::kBars);
   volatile int* abort_flag = &b.abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = a.H / a.Hk;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < C::kStages; ++i) {
+    for (int i = 0; i < C::kNq; ++i) {
       mbar_init(b.q_full + i, 1);
       mbar_init(b.q_empty + i, 1);
+    }
+    for (int i = 0; i < C::kNdo; ++i) {
       mbar_init(b.do_full + i, 1);
       mbar_init(b.do_empty + i, 1);
     }
@@ -146,7 +156,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(b.next_full + i, 1);
       mbar_init(b.next_empty + i, C::kReaders);
       mbar_init(b.stat_full + i, 1);
-      mbar_init(b.stat_empty + i, 8);
+      mbar_init(b.stat_empty + i, kCompute);
     }
     mbar_init(&b.k_full, 1);
     mbar_init(&b.k_empty, 1);
@@ -154,16 +164,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&b.v_empty, 1);
     mbar_init(&b.s, 1);
     mbar_init(&b.dp, 1);
-    mbar_init(&b.p_ready, 8);
-    mbar_init(&b.ds_ready, 8);
+    mbar_init(&b.p_ready, kCompute);
+    mbar_init(&b.ds_ready, kCompute);
     mbar_init(&b.out_full, 1);
-    mbar_init(&b.out_empty, 8);
+    mbar_init(&b.out_empty, C::kOutWarps);
     mbar_init(&b.fix, 1);
     mbar_init(&b.drain, 1);
     b.abort = 0;
     fence_mbar_init();
   }
-  if (warp == 9) tmem_alloc(&b.tmem, 512);
+  if (warp == kCompute + 1) tmem_alloc(&b.tmem, 512);
   fence_before();
   __syncthreads();
   fence_after();
@@ -184,10 +194,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   };
 
-  // 384 threads start with 168 registers each, 64,512 together: 256 x 224 + 128 x 56.
-  if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == 8) {
+  // 384 threads start with 168 registers each, 64,512 together: 256 x 208 + 128 x 88.
+  if (warp >= kCompute) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == kCompute) {
       // ---------------------------------------------------------- loads, and the tiles to come
       bool ok = true;
       uint32_t n = 0, items = 0, fixes = 0;                  // query tiles, key tiles so far
@@ -197,7 +207,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) ask_for_work(b.next + (k & 1), b.next_full + (k & 1));
         const DkvWork w = dkv_work_at(a, (unsigned)id);
         for (int i = 0; i < w.total && ok; ++i, ++n) {
-          const uint32_t st = n % C::kStages, ph = (n / C::kStages) & 1u;
           const int hg = i / w.per_head, head = w.kv_head * group + hg, row = (w.first + i - hg * w.per_head) * 128;
           // the rows behind a packed sequence are its neighbour's, and both tiles are contracted along their rows
           const bool ragged = a.cu_q != nullptr && row + 128 > w.sp.len_q;
@@ -211,6 +220,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 load_tile<DP>(smem + which * C::kTile, which == 0 ? &map_k : &map_v, w.kv_head, w.sp.first_k + w.key0, w.sp.batch, full);
               }
             }
+            const uint32_t stages = which == 0 ? C::kNq : C::kNdo, st = n % stages, ph = (n / stages) & 1u;
             uint64_t* full = (which == 0 ? b.q_full : b.do_full) + st;
             if (!(ok = wait_warp((which == 0 ? b.q_empty : b.do_empty) + st, ph ^ 1u, abort_flag))) break;
             unsigned char* dst = smem + (which == 0 ? C::kQ : C::kDo) + st * C::kTile;
@@ -236,7 +246,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         fail(kErrLoad);
         for (int i = 0; i < 1000; ++i) __nanosleep(1000);    // which copies are on their way is not known: the time that they can take
       }
-    } else if (warp == 9) {
+    } else if (warp == kCompute + 1) {
       // ---------------------------------------------------------- products
       constexpr uint32_t id_s = idesc(BF16, 128, false), id_o = idesc(BF16, DP, true);
       const uint32_t k_addr = smem_u32(smem), v_addr = k_addr + C::kTile;
@@ -246,61 +256,69 @@ __global__ void __launch_bounds__(kThreads, 1)
       int id = (int)blockIdx.x;
       for (int k = 0;; ++k) {
         const DkvWork w = dkv_work_at(a, (unsigned)id);
-        if (lane == 0 && w.total > 0) {
-          auto at = [&](uint32_t ring, uint32_t m) { return ring + (m % C::kStages) * C::kTile; };
+        if (w.total > 0) {
+          auto q_at = [&](uint32_t m) { return q_ring + (m % C::kNq) * C::kTile; };
+          auto do_at = [&](uint32_t m) { return do_ring + (m % C::kNdo) * C::kTile; };
           auto scores = [&](int i) {
             const uint32_t m = n + (uint32_t)i;
-            if (!wait(b.q_full + m % C::kStages, (m / C::kStages) & 1u, abort_flag)) return false;
-            mma_columns<DP>(tmem + C::kS, k_addr, at(q_ring, m), id_s);
-            commit(&b.s);
-            if (i + 1 == w.total) commit(&b.k_empty);
+            if (!wait_warp(b.q_full + m % C::kNq, (m / C::kNq) & 1u, abort_flag)) return false;
+            if (elect()) {
+              mma_columns<DP>(tmem + C::kS, k_addr, q_at(m), id_s);
+              commit(&b.s);
+              if (i + 1 == w.total) commit(&b.k_empty);
+            }
+            __syncwarp();
             return true;
           };
           auto dprobs = [&](int i) {
             const uint32_t m = n + (uint32_t)i;
-            if (!wait(b.do_full + m % C::kStages, (m / C::kStages) & 1u, abort_flag)) return false;
-            mma_columns<DP>(tmem + C::kDp, v_addr, at(do_ring, m), id_s);
-            commit(&b.dp);
-            if (i + 1 == w.total) commit(&b.v_empty);
+            if (!wait_warp(b.do_full + m % C::kNdo, (m / C::kNdo) & 1u, abort_flag)) return false;
+            if (elect()) {
+              mma_columns<DP>(tmem + C::kDp, v_addr, do_at(m), id_s);
+              commit(&b.dp);
+              if (i + 1 == w.total) commit(&b.v_empty);
+            }
+            __syncwarp();
             return true;
           };
-          ok = wait(&b.k_full, items & 1u, abort_flag) && scores(0) && wait(&b.v_full, items & 1u, abort_flag) && dprobs(0);
+          ok = wait_warp(&b.k_full, items & 1u, abort_flag) && scores(0) && wait_warp(&b.v_full, items & 1u, abort_flag) && dprobs(0);
           for (int i = 0; i < w.total && ok; ++i) {
             const uint32_t m = n + (uint32_t)i;
             // the last tile's sums have been read before this one's are begun
-            if (i == 0 && !(ok = wait(&b.out_empty, (items & 1u) ^ 1u, abort_flag))) break;
-            if (!(ok = wait(&b.p_ready, m & 1u, abort_flag))) break;
+            if (i == 0 && !(ok = wait_warp(&b.out_empty, (items & 1u) ^ 1u, abort_flag))) break;
+            if (!(ok = wait_warp(&b.p_ready, m & 1u, abort_flag))) break;
             fence_after();
-            mma_rows<0, 8>(tmem + C::kDv, tmem + C::kS, tmem + C::kS + 64, at(do_ring, m), id_o, i > 0);
-            commit(b.do_empty + m % C::kStages);
+            if (elect()) {
+              mma_rows<0, 8, kCols / 16, kCols>(tmem + C::kDv, tmem + C::kS, do_at(m), id_o, i > 0);
+              commit(b.do_empty + m % C::kNdo);
+            }
+            __syncwarp();
             if (i + 1 < w.total && !(ok = scores(i + 1))) break;
-            if (!(ok = wait(&b.ds_ready, m & 1u, abort_flag))) break;
+            if (!(ok = wait_warp(&b.ds_ready, m & 1u, abort_flag))) break;
             fence_after();
-            mma_rows<0, 8>(tmem + C::kDk, tmem + C::kDp, tmem + C::kDp + 64, at(q_ring, m), id_o, i > 0);
-            commit(b.q_empty + m % C::kStages);
+            if (elect()) {
+              mma_rows<0, 8, kCols / 16, kCols>(tmem + C::kDk, tmem + C::kDp, q_at(m), id_o, i > 0);
+              commit(b.q_empty + m % C::kNq);
+              if (i + 1 == w.total) commit(&b.out_full);
+            }
+            __syncwarp();
             if (i + 1 < w.total) ok = dprobs(i + 1);
           }
-          if (ok) commit(&b.out_full);
           n += (uint32_t)w.total;
           ++items;
         }
-        __syncwarp();
-        if (__any_sync(0xffffffffu, !ok)) {
-          ok = false;
-          break;
-        }
+        if (!ok) break;
         id = next_tile(k);
         ok = id != -2;
         if (id < 0) break;
       }
       if (!ok) fail(kErrMma);
-      if (lane == 0) {
-        commit(&b.drain);
-        mbar_wait(&b.drain, 0, kWaitNs);
-      }
       __syncwarp();
-    } else if (warp == 10) {
-      // ---------------------------------------------------------- statistics: lse in powers of two, delta.  Queries that do not
+      if (elect()) commit(&b.drain);
+      __syncwarp();
+      mbar_wait(&b.drain, 0, kWaitNs);
+    } else if (warp == kCompute + 2) {
+      // ---------------------------------------------------------- statistics: -lse in powers of two, -delta.  Queries that do not
       // exist or see no key get probabilities of zero.
       bool ok = true;
       uint32_t n = 0;
@@ -316,8 +334,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int r = row + e * 32 + lane;
             const bool exists = r < w.sp.len_q;
             const float l = exists ? a.lse[at + r] : -INFINITY;
-            x[e] = l == -INFINITY ? INFINITY : l * kLog2e;
-            y[e] = exists ? a.delta[at + r] : 0.f;
+            x[e] = l == -INFINITY ? -INFINITY : l * -kLog2e;
+            y[e] = exists ? -a.delta[at + r] : 0.f;
           }
           if (!(ok = wait_warp(b.stat_empty + (n & 1), ((n >> 1) & 1u) ^ 1u, abort_flag))) break;
           float* st = reinterpret_cast<float*>(smem + C::kStat) + (n & 1) * 256;
@@ -338,10 +356,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     // ------------------------------------------------------------ probabilities and score gradients: thread = key
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const int g = warp >> 2;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t t_s = tmem + C::kS + g * 64 + lanes, t_dp = tmem + C::kDp + g * 64 + lanes;
+    const uint32_t t_s = tmem + C::kS + g * kCols + lanes, t_dp = tmem + C::kDp + g * kCols + lanes;
     const F2 scale2 = f2(a.scale * kLog2e);
     bool ok = true;
     uint32_t n = 0, items = 0;
@@ -351,29 +369,29 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int key = w.key0 + (warp & 3) * 32 + lane;
       int tile = w.first;                                    // query tile within its head
       for (int i = 0; i < w.total; ++i, ++n) {
-        const float* st = reinterpret_cast<const float*>(smem + C::kStat) + (n & 1) * 256 + g * 64;
-        const int q0 = tile * 128 + g * 64;
+        const float* st = reinterpret_cast<const float*>(smem + C::kStat) + (n & 1) * 256 + g * kCols;
+        const int q0 = tile * 128 + g * kCols;
         if (++tile == w.first + w.per_head) tile = w.first;
         const int hidden = a.causal ? key - w.offset - q0 : 0;               // this key is not seen by the first so many queries
         const bool masked = a.causal && w.key0 + (warp & 3) * 32 + 31 - w.offset - q0 > 0;
         if (!(ok = wait_warp(b.stat_full + (n & 1), (n >> 1) & 1u, abort_flag))) break;
         if (!(ok = wait_warp(&b.s, n & 1u, abort_flag))) break;
         fence_after();
-        float p[64];
-        uint32_t s[2][32];
-        tmem_ld32(t_s, s[0]);
-        tmem_ld32(t_s + 32, s[1]);
-        tmem_wait_ld(s[0]);
-        tmem_wait_ld(s[1]);
+        float p[kCols];
+        uint32_t s[kCols / 32][32];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+        for (int c = 0; c < kCols / 32; ++c) tmem_ld32(t_s + c * 32, s[c]);
+#pragma unroll
+        for (int c = 0; c < kCols / 32; ++c) tmem_wait_ld(s[c]);
+#pragma unroll
+        for (int c = 0; c < kCols / 32; ++c) {
           uint32_t wd[16];
 #pragma unroll
           for (int e = 0; e < 16; e += 2) {
             const float4 base = *reinterpret_cast<const float4*>(st + c * 32 + 2 * e);
             float x[4];
-            split(fma2(f2(__uint_as_float(s[c][2 * e]), __uint_as_float(s[c][2 * e + 1])), scale2, f2(-base.x, -base.y)), x[0], x[1]);
-            split(fma2(f2(__uint_as_float(s[c][2 * e + 2]), __uint_as_float(s[c][2 * e + 3])), scale2, f2(-base.z, -base.w)), x[2], x[3]);
+            split(fma2(f2(__uint_as_float(s[c][2 * e]), __uint_as_float(s[c][2 * e + 1])), scale2, f2(base.x, base.y)), x[0], x[1]);
+            split(fma2(f2(__uint_as_float(s[c][2 * e + 2]), __uint_as_float(s[c][2 * e + 3])), scale2, f2(base.z, base.w)), x[2], x[3]);
 #pragma unroll
             for (int v = 0; v < 4; ++v) x[v] = ex2_hw(x[v]);
             if (masked) {
@@ -394,20 +412,20 @@ __global__ void __launch_bounds__(kThreads, 1)
 
         if (!(ok = wait_warp(&b.dp, n & 1u, abort_flag))) break;
         fence_after();
-        tmem_ld32(t_dp, s[0]);
-        tmem_ld32(t_dp + 32, s[1]);
-        tmem_wait_ld(s[0]);
-        tmem_wait_ld(s[1]);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+        for (int c = 0; c < kCols / 32; ++c) tmem_ld32(t_dp + c * 32, s[c]);
+#pragma unroll
+        for (int c = 0; c < kCols / 32; ++c) tmem_wait_ld(s[c]);
+#pragma unroll
+        for (int c = 0; c < kCols / 32; ++c) {
           uint32_t wd[16];
 #pragma unroll
           for (int e = 0; e < 16; e += 2) {
             const float4 d = *reinterpret_cast<const float4*>(st + 128 + c * 32 + 2 * e);
             const int i0 = c * 32 + 2 * e;
             float x[4];
-            split(f2(p[i0], p[i0 + 1]) * (f2(__uint_as_float(s[c][2 * e]), __uint_as_float(s[c][2 * e + 1])) + f2(-d.x, -d.y)), x[0], x[1]);
-            split(f2(p[i0 + 2], p[i0 + 3]) * (f2(__uint_as_float(s[c][2 * e + 2]), __uint_as_float(s[c][2 * e + 3])) + f2(-d.z, -d.w)), x[2],
+            split(f2(p[i0], p[i0 + 1]) * (f2(__uint_as_float(s[c][2 * e]), __uint_as_float(s[c][2 * e + 1])) + f2(d.x, d.y)), x[0], x[1]);
+            split(f2(p[i0 + 2], p[i0 + 3]) * (f2(__uint_as_float(s[c][2 * e + 2]), __uint_as_float(s[c][2 * e + 3])) + f2(d.z, d.w)), x[2],
                   x[3]);
             if (masked) {
 #pragma unroll
@@ -434,30 +452,33 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) break;
       if (w.sp.tile < 0) {
         if (a.zero_tail) {
-          zero_rows(a.dk, w.kv_head, w.sp.first_k, 128, a.Sk, a.D, threadIdx.x, 256);
-          zero_rows(a.dv, w.kv_head, w.sp.first_k, 128, a.Sk, a.D, threadIdx.x, 256);
+          zero_rows(a.dk, w.kv_head, w.sp.first_k, 128, a.Sk, a.D, threadIdx.x, kCompute * 32);
+          zero_rows(a.dv, w.kv_head, w.sp.first_k, 128, a.Sk, a.D, threadIdx.x, kCompute * 32);
         }
       } else {
-        // the first warpgroup writes dv, the second dk
-        const AttnTensor& dst = g == 0 ? a.dv : a.dk;
+        // the first half of the warps writes dv, the second dk, each warpgroup its share of the columns
+        constexpr int per = DP * 2 / (kCompute / 4);
+        const bool keys_grad = g >= kCompute / 8;
+        const AttnTensor& dst = keys_grad ? a.dk : a.dv;
+        const int col0 = (g % (kCompute / 8)) * per;
         const bool exists = key < w.sp.len_k, wide = rows_are_wide(dst);
         uint16_t* out = row_ptr(dst, w.sp.batch, w.kv_head, w.sp.first_k + key);
-        const uint32_t t_out = tmem + (g == 0 ? C::kDv : C::kDk) + lanes;
+        const uint32_t t_out = tmem + (keys_grad ? C::kDk : C::kDv) + lanes + col0;
 #pragma unroll
-        for (int c = 0; c < DP / 32; ++c) {
+        for (int c = 0; c < per / 32; ++c) {
           uint32_t o[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) o[e] = 0;
           if (w.total > 0) {
             tmem_ld32(t_out + c * 32, o);
             tmem_wait_ld(o);
-            if (c == DP / 32 - 1) {                          // the sums may be written again
+            if (c == per / 32 - 1) {                         // the sums may be written again
               fence_before();
               __syncwarp();
               if (lane == 0) mbar_arrive(&b.out_empty);
             }
           }
-          if (exists) store32<BF16>(out, c * 32, a.D, o, g == 0 ? 1.f : a.scale, wide);
+          if (exists) store32<BF16>(out, col0 + c * 32, a.D, o, keys_grad ? a.scale : 1.f, wide);
         }
       }
       id = next_tile(k);
@@ -468,7 +489,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == kCompute + 1) {
     fence_after();
     tmem_free(tmem, 512);
   }
@@ -483,7 +504,8 @@ struct Dq {
   static constexpr uint32_t kBars = kVRing + kV * kTile;
   static constexpr uint32_t kSmem = kBars + 512 + 1024;
   static constexpr uint32_t kS = 0, kDp = 256, kDq = 384;
-  static constexpr int kReaders = 10;                        // of the next tile's number: warps 0-9
+  static constexpr int kOutWarps = DP / 32 * 4 < kCompute ? DP / 32 * 4 : kCompute;   // that read the finished sums, 32 columns or more each
+  static constexpr int kReaders = kCompute + 2;              // of the next tile's number: all warps but the last two
 };
 struct DqBars {
   Handle next[2];
@@ -547,22 +569,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(b.next_full + i, 1);
       mbar_init(b.next_empty + i, C::kReaders);
       mbar_init(b.s + i, 1);
-      mbar_init(b.ds_ready + i, 8);
+      mbar_init(b.ds_ready + i, kCompute);
     }
     mbar_init(&b.q_full, 1);
     mbar_init(&b.q_empty, 1);
     mbar_init(&b.do_full, 1);
     mbar_init(&b.do_empty, 1);
     mbar_init(&b.dp, 1);
-    mbar_init(&b.dp_read, 8);
+    mbar_init(&b.dp_read, kCompute);
     mbar_init(&b.out_full, 1);
-    mbar_init(&b.out_empty, 8);
+    mbar_init(&b.out_empty, C::kOutWarps);
     mbar_init(&b.fix, 1);
     mbar_init(&b.drain, 1);
     b.abort = 0;
     fence_mbar_init();
   }
-  if (warp == 9) tmem_alloc(&b.tmem, 512);
+  if (warp == kCompute + 1) tmem_alloc(&b.tmem, 512);
   fence_before();
   __syncthreads();
   fence_after();
@@ -583,10 +605,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   };
 
-  // 384 threads start with 168 registers each, 64,512 together: 256 x 224 + 128 x 56.
-  if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == 8) {
+  // 384 threads start with 168 registers each, 64,512 together: 256 x 208 + 128 x 88.
+  if (warp >= kCompute) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == kCompute) {
       // ---------------------------------------------------------- loads, and the tiles to come
       bool ok = true;
       uint32_t n = 0, items = 0, fixes = 0;                  // key tiles, query tiles so far
@@ -642,7 +664,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         fail(kErrLoad);
         for (int i = 0; i < 1000; ++i) __nanosleep(1000);    // which copies are on their way is not known: the time that they can take
       }
-    } else if (warp == 9) {
+    } else if (warp == kCompute + 1) {
       // ---------------------------------------------------------- products
       constexpr uint32_t id_s = idesc(BF16, 128, false), id_o = idesc(BF16, DP, true);
       const uint32_t q_addr = smem_u32(smem), do_addr = q_addr + C::kTile;
@@ -652,70 +674,73 @@ __global__ void __launch_bounds__(kThreads, 1)
       int id = (int)blockIdx.x;
       for (int k = 0;; ++k) {
         const DqWork w = dq_work_at(a, (unsigned)id, tiles);
-        if (lane == 0 && w.n > 0) {
+        if (w.n > 0) {
           auto scores = [&](int j) {
             const uint32_t m = n + (uint32_t)j;
-            if (!wait(b.k_full + m % C::kK, (m / C::kK) & 1u, abort_flag)) return false;
-            mma_columns<DP>(tmem + C::kS + (m & 1) * 128, q_addr, k_ring + (m % C::kK) * C::kTile, id_s);
-            commit(b.s + (m & 1));
-            if (j + 1 == w.n) commit(&b.q_empty);
+            if (!wait_warp(b.k_full + m % C::kK, (m / C::kK) & 1u, abort_flag)) return false;
+            if (elect()) {
+              mma_columns<DP>(tmem + C::kS + (m & 1) * 128, q_addr, k_ring + (m % C::kK) * C::kTile, id_s);
+              commit(b.s + (m & 1));
+              if (j + 1 == w.n) commit(&b.q_empty);
+            }
+            __syncwarp();
             return true;
           };
           auto dprobs = [&](int j) {
             const uint32_t m = n + (uint32_t)j;
-            if (!wait(b.v_full + m % C::kV, (m / C::kV) & 1u, abort_flag)) return false;
-            mma_columns<DP>(tmem + C::kDp, do_addr, v_ring + (m % C::kV) * C::kTile, id_s);
-            commit(&b.dp);
-            commit(b.v_empty + m % C::kV);
-            if (j + 1 == w.n) commit(&b.do_empty);
+            if (!wait_warp(b.v_full + m % C::kV, (m / C::kV) & 1u, abort_flag)) return false;
+            if (elect()) {
+              mma_columns<DP>(tmem + C::kDp, do_addr, v_ring + (m % C::kV) * C::kTile, id_s);
+              commit(&b.dp);
+              commit(b.v_empty + m % C::kV);
+              if (j + 1 == w.n) commit(&b.do_empty);
+            }
+            __syncwarp();
             return true;
           };
-          ok = wait(&b.q_full, items & 1u, abort_flag) && scores(0);
-          // dP of the last tile has been read (its dS is complete: waited for below)
-          if (ok) ok = wait(&b.do_full, items & 1u, abort_flag) && dprobs(0);
+          ok = wait_warp(&b.q_full, items & 1u, abort_flag) && scores(0);
+          if (ok) ok = wait_warp(&b.do_full, items & 1u, abort_flag) && dprobs(0);
           if (ok && w.n > 1) ok = scores(1);
           for (int j = 0; j < w.n && ok; ++j) {
             const uint32_t m = n + (uint32_t)j;
-            if (!(ok = wait(&b.dp_read, m & 1u, abort_flag))) break;
+            if (!(ok = wait_warp(&b.dp_read, m & 1u, abort_flag))) break;
             if (j + 1 < w.n) {
               fence_after();
               if (!(ok = dprobs(j + 1))) break;
             }
             // the last tile's sums have been read before this one's are begun
-            if (j == 0 && !(ok = wait(&b.out_empty, (items & 1u) ^ 1u, abort_flag))) break;
-            if (!(ok = wait(b.ds_ready + (m & 1), (m >> 1) & 1u, abort_flag))) break;
+            if (j == 0 && !(ok = wait_warp(&b.out_empty, (items & 1u) ^ 1u, abort_flag))) break;
+            if (!(ok = wait_warp(b.ds_ready + (m & 1), (m >> 1) & 1u, abort_flag))) break;
             fence_after();
-            const uint32_t ds = tmem + C::kS + (m & 1) * 128;
-            mma_rows<0, 8>(tmem + C::kDq, ds, ds + 64, k_ring + (m % C::kK) * C::kTile, id_o, j > 0);
-            commit(b.k_empty + m % C::kK);
+            if (elect()) {
+              const uint32_t ds = tmem + C::kS + (m & 1) * 128;
+              mma_rows<0, 8, kCols / 16, kCols>(tmem + C::kDq, ds, k_ring + (m % C::kK) * C::kTile, id_o, j > 0);
+              commit(b.k_empty + m % C::kK);
+              if (j + 1 == w.n) commit(&b.out_full);
+            }
+            __syncwarp();
             if (j + 2 < w.n) ok = scores(j + 2);
           }
-          if (ok) commit(&b.out_full);
           n += (uint32_t)w.n;
           ++items;
         }
-        __syncwarp();
-        if (__any_sync(0xffffffffu, !ok)) {
-          ok = false;
-          break;
-        }
+        if (!ok) break;
         id = next_tile(k);
         ok = id != -2;
         if (id < 0) break;
       }
       if (!ok) fail(kErrMma);
-      if (lane == 0) {
-        commit(&b.drain);
-        mbar_wait(&b.drain, 0, kWaitNs);
-      }
       __syncwarp();
+      if (elect()) commit(&b.drain);
+      __syncwarp();
+      mbar_wait(&b.drain, 0, kWaitNs);
     }
   } else {
     // ------------------------------------------------------------ probabilities and score gradients: thread = query
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const int g = warp >> 2;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t t_dp = tmem + C::kDp + g * 64 + lanes;
+    const uint32_t t_dp = tmem + C::kDp + g * kCols + lanes;
     const F2 scale2 = f2(a.scale * kLog2e);
     bool ok = true;
     uint32_t n = 0, items = 0;
@@ -735,19 +760,19 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int keys_all = __shfl_sync(0xffffffffu, keys, 0);
       const F2 base2 = f2(-lse2), delta2 = f2(-delta);
       for (int j = 0; j < w.n; ++j, ++n) {
-        const bool masked = keys_all < j * 128 + g * 64 + 64;
-        const int left = keys - j * 128 - g * 64;
+        const bool masked = keys_all < j * 128 + (g + 1) * kCols;
+        const int left = keys - j * 128 - g * kCols;
         if (!(ok = wait_warp(b.s + (n & 1), (n >> 1) & 1u, abort_flag))) break;
         fence_after();
-        const uint32_t t_s = tmem + C::kS + (n & 1) * 128 + g * 64 + lanes;
-        F2 p[32];
-        uint32_t s[2][32];
-        tmem_ld32(t_s, s[0]);
-        tmem_ld32(t_s + 32, s[1]);
-        tmem_wait_ld(s[0]);
-        tmem_wait_ld(s[1]);
+        const uint32_t t_s = tmem + C::kS + (n & 1) * 128 + g * kCols + lanes;
+        F2 p[kCols / 2];
+        uint32_t s[kCols / 32][32];
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
+        for (int c = 0; c < kCols / 32; ++c) tmem_ld32(t_s + c * 32, s[c]);
+#pragma unroll
+        for (int c = 0; c < kCols / 32; ++c) tmem_wait_ld(s[c]);
+#pragma unroll
+        for (int c = 0; c < kCols / 32; ++c)
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             float x0, x1;
@@ -756,15 +781,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         if (!(ok = wait_warp(&b.dp, n & 1u, abort_flag))) break;
         fence_after();
-        tmem_ld32(t_dp, s[0]);
-        tmem_ld32(t_dp + 32, s[1]);
-        tmem_wait_ld(s[0]);
-        tmem_wait_ld(s[1]);
+#pragma unroll
+        for (int c = 0; c < kCols / 32; ++c) tmem_ld32(t_dp + c * 32, s[c]);
+#pragma unroll
+        for (int c = 0; c < kCols / 32; ++c) tmem_wait_ld(s[c]);
         fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&b.dp_read);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+        for (int c = 0; c < kCols / 32; ++c) {
           uint32_t wd[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
@@ -790,27 +815,30 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!ok) break;
       if (w.sp.tile < 0) {
-        if (a.zero_tail) zero_rows(a.dq, w.head, w.sp.first_q, 128, a.Sq, a.D, threadIdx.x, 256);
+        if (a.zero_tail) zero_rows(a.dq, w.head, w.sp.first_q, 128, a.Sq, a.D, threadIdx.x, kCompute * 32);
       } else {
-        // each warpgroup writes half of the columns
+        // each warpgroup writes its share of the columns
+        constexpr int per = DP * 4 / C::kOutWarps;
         const bool wide = rows_are_wide(a.dq);
         uint16_t* out = row_ptr(a.dq, w.sp.batch, w.head, w.sp.first_q + row);
+        if (warp < C::kOutWarps) {
 #pragma unroll
-        for (int c = 0; c < DP / 64; ++c) {
-          const int col = g * (DP / 2) + c * 32;
-          uint32_t o[32];
+          for (int c = 0; c < per / 32; ++c) {
+            const int col = g * per + c * 32;
+            uint32_t o[32];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = 0;
-          if (w.n > 0) {
-            tmem_ld32(tmem + C::kDq + lanes + col, o);
-            tmem_wait_ld(o);
-            if (c == DP / 64 - 1) {                          // the sums may be written again
-              fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&b.out_empty);
+            for (int e = 0; e < 32; ++e) o[e] = 0;
+            if (w.n > 0) {
+              tmem_ld32(tmem + C::kDq + lanes + col, o);
+              tmem_wait_ld(o);
+              if (c == per / 32 - 1) {                       // the sums may be written again
+                fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&b.out_empty);
+              }
             }
+            if (exists) store32<BF16>(out, col, a.D, o, a.scale, wide);
           }
-          if (exists) store32<BF16>(out, col, a.D, o, a.scale, wide);
         }
       }
       id = next_tile(k);
@@ -821,7 +849,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == kCompute + 1) {
     fence_after();
     tmem_free(tmem, 512);
   }

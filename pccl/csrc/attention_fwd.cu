@@ -141,9 +141,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
 
   // Registers: 384 threads start with 168 each, 64,512 together.  A thread that holds 128 scores wants more, the issuing warps
-  // less: 256 x 224 + 128 x 56 = 64,512.
+  // less: 256 x 216 + 128 x 72 = 64,512.
   if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 8) {
       // ---------------------------------------------------------- loads, and the tiles to come
       bool ok = true;
@@ -212,22 +212,29 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int k = 0;; ++k) {
         const Work w = work_at(a, (unsigned)id, tiles);
         const int nmax = w.n[0] > w.n[1] ? w.n[0] : w.n[1];
-        if (lane == 0 && nmax > 0) {
+        if (nmax > 0) {
           auto tile_at = [&](uint32_t i) { return ring + (i % C::kStages) * C::kTile; };
-          auto loaded = [&](uint32_t i) { return wait(b.full + i % C::kStages, (i / C::kStages) & 1u, abort_flag); };
+          auto loaded = [&](uint32_t i) { return wait_warp(b.full + i % C::kStages, (i / C::kStages) & 1u, abort_flag); };
           auto scores = [&](int h, int j) {
-            mma_columns<DP>(tmem + C::kS + h * 128, q_addr + h * C::kTile, tile_at(it + 2 * j), id_s);
-            commit(b.s + h);
-            if (j + 1 == w.n[h]) commit(b.q_empty + h);      // the queries are not read again
+            if (elect()) {
+              mma_columns<DP>(tmem + C::kS + h * 128, q_addr + h * C::kTile, tile_at(it + 2 * j), id_s);
+              commit(b.s + h);
+              if (j + 1 == w.n[h]) commit(b.q_empty + h);    // the queries are not read again
+            }
+            __syncwarp();
+          };
+          auto release = [&](uint32_t i) {
+            if (elect()) commit(b.empty + i % C::kStages);
+            __syncwarp();
           };
           ok = loaded(it);
 #pragma unroll
           for (int h = 0; h < 2; ++h)
             if (ok && w.n[h] > 0) {
-              ok = wait(b.q_full + h, items[h] & 1u, abort_flag);
+              ok = wait_warp(b.q_full + h, items[h] & 1u, abort_flag);
               if (ok) scores(h, 0);
             }
-          if (ok) commit(b.empty + it % C::kStages);
+          if (ok) release(it);
           for (int j = 0; j < nmax && ok; ++j) {
             if (!(ok = loaded(it + 2 * j + 1))) break;
 #pragma unroll
@@ -235,22 +242,26 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (!ok) break;
               if (j < w.n[h]) {
                 // the last tile's sums have been read out of O before this one's are begun
-                if (j == 0 && !(ok = wait(b.o_empty + h, (items[h] & 1u) ^ 1u, abort_flag))) break;
+                if (j == 0 && !(ok = wait_warp(b.o_empty + h, (items[h] & 1u) ^ 1u, abort_flag))) break;
                 const uint32_t ph = (s_count[h] + (uint32_t)j) & 1u, p = tmem + C::kS + h * 128, v = tile_at(it + 2 * j + 1);
-                if (!(ok = wait(b.p0 + h, ph, abort_flag))) break;
+                if (!(ok = wait_warp(b.p0 + h, ph, abort_flag))) break;
                 fence_after();
-                mma_rows<0, 4>(tmem + C::kO + h * 128, p, p + 32, v, id_o, j > 0);
-                if (!(ok = wait(b.p1 + h, ph, abort_flag))) break;
+                if (elect()) mma_rows<0, 4, 8, 0>(tmem + C::kO + h * 128, p, v, id_o, j > 0);
+                __syncwarp();
+                if (!(ok = wait_warp(b.p1 + h, ph, abort_flag))) break;
                 fence_after();
-                mma_rows<4, 8>(tmem + C::kO + h * 128, p, p + 32, v, id_o, true);
-                if (j + 1 == w.n[h]) commit(b.o_full + h);
+                if (elect()) {
+                  mma_rows<4, 8, 8, 0>(tmem + C::kO + h * 128, p, v, id_o, true);
+                  if (j + 1 == w.n[h]) commit(b.o_full + h);
+                }
+                __syncwarp();
               }
               if (h == 0 && j + 1 < nmax) ok = loaded(it + 2 * j + 2);
               if (ok && j + 1 < w.n[h]) scores(h, j + 1);
             }
             if (!ok) break;
-            commit(b.empty + (it + 2 * j + 1) % C::kStages);
-            if (j + 1 < nmax) commit(b.empty + (it + 2 * j + 2) % C::kStages);
+            release(it + 2 * j + 1);
+            if (j + 1 < nmax) release(it + 2 * j + 2);
           }
           it += 2 * (uint32_t)nmax;
 #pragma unroll
@@ -260,30 +271,25 @@ __global__ void __launch_bounds__(kThreads, 1)
               ++items[h];
             }
         }
-        __syncwarp();
-        if (__any_sync(0xffffffffu, !ok)) {
-          ok = false;
-          break;
-        }
+        if (!ok) break;
         id = next_tile(k);
         if (id < 0) {
           ok = id == -1;
           break;
         }
       }
-      if (lane == 0) {
-        if (!ok) {
-          atomicCAS(a.error, 0, kErrMma);
-          *abort_flag = 1;
-        }
-        commit(&b.drain);
-        mbar_wait(&b.drain, 0, kWaitNs);
+      if (!ok && lane == 0) {
+        atomicCAS(a.error, 0, kErrMma);
+        *abort_flag = 1;
       }
       __syncwarp();
+      if (elect()) commit(&b.drain);
+      __syncwarp();
+      mbar_wait(&b.drain, 0, kWaitNs);
     }
   } else {
     // ------------------------------------------------------------ softmax: thread = query
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     const int h = warp >> 2;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem + C::kS + h * 128 + lanes, t_o = tmem + C::kO + h * 128 + lanes;
