@@ -227,57 +227,72 @@ __device__ __forceinline__ int work_taken(const Handle* slot) {
   return taken ? x : -1;
 }
 
-// ---- which rows a CTA works on.  Packed sequences are cut into tiles of `rows` each on its own; tile numbers run through
-// them in order.  The starts are clamped into [0, limit], so that starts that are out of order or out of range make tiles
-// fewer, shorter or equal, never out of range.
+// ---- which rows a CTA works on.  Packed sequences are cut into tiles of `rows` each on its own.  Tiles are numbered by what is
+// left of their sequence behind them (keys: that many query tiles see them) or lies before them (queries: they see that many
+// key tiles), most first, so that with a causal mask the longest come first, whatever the order of the sequences.  A kernel of
+// one block per table writes down which is which.  The starts are clamped into [0, limit], so that starts that are out of
+// order or out of range make tiles fewer, shorter or equal, never out of range.
 struct Span {
   int batch, first_q, len_q, first_k, len_k;   // the sequence
   int tile;                                    // tile number within it, or -1: no tile left
 };
 __device__ __forceinline__ int clamp_start(int x, int limit) { return x < 0 ? 0 : (x > limit ? limit : x); }
+__host__ __device__ __forceinline__ int64_t max_tiles(int64_t limit, int64_t nseq, int rows) { return limit / rows + nseq + 1; }
 
-// The sequence that holds tile t, counted over tiles of `rows` query rows (of_keys: key rows).  Whole warps only.  Where the
-// tiles run out, tile is -1 and first_q (first_k) the first row of the tail that tile t - tiles stands for.
-__device__ __forceinline__ Span find_span(const AttnArgs& a, int t, int rows, bool of_keys) {
-  const int lane = threadIdx.x & 31;
-  const int* cu = of_keys ? a.cu_k : a.cu_q;
-  const int limit = of_keys ? a.Sk : a.Sq;
-  int before = 0;
-  for (int s0 = 0; s0 < a.nseq; s0 += 32) {
-    const int s = s0 + lane;
-    int n = 0;
-    if (s < a.nseq) {
-      const int len = clamp_start(cu[s + 1], limit) - clamp_start(cu[s], limit);
-      n = len > 0 ? (len + rows - 1) / rows : 0;
+// order[t] = (sequence, tile), or (-1, how many tiles of the tail lie before it) behind the last one.  A sequence of n tiles has one on each
+// of the levels 1 to n; levels are listed from the highest on, sequences in order on each.  A warp takes a level.
+__device__ __forceinline__ void write_order(const int* cu, int nseq, int limit, int rows, bool of_keys, int2* order) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int entries = (int)max_tiles(limit, nseq, rows);
+  auto tiles_of = [&](int s) {
+    if (s >= nseq) return 0;
+    const int len = clamp_start(cu[s + 1], limit) - clamp_start(cu[s], limit);
+    return len > 0 ? (len + rows - 1) / rows : 0;
+  };
+  // how many tiles are on level r or above (starts that overlap may make more than there are entries)
+  auto above = [&](int r) {
+    int64_t n = 0;
+    for (int s = lane; s < nseq; s += 32) {
+      const int m = tiles_of(s) - r + 1;
+      n += m > 0 ? m : 0;
     }
-    int upto = n;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += x;
+    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    return n;
+  };
+  const int most = (int)((limit + rows - 1) / rows);
+  for (int level = warp + 1; level <= most; level += warps) {
+    int64_t at = above(level + 1);
+    for (int s0 = 0; s0 < nseq && at < entries; s0 += 32) {
+      const int n = tiles_of(s0 + lane);
+      const unsigned hit = __ballot_sync(0xffffffffu, n >= level);
+      const int64_t t = at + __popc(hit & ((1u << lane) - 1u));
+      if (n >= level && t < entries) order[t] = make_int2(s0 + lane, of_keys ? n - level : level - 1);
+      at += __popc(hit);
     }
-    const unsigned hit = __ballot_sync(0xffffffffu, t < before + upto);
-    if (hit != 0u) {
-      const int who = __ffs(hit) - 1;
-      const int start = before + __shfl_sync(0xffffffffu, upto - n, who);
-      Span sp;
-      const int sq = s0 + who;
-      sp.batch = 0;
-      sp.first_q = clamp_start(a.cu_q[sq], a.Sq);
-      sp.len_q = clamp_start(a.cu_q[sq + 1], a.Sq) - sp.first_q;
-      sp.first_k = clamp_start(a.cu_k[sq], a.Sk);
-      sp.len_k = clamp_start(a.cu_k[sq + 1], a.Sk) - sp.first_k;
-      if (sp.len_q < 0) sp.len_q = 0;
-      if (sp.len_k < 0) sp.len_k = 0;
-      sp.tile = t - start;
-      return sp;
-    }
-    before += __shfl_sync(0xffffffffu, upto, 31);
   }
+  const int64_t total = above(1);
+  for (int64_t t = total + threadIdx.x; t < entries; t += blockDim.x) order[t] = make_int2(-1, (int)(t - total));
+}
+__device__ __forceinline__ Span find_span(const AttnArgs& a, int t, int rows, bool of_keys) {
+  const int2 e = (of_keys ? a.order_k : a.order_q)[t];
   Span sp;
-  sp.batch = sp.len_q = sp.len_k = 0;
-  sp.tile = -1;
-  sp.first_q = sp.first_k = clamp_start(cu[a.nseq], limit) + (t - before) * rows;
+  sp.batch = 0;
+  if (e.x < 0) {
+    const int limit = of_keys ? a.Sk : a.Sq;
+    const int64_t first = (int64_t)clamp_start((of_keys ? a.cu_k : a.cu_q)[a.nseq], limit) + (int64_t)e.y * rows;
+    sp.len_q = sp.len_k = 0;
+    sp.tile = -1;
+    sp.first_q = sp.first_k = first > limit ? limit : (int)first;
+    return sp;
+  }
+  sp.first_q = clamp_start(a.cu_q[e.x], a.Sq);
+  sp.len_q = clamp_start(a.cu_q[e.x + 1], a.Sq) - sp.first_q;
+  sp.first_k = clamp_start(a.cu_k[e.x], a.Sk);
+  sp.len_k = clamp_start(a.cu_k[e.x + 1], a.Sk) - sp.first_k;
+  if (sp.len_q < 0) sp.len_q = 0;
+  if (sp.len_k < 0) sp.len_k = 0;
+  sp.tile = e.y;
   return sp;
 }
 
@@ -317,6 +332,18 @@ __device__ __forceinline__ bool rows_are_wide(const AttnTensor& t) {
 }
 __device__ __forceinline__ uint16_t* row_ptr(const AttnTensor& t, int batch, int head, int row) {
   return reinterpret_cast<uint16_t*>(const_cast<void*>(t.p)) + (int64_t)batch * t.sb + (int64_t)row * t.ss + (int64_t)head * t.sh;
+}
+// Where the row of one part's sums starts (H heads of S rows).
+__device__ __forceinline__ float* part_row(float* partial, int part, int B, int H, int S, int D, int batch, int head, int row) {
+  return partial + ((((int64_t)part * B + batch) * H + head) * S + row) * D;
+}
+// 32 accumulator columns of one row, times f, in fp32.
+__device__ __forceinline__ void store32_f32(float* row, int col0, int D, const uint32_t* r, float f) {
+#pragma unroll
+  for (int v = 0; v < 8; ++v)
+    if (col0 + v * 4 < D)
+      *reinterpret_cast<float4*>(row + col0 + v * 4) = make_float4(__uint_as_float(r[v * 4]) * f, __uint_as_float(r[v * 4 + 1]) * f,
+                                                                   __uint_as_float(r[v * 4 + 2]) * f, __uint_as_float(r[v * 4 + 3]) * f);
 }
 // Where the row statistics of one head start.
 __device__ __forceinline__ int64_t stat_row(const AttnArgs& a, int batch, int head) { return ((int64_t)batch * a.H + head) * a.Sq; }

@@ -29,14 +29,28 @@ struct AttnArgs {
   const int* cu_q;                   // packed: nseq + 1 starts of the sequences (device), nullptr where not packed
   const int* cu_k;
   int nseq;
+  int2* order_q;                     // packed: which sequence and which of its tiles each tile number stands for (scratch; forward:
+  int2* order_k;                     // order_q; backward: both)
   int causal;
   int zero_tail;                     // packed: rows behind the last sequence are set to 0 (lse: -inf); else they are left alone
   float scale;
   int* error;
+  // Work split over a long axis (not for packed sequences), where there are too few tiles for the device: the parts of one
+  // tile's sum go to partial, [part][batch][head][row][D] in fp32, and are added up by a small kernel.
+  int parts_o, parts_dq, parts_dkv;  // 1: not split
+  float* partial;
+  float* partial_lse;                // forward: lse of each part, [part][batch][head][row]
 };
 
 constexpr int kAttnMaxDim = 128;     // columns of a head: a multiple of 8 up to this
 
+// How many parts to cut each tile's work into: fills in parts_* and returns what partial, partial_lse (floats) and order_* need.
+struct AttnScratch {
+  int64_t partial, partial_lse;
+  int64_t order_q, order_k;          // entries
+};
+AttnScratch plan_attention_forward(AttnArgs& a, int sm_count);
+AttnScratch plan_attention_backward(AttnArgs& a, int sm_count);
 cudaError_t launch_attention_forward(const AttnArgs& a, cudaStream_t stream);
 cudaError_t launch_attention_backward(const AttnArgs& a, cudaStream_t stream);
 

@@ -142,6 +142,18 @@ std::tuple<at::Tensor, at::Tensor> attention_forward(const at::Tensor& q, const 
   at::Tensor lse = s.packed ? at::empty({s.H, s.Sq}, f32) : at::empty({s.B, s.H, s.Sq}, f32);
   a.lse = lse.data_ptr<float>();
   a.zero_tail = !out_.has_value();
+  const AttnScratch need = plan_attention_forward(a, at::cuda::getCurrentDeviceProperties()->multiProcessorCount);
+  at::Tensor partial, partial_lse, order;
+  if (need.order_q > 0) {
+    order = at::empty({2 * need.order_q}, q.options().dtype(at::kInt));
+    a.order_q = reinterpret_cast<int2*>(order.data_ptr<int>());
+  }
+  if (need.partial > 0) {
+    partial = at::empty({need.partial}, f32);
+    partial_lse = at::empty({need.partial_lse}, f32);
+    a.partial = partial.data_ptr<float>();
+    a.partial_lse = partial_lse.data_ptr<float>();
+  }
   PCCL_CUDA(launch_attention_forward(a, at::cuda::getCurrentCUDAStream().stream()));
   return {out, lse};
 }
@@ -170,6 +182,17 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_backward(const at::Tens
   at::Tensor delta = at::empty_like(lse);
   a.delta = delta.data_ptr<float>();
   a.zero_tail = !dq_.has_value();
+  const AttnScratch need = plan_attention_backward(a, at::cuda::getCurrentDeviceProperties()->multiProcessorCount);
+  at::Tensor partial, order;
+  if (need.order_q > 0) {
+    order = at::empty({2 * (need.order_q + need.order_k)}, q.options().dtype(at::kInt));
+    a.order_q = reinterpret_cast<int2*>(order.data_ptr<int>());
+    a.order_k = a.order_q + need.order_q;
+  }
+  if (need.partial > 0) {
+    partial = at::empty({need.partial}, lse.options());
+    a.partial = partial.data_ptr<float>();
+  }
   PCCL_CUDA(launch_attention_backward(a, at::cuda::getCurrentCUDAStream().stream()));
   return {dq, dk, dv};
 }

@@ -72,6 +72,11 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(const __grid_const
   }
 }
 
+__global__ void __launch_bounds__(1024) attention_orders_kernel(const __grid_constant__ AttnArgs a) {
+  if (blockIdx.x == 0) write_order(a.cu_k, a.nseq, a.Sk, 128, true, a.order_k);
+  else write_order(a.cu_q, a.nseq, a.Sq, 128, false, a.order_q);
+}
+
 // ---------------------------------------------------------------- dk, dv
 template <int DP>
 struct Dkv {
@@ -98,13 +103,18 @@ struct DkvBars {
 static_assert(sizeof(DkvBars) <= 512, "the barriers' part of shared memory");
 
 // The keys of one tile number, and the query tiles that see one of them: per_head of them from tile `first` on, for each head
-// of the group.
+// of the group.  Of that sequence of steps, `total` from i0 on are this part's.
 struct DkvWork {
   Span sp;
-  int kv_head, key0, offset, first, per_head, total;
+  int kv_head, key0, offset, first, per_head, part, i0, total;
 };
 __device__ __forceinline__ DkvWork dkv_work_at(const AttnArgs& a, unsigned id) {
   DkvWork w;
+  w.part = 0;
+  if (a.parts_dkv > 1) {
+    w.part = (int)(id % (unsigned)a.parts_dkv);
+    id /= (unsigned)a.parts_dkv;
+  }
   if (a.cu_q != nullptr) {
     w.kv_head = (int)(id % (unsigned)a.Hk);
     w.sp = find_span(a, (int)(id / (unsigned)a.Hk), 128, true);
@@ -123,7 +133,12 @@ __device__ __forceinline__ DkvWork dkv_work_at(const AttnArgs& a, unsigned id) {
   w.first = a.causal && w.key0 - w.offset > 0 ? (w.key0 - w.offset) / 128 : 0;
   const int tiles = (w.sp.len_q + 127) / 128;
   w.per_head = w.sp.tile >= 0 && tiles > w.first ? tiles - w.first : 0;
+  w.i0 = 0;
   w.total = a.H / a.Hk * w.per_head;
+  if (a.parts_dkv > 1) {
+    w.i0 = (int)((int64_t)w.total * w.part / a.parts_dkv);
+    w.total = (int)((int64_t)w.total * (w.part + 1) / a.parts_dkv) - w.i0;
+  }
   return w;
 }
 
@@ -207,7 +222,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) ask_for_work(b.next + (k & 1), b.next_full + (k & 1));
         const DkvWork w = dkv_work_at(a, (unsigned)id);
         for (int i = 0; i < w.total && ok; ++i, ++n) {
-          const int hg = i / w.per_head, head = w.kv_head * group + hg, row = (w.first + i - hg * w.per_head) * 128;
+          const int hg = (w.i0 + i) / w.per_head, head = w.kv_head * group + hg, row = (w.first + w.i0 + i - hg * w.per_head) * 128;
           // the rows behind a packed sequence are its neighbour's, and both tiles are contracted along their rows
           const bool ragged = a.cu_q != nullptr && row + 128 > w.sp.len_q;
 #pragma unroll
@@ -326,7 +341,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int k = 0; ok; ++k) {
         const DkvWork w = dkv_work_at(a, (unsigned)id);
         for (int i = 0; i < w.total; ++i, ++n) {
-          const int hg = i / w.per_head, head = w.kv_head * group + hg, row = (w.first + i - hg * w.per_head) * 128;
+          const int hg = (w.i0 + i) / w.per_head, head = w.kv_head * group + hg, row = (w.first + w.i0 + i - hg * w.per_head) * 128;
           const int64_t at = stat_row(a, w.sp.batch, head) + w.sp.first_q;
           float x[4], y[4];
 #pragma unroll
@@ -367,7 +382,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int k = 0; ok; ++k) {
       const DkvWork w = dkv_work_at(a, (unsigned)id);
       const int key = w.key0 + (warp & 3) * 32 + lane;
-      int tile = w.first;                                    // query tile within its head
+      int tile = w.first + (w.per_head > 0 ? w.i0 % w.per_head : 0);            // query tile within its head
       for (int i = 0; i < w.total; ++i, ++n) {
         const float* st = reinterpret_cast<const float*>(smem + C::kStat) + (n & 1) * 256 + g * kCols;
         const int q0 = tile * 128 + g * kCols;
@@ -478,7 +493,14 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (lane == 0) mbar_arrive(&b.out_empty);
             }
           }
-          if (exists) store32<BF16>(out, col0 + c * 32, a.D, o, keys_grad ? a.scale : 1.f, wide);
+          if (!exists) continue;
+          if (a.parts_dkv > 1) {
+            // dv's parts first, then dk's
+            float* sums = part_row(a.partial, keys_grad ? a.parts_dkv + w.part : w.part, a.B, a.Hk, a.Sk, a.D, w.sp.batch, w.kv_head, key);
+            store32_f32(sums, col0 + c * 32, a.D, o, keys_grad ? a.scale : 1.f);
+          } else {
+            store32<BF16>(out, col0 + c * 32, a.D, o, keys_grad ? a.scale : 1.f, wide);
+          }
         }
       }
       id = next_tile(k);
@@ -517,13 +539,18 @@ struct DqBars {
 };
 static_assert(sizeof(DqBars) <= 512, "the barriers' part of shared memory");
 
-// The queries of one tile number, and how many key tiles they see.
+// The queries of one tile number, and the key tiles that this part of them has to do with: n of them from tile j0 on.
 struct DqWork {
   Span sp;
-  int head, row0, offset, n;
+  int head, row0, offset, part, j0, n;
 };
 __device__ __forceinline__ DqWork dq_work_at(const AttnArgs& a, unsigned id, int tiles) {
   DqWork w;
+  w.part = 0;
+  if (a.parts_dq > 1) {
+    w.part = (int)(id % (unsigned)a.parts_dq);
+    id /= (unsigned)a.parts_dq;
+  }
   if (a.cu_q != nullptr) {
     w.head = (int)(id % (unsigned)a.H);
     w.sp = find_span(a, (int)(id / (unsigned)a.H), 128, false);
@@ -541,6 +568,11 @@ __device__ __forceinline__ DqWork dq_work_at(const AttnArgs& a, unsigned id, int
   const int last = w.row0 + 127 < w.sp.len_q - 1 ? w.row0 + 127 : w.sp.len_q - 1;
   const int keys = !a.causal ? w.sp.len_k : (last + w.offset + 1 < w.sp.len_k ? last + w.offset + 1 : w.sp.len_k);
   w.n = w.sp.tile >= 0 && keys > 0 ? (keys + 127) / 128 : 0;
+  w.j0 = 0;
+  if (a.parts_dq > 1) {
+    w.j0 = w.n * w.part / a.parts_dq;
+    w.n = w.n * (w.part + 1) / a.parts_dq - w.j0;
+  }
   return w;
 }
 
@@ -623,15 +655,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!(ok = wait_warp(b.k_empty + ks, ((n / C::kK) & 1u) ^ 1u, abort_flag))) break;
           unsigned char* dst = smem + C::kKRing + ks * C::kTile;
           // the rows behind a packed sequence are its neighbour's
-          const bool ragged = a.cu_q != nullptr && (j + 1) * 128 > w.sp.len_k;
+          const int row = (w.j0 + j) * 128;
+          const bool ragged = a.cu_q != nullptr && row + 128 > w.sp.len_k;
           uint64_t* bar = ragged ? &b.fix : b.k_full + ks;
           if (lane == 0) {
             mbar_expect_tx(bar, C::kTile);
-            load_tile<DP>(dst, &map_k, kv_head, w.sp.first_k + j * 128, w.sp.batch, bar);
+            load_tile<DP>(dst, &map_k, kv_head, w.sp.first_k + row, w.sp.batch, bar);
           }
           if (ragged) {
             if (!(ok = wait_warp(&b.fix, fixes++ & 1u, abort_flag))) break;
-            clear_rows<DP>(dst, w.sp.len_k - j * 128);
+            clear_rows<DP>(dst, w.sp.len_k - row);
             if (lane == 0) mbar_arrive(b.k_full + ks);
           }
           if (j == 0) {                                      // behind the first keys: the queries of the last tile may still be in use
@@ -644,7 +677,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!(ok = wait_warp(b.v_empty + vs, ((n / C::kV) & 1u) ^ 1u, abort_flag))) break;
           if (lane == 0) {
             mbar_expect_tx(b.v_full + vs, C::kTile);
-            load_tile<DP>(smem + C::kVRing + vs * C::kTile, &map_v, kv_head, w.sp.first_k + j * 128, w.sp.batch, b.v_full + vs);
+            load_tile<DP>(smem + C::kVRing + vs * C::kTile, &map_v, kv_head, w.sp.first_k + row, w.sp.batch, b.v_full + vs);
           }
           if (j == 0) {
             if (!(ok = wait_warp(&b.do_empty, (items & 1u) ^ 1u, abort_flag))) break;
@@ -760,8 +793,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int keys_all = __shfl_sync(0xffffffffu, keys, 0);
       const F2 base2 = f2(-lse2), delta2 = f2(-delta);
       for (int j = 0; j < w.n; ++j, ++n) {
-        const bool masked = keys_all < j * 128 + (g + 1) * kCols;
-        const int left = keys - j * 128 - g * kCols;
+        const int key0 = (w.j0 + j) * 128 + g * kCols;
+        const bool masked = keys_all < key0 + kCols;
+        const int left = keys - key0;
         if (!(ok = wait_warp(b.s + (n & 1), (n >> 1) & 1u, abort_flag))) break;
         fence_after();
         const uint32_t t_s = tmem + C::kS + (n & 1) * 128 + g * kCols + lanes;
@@ -837,7 +871,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (lane == 0) mbar_arrive(&b.out_empty);
               }
             }
-            if (exists) store32<BF16>(out, col, a.D, o, a.scale, wide);
+            if (!exists) continue;
+            if (a.parts_dq > 1) store32_f32(part_row(a.partial, w.part, a.B, a.H, a.Sq, a.D, w.sp.batch, w.head, row), col, a.D, o, a.scale);
+            else store32<BF16>(out, col, a.D, o, a.scale, wide);
           }
         }
       }
@@ -853,6 +889,34 @@ __global__ void __launch_bounds__(kThreads, 1)
     fence_after();
     tmem_free(tmem, 512);
   }
+}
+
+// A gradient from its parts, added up in order: dst = sum of `parts` arrays of [batch][head][row][D].  Sixteen lanes per row.
+template <bool BF16>
+__global__ void __launch_bounds__(256) attention_sum_kernel(const float* partial, int parts, AttnTensor dst, int B, int H, int S, int D) {
+  const int sub = threadIdx.x & 15;
+  const int64_t rows = (int64_t)B * H * S, r = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 4;
+  if (r >= rows || sub * 8 >= D) return;
+  const int64_t bh = r / S;
+  const int row = (int)(r - bh * S), b = (int)(bh / H), h = (int)(bh - (int64_t)b * H);
+  float o[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) o[e] = 0.f;
+  for (int p = 0; p < parts; ++p) {
+    const float4* v = reinterpret_cast<const float4*>(partial + (p * rows + r) * D + sub * 8);
+    const float4 u = v[0], w = v[1];
+    o[0] += u.x, o[1] += u.y, o[2] += u.z, o[3] += u.w;
+    o[4] += w.x, o[5] += w.y, o[6] += w.z, o[7] += w.w;
+  }
+  *reinterpret_cast<uint4*>(row_ptr(dst, b, h, row) + sub * 8) =
+      make_uint4(pack2<BF16>(o[0], o[1]), pack2<BF16>(o[2], o[3]), pack2<BF16>(o[4], o[5]), pack2<BF16>(o[6], o[7]));
+}
+template <bool BF16>
+cudaError_t add_parts(const float* partial, int parts, const AttnTensor& dst, int B, int H, int S, int D, cudaStream_t stream) {
+  const int64_t blocks = ((int64_t)B * H * S + 15) / 16;
+  if (blocks > INT32_MAX) return cudaErrorInvalidValue;
+  attention_sum_kernel<BF16><<<(unsigned)blocks, 256, 0, stream>>>(partial, parts, dst, B, H, S, D);
+  return cudaGetLastError();
 }
 
 // The shared-memory limit is an attribute of the function on the current device.
@@ -878,6 +942,11 @@ cudaError_t launch(const AttnArgs& a, cudaStream_t stream) {
     return cudaErrorInvalidValue;
   if (a.Sq == 0) mq = mdo = mk;                              // nothing of what is missing is ever loaded
   if (a.Sk == 0) mk = mv = mq;
+  if (packed) {
+    attention_orders_kernel<<<2, 1024, 0, stream>>>(a);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+  }
   if (a.Sq > 0) {
     if (a.B > 65535) return cudaErrorInvalidValue;
     attention_delta_kernel<BF16><<<dim3((unsigned)((a.Sq + 63) / 64), (unsigned)a.H, (unsigned)a.B), 256, 0, stream>>>(a);
@@ -887,29 +956,65 @@ cudaError_t launch(const AttnArgs& a, cudaStream_t stream) {
   if (a.Sk > 0) {
     cudaError_t e = allow_smem<attention_dkv_kernel<DP, BF16>>(Dkv<DP>::kSmem);
     if (e != cudaSuccess) return e;
-    const int64_t tiles = packed ? a.Sk / 128 + (int64_t)a.nseq + 1 : ((int64_t)a.Sk + 127) / 128;
-    const int64_t ctas = tiles * a.Hk * a.B;
+    const int64_t tiles = packed ? max_tiles(a.Sk, a.nseq, 128) : ((int64_t)a.Sk + 127) / 128;
+    const int64_t ctas = tiles * a.Hk * a.B * a.parts_dkv;
     if (ctas > INT32_MAX) return cudaErrorInvalidValue;
     attention_dkv_kernel<DP, BF16><<<(unsigned)ctas, kThreads, Dkv<DP>::kSmem, stream>>>(mq, mk, mv, mdo, a);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    if (a.parts_dkv > 1) {
+      if ((e = add_parts<BF16>(a.partial, a.parts_dkv, a.dv, a.B, a.Hk, a.Sk, a.D, stream)) != cudaSuccess) return e;
+      const float* dk = a.partial + (int64_t)a.parts_dkv * a.B * a.Hk * a.Sk * a.D;
+      if ((e = add_parts<BF16>(dk, a.parts_dkv, a.dk, a.B, a.Hk, a.Sk, a.D, stream)) != cudaSuccess) return e;
+    }
   }
   if (a.Sq > 0) {
     cudaError_t e = allow_smem<attention_dq_kernel<DP, BF16>>(Dq<DP>::kSmem);
     if (e != cudaSuccess) return e;
-    const int64_t tiles = packed ? a.Sq / 128 + (int64_t)a.nseq + 1 : ((int64_t)a.Sq + 127) / 128;
-    const int64_t ctas = tiles * a.H * a.B;
+    const int64_t tiles = packed ? max_tiles(a.Sq, a.nseq, 128) : ((int64_t)a.Sq + 127) / 128;
+    const int64_t ctas = tiles * a.H * a.B * a.parts_dq;
     if (ctas > INT32_MAX) return cudaErrorInvalidValue;
     attention_dq_kernel<DP, BF16><<<(unsigned)ctas, kThreads, Dq<DP>::kSmem, stream>>>(mq, mk, mv, mdo, a, (int)tiles);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    if (a.parts_dq > 1 && (e = add_parts<BF16>(a.partial, a.parts_dq, a.dq, a.B, a.H, a.Sq, a.D, stream)) != cudaSuccess) return e;
   }
   return cudaSuccess;
 }
 
 }  // namespace
 
+// Tiles are split where they alone leave SMs without work, into parts of two key tiles (dq) or four steps (dk, dv) or more.  A group
+// of many heads on few key heads makes few and long tiles: those are cut until there are two for each SM.  Both kernels use the
+// same memory for their parts, one after the other.
+AttnScratch plan_attention_backward(AttnArgs& a, int sm_count) {
+  a.parts_dq = a.parts_dkv = 1;
+  if (a.cu_q == nullptr && a.Sq > 0 && a.Sk > 0) {
+    const int64_t q_tiles = ((int64_t)a.Sq + 127) / 128, k_tiles = ((int64_t)a.Sk + 127) / 128;
+    const int64_t dq = q_tiles * a.H * a.B, dkv = k_tiles * a.Hk * a.B, steps = q_tiles * (a.H / a.Hk);
+    if (dq < sm_count) {
+      const int64_t room = sm_count / dq, most = k_tiles / 2;
+      a.parts_dq = (int)(room < most ? room : most);
+    }
+    if (dkv < sm_count) {
+      const int64_t room = (a.H > a.Hk ? 2 : 1) * sm_count / dkv, most = steps / 4;
+      a.parts_dkv = (int)(room < most ? room : most);
+    }
+    if (a.parts_dq < 1) a.parts_dq = 1;
+    if (a.parts_dkv < 1) a.parts_dkv = 1;
+  }
+  const int64_t dq = a.parts_dq > 1 ? (int64_t)a.parts_dq * a.B * a.H * a.Sq * a.D : 0;
+  const int64_t dkv = a.parts_dkv > 1 ? (int64_t)2 * a.parts_dkv * a.B * a.Hk * a.Sk * a.D : 0;
+  AttnScratch need = {dq > dkv ? dq : dkv, 0, 0, 0};
+  if (a.cu_q != nullptr) {
+    need.order_q = max_tiles(a.Sq, a.nseq, 128);
+    need.order_k = max_tiles(a.Sk, a.nseq, 128);
+  }
+  return need;
+}
+
 cudaError_t launch_attention_backward(const AttnArgs& a, cudaStream_t stream) {
   if (a.B <= 0 || a.H <= 0 || (a.Sq <= 0 && a.Sk <= 0)) return cudaSuccess;
-  if (a.Hk <= 0 || a.H % a.Hk != 0 || a.D <= 0 || a.D % 8 != 0 || a.D > kAttnMaxDim || a.Sk < 0 || a.Sq < 0) return cudaErrorInvalidValue;
+  if (a.Hk <= 0 || a.H % a.Hk != 0 || a.D <= 0 || a.D % 8 != 0 || a.D > kAttnMaxDim || a.Sk < 0 || a.Sq < 0 || a.parts_dq < 1 || a.parts_dkv < 1)
+    return cudaErrorInvalidValue;
   if (a.D <= 64) return a.is_bf16 ? launch<64, true>(a, stream) : launch<64, false>(a, stream);
   return a.is_bf16 ? launch<128, true>(a, stream) : launch<128, false>(a, stream);
 }

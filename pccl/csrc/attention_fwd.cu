@@ -61,13 +61,18 @@ __device__ __forceinline__ void mask32(uint32_t* r, int left) {
   for (int e = 0; e < 32; ++e) r[e] = e < left ? r[e] : 0xff800000u;
 }
 
-// The queries of one tile number, and how many key tiles each half of them sees.
+// The queries of one tile number, and the key tiles that each half of them has to do with: n[h] of them from tile j0 on.
 struct Work {
   Span sp;
-  int head, row0, offset, n[2];
+  int head, row0, offset, j0, part, n[2];
 };
 __device__ __forceinline__ Work work_at(const AttnArgs& a, unsigned id, int tiles) {
   Work w;
+  w.part = 0;
+  if (a.parts_o > 1) {
+    w.part = (int)(id % (unsigned)a.parts_o);
+    id /= (unsigned)a.parts_o;
+  }
   if (a.cu_q != nullptr) {
     w.head = (int)(id % (unsigned)a.H);
     w.sp = find_span(a, (int)(id / (unsigned)a.H), 256, false);
@@ -89,6 +94,17 @@ __device__ __forceinline__ Work work_at(const AttnArgs& a, unsigned id, int tile
     const int last = first + 127 < w.sp.len_q - 1 ? first + 127 : w.sp.len_q - 1;
     const int keys = !a.causal ? w.sp.len_k : (last + w.offset + 1 < w.sp.len_k ? last + w.offset + 1 : w.sp.len_k);
     w.n[h] = w.sp.tile >= 0 && first < w.sp.len_q && keys > 0 ? (keys + 127) / 128 : 0;
+  }
+  w.j0 = 0;
+  if (a.parts_o > 1) {                                       // an even share of the longer half's key tiles
+    const int most = w.n[0] > w.n[1] ? w.n[0] : w.n[1];
+    w.j0 = most * w.part / a.parts_o;
+    const int j1 = most * (w.part + 1) / a.parts_o;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int end = w.n[h] < j1 ? w.n[h] : j1;
+      w.n[h] = end > w.j0 ? end - w.j0 : 0;
+    }
   }
   return w;
 }
@@ -160,7 +176,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i < 2 * nmax && ok; ++i, ++it) {     // K0, V0, K1, V1, ...
           const uint32_t st = it % C::kStages, ph = (it / C::kStages) & 1u;
           if (!(ok = wait_warp(b.empty + st, ph ^ 1u, abort_flag))) break;
-          const int row = (i >> 1) * 128;
+          const int row = (w.j0 + (i >> 1)) * 128;
           const bool value = (i & 1) != 0;
           unsigned char* dst = smem + C::kRing + st * C::kTile;
           // the rows behind a packed sequence are its neighbour's
@@ -304,6 +320,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int row = w.row0 + h * 128 + (warp & 3) * 32 + lane;         // within the sequence
       const int keys = !a.causal ? w.sp.len_k : (row + w.offset + 1 < w.sp.len_k ? row + w.offset + 1 : w.sp.len_k);   // that this query sees
       const int keys_all = __shfl_sync(0xffffffffu, keys, 0);           // that every query of the warp sees
+      const int keys_left = keys - w.j0 * 128, all_left = keys_all - w.j0 * 128;      // from the first of its key tiles on
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < n; ++j, ++s_count) {
         if (!(ok = wait_warp(b.s + h, s_count & 1u, abort_flag))) break;
@@ -313,10 +330,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int c = 0; c < 4; ++c) tmem_ld32(t_s + c * 32, s[c]);
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_wait_ld(s[c]);
-        const bool masked = keys_all < (j + 1) * 128;
+        const bool masked = all_left < (j + 1) * 128;
         if (masked) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) mask32(s[c], keys - j * 128 - c * 32);
+          for (int c = 0; c < 4; ++c) mask32(s[c], keys_left - j * 128 - c * 32);
         }
         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -408,9 +425,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = 0;
           }
-          if (exists) store32<BF16>(out, c * 32, a.D, o, inv, wide);
+          if (!exists) continue;
+          if (a.parts_o > 1) store32_f32(part_row(a.partial, w.part, a.B, a.H, a.Sq, a.D, w.sp.batch, w.head, row), c * 32, a.D, o, inv);
+          else store32<BF16>(out, c * 32, a.D, o, inv, wide);
         }
-        if (exists) a.lse[stat_row(a, w.sp.batch, w.head) + w.sp.first_q + row] = none ? -INFINITY : m * a.scale + logf(l);
+        if (exists) {
+          float* lse = a.parts_o > 1 ? a.partial_lse + (int64_t)w.part * a.B * a.H * a.Sq : a.lse;
+          lse[stat_row(a, w.sp.batch, w.head) + w.sp.first_q + row] = none ? -INFINITY : m * a.scale + logf(l);
+        }
       }
       id = next_tile(k);
       if (id < 0) {
@@ -431,6 +453,49 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+__global__ void __launch_bounds__(1024) attention_order_kernel(const __grid_constant__ AttnArgs a) {
+  write_order(a.cu_q, a.nseq, a.Sq, 256, false, a.order_q);
+}
+
+// The parts of one row joined: lse = log(sum of exp(lse_part)), o = sum of exp(lse_part - lse) o_part.  Sixteen lanes per row.
+template <bool BF16>
+__global__ void __launch_bounds__(256) attention_join_kernel(const __grid_constant__ AttnArgs a) {
+  const int sub = threadIdx.x & 15;
+  const int64_t rows = (int64_t)a.B * a.H * a.Sq, r = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 4;
+  if (r >= rows) return;
+  const int64_t bh = r / a.Sq;
+  const int row = (int)(r - bh * a.Sq), b = (int)(bh / a.H), h = (int)(bh - (int64_t)b * a.H);
+  float top = -INFINITY;
+  for (int p = 0; p < a.parts_o; ++p) {
+    const float x = a.partial_lse[p * rows + r];
+    top = x > top || x != x ? x : top;                       // NaN stays
+  }
+  float sum = 0.f, o[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) o[e] = 0.f;
+  const bool on = sub * 8 < a.D;
+  if (top != -INFINITY) {
+    for (int p = 0; p < a.parts_o; ++p) {
+      const float x = a.partial_lse[p * rows + r];
+      if (x == -INFINITY) continue;                          // a part in which this query sees no key
+      const float f = ex2_hw((x - top) * kLog2e);
+      sum += f;
+      if (on) {
+        const float4* v = reinterpret_cast<const float4*>(a.partial + (p * rows + r) * a.D + sub * 8);
+        const float4 u = v[0], w = v[1];
+        o[0] = fmaf(f, u.x, o[0]), o[1] = fmaf(f, u.y, o[1]), o[2] = fmaf(f, u.z, o[2]), o[3] = fmaf(f, u.w, o[3]);
+        o[4] = fmaf(f, w.x, o[4]), o[5] = fmaf(f, w.y, o[5]), o[6] = fmaf(f, w.z, o[6]), o[7] = fmaf(f, w.w, o[7]);
+      }
+    }
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  if (on)
+    *reinterpret_cast<uint4*>(row_ptr(a.o, b, h, row) + sub * 8) =
+        make_uint4(pack2<BF16>(o[0] * inv, o[1] * inv), pack2<BF16>(o[2] * inv, o[3] * inv), pack2<BF16>(o[4] * inv, o[5] * inv),
+                   pack2<BF16>(o[6] * inv, o[7] * inv));
+  if (sub == 0) a.lse[r] = top == -INFINITY ? -INFINITY : top + logf(sum);
+}
+
 template <int DP, bool BF16>
 cudaError_t launch(const AttnArgs& a, cudaStream_t stream) {
   using C = Fwd<DP>;
@@ -448,18 +513,46 @@ cudaError_t launch(const AttnArgs& a, cudaStream_t stream) {
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
-  const int64_t tiles = a.cu_q != nullptr ? a.Sq / 256 + (int64_t)a.nseq + 1 : ((int64_t)a.Sq + 255) / 256;
-  const int64_t ctas = tiles * a.H * (a.cu_q != nullptr ? 1 : a.B);
+  const int64_t tiles = a.cu_q != nullptr ? max_tiles(a.Sq, a.nseq, 256) : ((int64_t)a.Sq + 255) / 256;
+  const int64_t ctas = tiles * a.H * a.B * a.parts_o;
   if (ctas > INT32_MAX) return cudaErrorInvalidValue;
+  if (a.cu_q != nullptr) {
+    attention_order_kernel<<<1, 1024, 0, stream>>>(a);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  }
   kernel<<<(unsigned)ctas, kThreads, C::kSmem, stream>>>(mq, mk, mv, a, (int)tiles);
+  e = cudaGetLastError();
+  if (e != cudaSuccess || a.parts_o == 1) return e;
+  const int64_t blocks = ((int64_t)a.B * a.H * a.Sq + 15) / 16;
+  if (blocks > INT32_MAX) return cudaErrorInvalidValue;
+  attention_join_kernel<BF16><<<(unsigned)blocks, 256, 0, stream>>>(a);
   return cudaGetLastError();
 }
 
 }  // namespace
 
+// A tile's keys are split where the tiles alone leave SMs without work: into as many parts as the device has room for, of two
+// key tiles or more.
+AttnScratch plan_attention_forward(AttnArgs& a, int sm_count) {
+  a.parts_o = 1;
+  const int64_t tiles = ((int64_t)a.Sq + 255) / 256 * a.H * a.B, key_tiles = ((int64_t)a.Sk + 127) / 128;
+  if (a.cu_q == nullptr && tiles > 0 && tiles < sm_count) {
+    const int64_t room = sm_count / tiles, most = key_tiles / 2;
+    a.parts_o = (int)(room < most ? room : most);
+    if (a.parts_o < 1) a.parts_o = 1;
+  }
+  AttnScratch need = {0, 0, 0, 0};
+  if (a.cu_q != nullptr) need.order_q = max_tiles(a.Sq, a.nseq, 256);
+  if (a.parts_o > 1) {
+    need.partial_lse = (int64_t)a.parts_o * a.B * a.H * a.Sq;
+    need.partial = need.partial_lse * a.D;
+  }
+  return need;
+}
+
 cudaError_t launch_attention_forward(const AttnArgs& a, cudaStream_t stream) {
   if (a.B <= 0 || a.H <= 0 || a.Sq <= 0) return cudaSuccess;
-  if (a.Hk <= 0 || a.H % a.Hk != 0 || a.D <= 0 || a.D % 8 != 0 || a.D > kAttnMaxDim || a.Sk < 0) return cudaErrorInvalidValue;
+  if (a.Hk <= 0 || a.H % a.Hk != 0 || a.D <= 0 || a.D % 8 != 0 || a.D > kAttnMaxDim || a.Sk < 0 || a.parts_o < 1) return cudaErrorInvalidValue;
   if (a.D <= 64) return a.is_bf16 ? launch<64, true>(a, stream) : launch<64, false>(a, stream);
   return a.is_bf16 ? launch<128, true>(a, stream) : launch<128, false>(a, stream);
 }

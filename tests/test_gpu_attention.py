@@ -105,6 +105,7 @@ CASES = [
     (1, 640, 640, 2, 2, 8, False, BF), (1, 385, 385, 3, 3, 40, True, FP), (1, 200, 200, 2, 1, 72, False, FP),
     (1, 1, 700, 4, 2, 128, True, BF), (1, 130, 900, 4, 4, 64, True, FP), (2, 700, 100, 2, 2, 128, True, BF),
     (1, 900, 1, 2, 1, 64, True, BF), (1, 65, 1000, 2, 2, 128, False, BF), (3, 1000, 1000, 2, 1, 128, True, BF),
+    (1, 1, 4000, 16, 2, 128, False, BF), (1, 256, 2500, 4, 1, 128, True, BF), (1, 800, 800, 16, 1, 64, True, FP), (2, 40, 3333, 3, 3, 80, True, FP),
     (1, 2048, 2048, 2, 2, 128, True, FP), (1, 2047, 1025, 2, 2, 64, False, BF), (1, 1500, 1500, 2, 2, 96, True, BF),
 ]
 
@@ -139,7 +140,7 @@ def test_backward_matches_formula(case):
 PACKED = [
     ([(1, 1)], 0, 1, 1, 64, True), ([(5, 5), (0, 0), (130, 130), (1, 1), (128, 128), (257, 257)], 7, 4, 2, 128, True),
     ([(300, 300), (0, 40), (40, 0), (77, 500), (129, 64)], 130, 2, 1, 64, True), ([(33, 33)] * 40, 3, 2, 2, 80, False),
-    ([(0, 0), (0, 0)], 300, 2, 2, 128, True), ([(700, 300), (300, 700)], 1, 4, 4, 128, True), ([(7, 7), (2, 2)] * 37, 0, 3, 1, 40, True),
+    ([(0, 0), (0, 0)], 300, 2, 2, 128, True), ([(1 + i % 7, 1 + i % 7) for i in range(150)] + [(0, 0)] * 60 + [(400, 400)], 9, 2, 1, 64, True), ([(700, 300), (300, 700)], 1, 4, 4, 128, True), ([(7, 7), (2, 2)] * 37, 0, 3, 1, 40, True),
 ]
 
 
