@@ -51,6 +51,8 @@ __device__ __forceinline__ float dot8(const uint4& x, const uint4& y) {
 // A block takes 64 rows of one head, a warp eight of them, two at once; all loads first.
 template <bool BF16>
 __global__ void __launch_bounds__(256) attention_delta_kernel(const __grid_constant__ AttnArgs a) {
+  pdl_wait();
+  pdl_trigger();
   const int sub = threadIdx.x & 15, half = (threadIdx.x >> 4) & 1, warp = threadIdx.x >> 5;
   const int s0 = (int)blockIdx.x * 64 + warp * 8 + half, h = (int)blockIdx.y, b = (int)blockIdx.z;
   const bool on = sub * 8 < a.D;
@@ -73,6 +75,8 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(const __grid_const
 }
 
 __global__ void __launch_bounds__(1024) attention_orders_kernel(const __grid_constant__ AttnArgs a) {
+  pdl_wait();
+  pdl_trigger();
   if (blockIdx.x == 0) write_order(a.cu_k, a.nseq, a.Sk, 128, true, a.order_k);
   else write_order(a.cu_q, a.nseq, a.Sq, 128, false, a.order_q);
 }
@@ -108,10 +112,11 @@ struct DkvWork {
   Span sp;
   int kv_head, key0, offset, first, per_head, part, i0, total;
 };
+template <bool SPLIT>
 __device__ __forceinline__ DkvWork dkv_work_at(const AttnArgs& a, unsigned id) {
   DkvWork w;
   w.part = 0;
-  if (a.parts_dkv > 1) {
+  if constexpr (SPLIT) {
     w.part = (int)(id % (unsigned)a.parts_dkv);
     id /= (unsigned)a.parts_dkv;
   }
@@ -135,14 +140,14 @@ __device__ __forceinline__ DkvWork dkv_work_at(const AttnArgs& a, unsigned id) {
   w.per_head = w.sp.tile >= 0 && tiles > w.first ? tiles - w.first : 0;
   w.i0 = 0;
   w.total = a.H / a.Hk * w.per_head;
-  if (a.parts_dkv > 1) {
+  if constexpr (SPLIT) {
     w.i0 = (int)((int64_t)w.total * w.part / a.parts_dkv);
     w.total = (int)((int64_t)w.total * (w.part + 1) / a.parts_dkv) - w.i0;
   }
   return w;
 }
 
-template <int DP, bool BF16>
+template <int DP, bool BF16, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
     attention_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                          const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do,
@@ -193,6 +198,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   fence_after();
   const uint32_t tmem = b.tmem;
+  pdl_wait();
+  pdl_trigger();                                             // behind the wait: see the dq kernel
 
   // The tile after the k-th, for every role alike: -1 none, -2 a wait gave up.  Whole warps.
   auto next_tile = [&](int k) {
@@ -220,7 +227,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int k = 0; ok; ++k) {
         if (k >= 2 && !(ok = wait_warp(b.next_empty + (k & 1), ((k >> 1) - 1) & 1u, abort_flag))) break;
         if (lane == 0) ask_for_work(b.next + (k & 1), b.next_full + (k & 1));
-        const DkvWork w = dkv_work_at(a, (unsigned)id);
+        const DkvWork w = dkv_work_at<SPLIT>(a, (unsigned)id);
         for (int i = 0; i < w.total && ok; ++i, ++n) {
           const int hg = (w.i0 + i) / w.per_head, head = w.kv_head * group + hg, row = (w.first + w.i0 + i - hg * w.per_head) * 128;
           // the rows behind a packed sequence are its neighbour's, and both tiles are contracted along their rows
@@ -270,7 +277,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t n = 0, items = 0;
       int id = (int)blockIdx.x;
       for (int k = 0;; ++k) {
-        const DkvWork w = dkv_work_at(a, (unsigned)id);
+        const DkvWork w = dkv_work_at<SPLIT>(a, (unsigned)id);
         if (w.total > 0) {
           auto q_at = [&](uint32_t m) { return q_ring + (m % C::kNq) * C::kTile; };
           auto do_at = [&](uint32_t m) { return do_ring + (m % C::kNdo) * C::kTile; };
@@ -339,7 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t n = 0;
       int id = (int)blockIdx.x;
       for (int k = 0; ok; ++k) {
-        const DkvWork w = dkv_work_at(a, (unsigned)id);
+        const DkvWork w = dkv_work_at<SPLIT>(a, (unsigned)id);
         for (int i = 0; i < w.total; ++i, ++n) {
           const int hg = (w.i0 + i) / w.per_head, head = w.kv_head * group + hg, row = (w.first + w.i0 + i - hg * w.per_head) * 128;
           const int64_t at = stat_row(a, w.sp.batch, head) + w.sp.first_q;
@@ -380,7 +387,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t n = 0, items = 0;
     int id = (int)blockIdx.x;
     for (int k = 0; ok; ++k) {
-      const DkvWork w = dkv_work_at(a, (unsigned)id);
+      const DkvWork w = dkv_work_at<SPLIT>(a, (unsigned)id);
       const int key = w.key0 + (warp & 3) * 32 + lane;
       int tile = w.first + (w.per_head > 0 ? w.i0 % w.per_head : 0);            // query tile within its head
       for (int i = 0; i < w.total; ++i, ++n) {
@@ -494,7 +501,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           if (!exists) continue;
-          if (a.parts_dkv > 1) {
+          if constexpr (SPLIT) {
             // dv's parts first, then dk's
             float* sums = part_row(a.partial, keys_grad ? a.parts_dkv + w.part : w.part, a.B, a.Hk, a.Sk, a.D, w.sp.batch, w.kv_head, key);
             store32_f32(sums, col0 + c * 32, a.D, o, keys_grad ? a.scale : 1.f);
@@ -544,10 +551,11 @@ struct DqWork {
   Span sp;
   int head, row0, offset, part, j0, n;
 };
+template <bool SPLIT>
 __device__ __forceinline__ DqWork dq_work_at(const AttnArgs& a, unsigned id, int tiles) {
   DqWork w;
   w.part = 0;
-  if (a.parts_dq > 1) {
+  if constexpr (SPLIT) {
     w.part = (int)(id % (unsigned)a.parts_dq);
     id /= (unsigned)a.parts_dq;
   }
@@ -569,18 +577,18 @@ __device__ __forceinline__ DqWork dq_work_at(const AttnArgs& a, unsigned id, int
   const int keys = !a.causal ? w.sp.len_k : (last + w.offset + 1 < w.sp.len_k ? last + w.offset + 1 : w.sp.len_k);
   w.n = w.sp.tile >= 0 && keys > 0 ? (keys + 127) / 128 : 0;
   w.j0 = 0;
-  if (a.parts_dq > 1) {
+  if constexpr (SPLIT) {
     w.j0 = w.n * w.part / a.parts_dq;
     w.n = w.n * (w.part + 1) / a.parts_dq - w.j0;
   }
   return w;
 }
 
-template <int DP, bool BF16>
+template <int DP, bool BF16, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
     attention_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                         const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do,
-                        const __grid_constant__ AttnArgs a, int tiles) {
+                        const __grid_constant__ AttnArgs a, int tiles, bool beside) {
   using C = Dq<DP>;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -621,6 +629,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   fence_after();
   const uint32_t tmem = b.tmem;
+  // beside: the kernel in front is the one for dk and dv, which shares nothing with this one but what both read.  All of that,
+  // the row sums among it, was complete when its blocks let this one's in, so these begin on the SMs that it leaves, and wait
+  // for it at their end.
+  if (!beside) pdl_wait();
 
   // The tile after the k-th, for every role alike: -1 none, -2 a wait gave up.  Whole warps.
   auto next_tile = [&](int k) {
@@ -648,7 +660,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int k = 0; ok; ++k) {
         if (k >= 2 && !(ok = wait_warp(b.next_empty + (k & 1), ((k >> 1) - 1) & 1u, abort_flag))) break;
         if (lane == 0) ask_for_work(b.next + (k & 1), b.next_full + (k & 1));
-        const DqWork w = dq_work_at(a, (unsigned)id, tiles);
+        const DqWork w = dq_work_at<SPLIT>(a, (unsigned)id, tiles);
         const int kv_head = w.head / (a.H / a.Hk);
         for (int j = 0; j < w.n; ++j, ++n) {
           const uint32_t ks = n % C::kK, vs = n % C::kV;
@@ -706,7 +718,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t n = 0, items = 0;
       int id = (int)blockIdx.x;
       for (int k = 0;; ++k) {
-        const DqWork w = dq_work_at(a, (unsigned)id, tiles);
+        const DqWork w = dq_work_at<SPLIT>(a, (unsigned)id, tiles);
         if (w.n > 0) {
           auto scores = [&](int j) {
             const uint32_t m = n + (uint32_t)j;
@@ -779,7 +791,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t n = 0, items = 0;
     int id = (int)blockIdx.x;
     for (int k = 0; ok; ++k) {
-      const DqWork w = dq_work_at(a, (unsigned)id, tiles);
+      const DqWork w = dq_work_at<SPLIT>(a, (unsigned)id, tiles);
       const int row = w.row0 + (warp & 3) * 32 + lane;
       const bool exists = w.sp.tile >= 0 && row < w.sp.len_q;
       float lse2 = INFINITY, delta = 0.f;
@@ -872,7 +884,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             }
             if (!exists) continue;
-            if (a.parts_dq > 1) store32_f32(part_row(a.partial, w.part, a.B, a.H, a.Sq, a.D, w.sp.batch, w.head, row), col, a.D, o, a.scale);
+            if constexpr (SPLIT) store32_f32(part_row(a.partial, w.part, a.B, a.H, a.Sq, a.D, w.sp.batch, w.head, row), col, a.D, o, a.scale);
             else store32<BF16>(out, col, a.D, o, a.scale, wide);
           }
         }
@@ -883,6 +895,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (!ok) fail(kErrCompute);
   }
+  if (beside) pdl_wait();
   fence_before();
   __syncthreads();
   if (warp == kCompute + 1) {
@@ -894,6 +907,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 // A gradient from its parts, added up in order: dst = sum of `parts` arrays of [batch][head][row][D].  Sixteen lanes per row.
 template <bool BF16>
 __global__ void __launch_bounds__(256) attention_sum_kernel(const float* partial, int parts, AttnTensor dst, int B, int H, int S, int D) {
+  pdl_wait();
+  pdl_trigger();
   const int sub = threadIdx.x & 15;
   const int64_t rows = (int64_t)B * H * S, r = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 4;
   if (r >= rows || sub * 8 >= D) return;
@@ -915,8 +930,7 @@ template <bool BF16>
 cudaError_t add_parts(const float* partial, int parts, const AttnTensor& dst, int B, int H, int S, int D, cudaStream_t stream) {
   const int64_t blocks = ((int64_t)B * H * S + 15) / 16;
   if (blocks > INT32_MAX) return cudaErrorInvalidValue;
-  attention_sum_kernel<BF16><<<(unsigned)blocks, 256, 0, stream>>>(partial, parts, dst, B, H, S, D);
-  return cudaGetLastError();
+  return launch_pdl(attention_sum_kernel<BF16>, dim3((unsigned)blocks), dim3(256), 0, stream, partial, parts, dst, B, H, S, D);
 }
 
 // The shared-memory limit is an attribute of the function on the current device.
@@ -932,6 +946,29 @@ cudaError_t allow_smem(uint32_t bytes) {
   return e;
 }
 
+template <int DP, bool BF16, bool SPLIT>
+cudaError_t launch_dkv(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mdo, const AttnArgs& a,
+                       cudaStream_t stream) {
+  const cudaError_t e = allow_smem<attention_dkv_kernel<DP, BF16, SPLIT>>(Dkv<DP>::kSmem);
+  if (e != cudaSuccess) return e;
+  const int64_t tiles = a.cu_q != nullptr ? max_tiles(a.Sk, a.nseq, 128) : ((int64_t)a.Sk + 127) / 128;
+  const int64_t ctas = tiles * a.Hk * a.B * a.parts_dkv;
+  if (ctas > INT32_MAX) return cudaErrorInvalidValue;
+  return launch_pdl(attention_dkv_kernel<DP, BF16, SPLIT>, dim3((unsigned)ctas), dim3(kThreads), Dkv<DP>::kSmem, stream, mq, mk, mv, mdo, a);
+}
+template <int DP, bool BF16, bool SPLIT>
+cudaError_t launch_dq(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mdo, const AttnArgs& a,
+                      cudaStream_t stream) {
+  const cudaError_t e = allow_smem<attention_dq_kernel<DP, BF16, SPLIT>>(Dq<DP>::kSmem);
+  if (e != cudaSuccess) return e;
+  const int64_t tiles = a.cu_q != nullptr ? max_tiles(a.Sq, a.nseq, 128) : ((int64_t)a.Sq + 127) / 128;
+  const int64_t ctas = tiles * a.H * a.B * a.parts_dq;
+  if (ctas > INT32_MAX) return cudaErrorInvalidValue;
+  const bool beside = a.Sk > 0 && a.parts_dkv == 1;          // the dk/dv kernel is right in front, and no part of its work is in this one's memory
+  return launch_pdl(attention_dq_kernel<DP, BF16, SPLIT>, dim3((unsigned)ctas), dim3(kThreads), Dq<DP>::kSmem, stream, mq, mk, mv, mdo, a,
+                    (int)tiles, beside);
+}
+
 template <int DP, bool BF16>
 cudaError_t launch(const AttnArgs& a, cudaStream_t stream) {
   const bool packed = a.cu_q != nullptr;
@@ -943,24 +980,18 @@ cudaError_t launch(const AttnArgs& a, cudaStream_t stream) {
   if (a.Sq == 0) mq = mdo = mk;                              // nothing of what is missing is ever loaded
   if (a.Sk == 0) mk = mv = mq;
   if (packed) {
-    attention_orders_kernel<<<2, 1024, 0, stream>>>(a);
-    const cudaError_t e = cudaGetLastError();
+    const cudaError_t e = launch_pdl(attention_orders_kernel, dim3(2), dim3(1024), 0, stream, a);
     if (e != cudaSuccess) return e;
   }
   if (a.Sq > 0) {
     if (a.B > 65535) return cudaErrorInvalidValue;
-    attention_delta_kernel<BF16><<<dim3((unsigned)((a.Sq + 63) / 64), (unsigned)a.H, (unsigned)a.B), 256, 0, stream>>>(a);
-    const cudaError_t e = cudaGetLastError();
+    const cudaError_t e = launch_pdl(attention_delta_kernel<BF16>, dim3((unsigned)((a.Sq + 63) / 64), (unsigned)a.H, (unsigned)a.B), dim3(256), 0,
+                                     stream, a);
     if (e != cudaSuccess) return e;
   }
   if (a.Sk > 0) {
-    cudaError_t e = allow_smem<attention_dkv_kernel<DP, BF16>>(Dkv<DP>::kSmem);
+    cudaError_t e = a.parts_dkv > 1 ? launch_dkv<DP, BF16, true>(mq, mk, mv, mdo, a, stream) : launch_dkv<DP, BF16, false>(mq, mk, mv, mdo, a, stream);
     if (e != cudaSuccess) return e;
-    const int64_t tiles = packed ? max_tiles(a.Sk, a.nseq, 128) : ((int64_t)a.Sk + 127) / 128;
-    const int64_t ctas = tiles * a.Hk * a.B * a.parts_dkv;
-    if (ctas > INT32_MAX) return cudaErrorInvalidValue;
-    attention_dkv_kernel<DP, BF16><<<(unsigned)ctas, kThreads, Dkv<DP>::kSmem, stream>>>(mq, mk, mv, mdo, a);
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
     if (a.parts_dkv > 1) {
       if ((e = add_parts<BF16>(a.partial, a.parts_dkv, a.dv, a.B, a.Hk, a.Sk, a.D, stream)) != cudaSuccess) return e;
       const float* dk = a.partial + (int64_t)a.parts_dkv * a.B * a.Hk * a.Sk * a.D;
@@ -968,13 +999,8 @@ cudaError_t launch(const AttnArgs& a, cudaStream_t stream) {
     }
   }
   if (a.Sq > 0) {
-    cudaError_t e = allow_smem<attention_dq_kernel<DP, BF16>>(Dq<DP>::kSmem);
+    cudaError_t e = a.parts_dq > 1 ? launch_dq<DP, BF16, true>(mq, mk, mv, mdo, a, stream) : launch_dq<DP, BF16, false>(mq, mk, mv, mdo, a, stream);
     if (e != cudaSuccess) return e;
-    const int64_t tiles = packed ? max_tiles(a.Sq, a.nseq, 128) : ((int64_t)a.Sq + 127) / 128;
-    const int64_t ctas = tiles * a.H * a.B * a.parts_dq;
-    if (ctas > INT32_MAX) return cudaErrorInvalidValue;
-    attention_dq_kernel<DP, BF16><<<(unsigned)ctas, kThreads, Dq<DP>::kSmem, stream>>>(mq, mk, mv, mdo, a, (int)tiles);
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
     if (a.parts_dq > 1 && (e = add_parts<BF16>(a.partial, a.parts_dq, a.dq, a.B, a.H, a.Sq, a.D, stream)) != cudaSuccess) return e;
   }
   return cudaSuccess;

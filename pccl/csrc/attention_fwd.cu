@@ -66,10 +66,11 @@ struct Work {
   Span sp;
   int head, row0, offset, j0, part, n[2];
 };
+template <bool SPLIT>
 __device__ __forceinline__ Work work_at(const AttnArgs& a, unsigned id, int tiles) {
   Work w;
   w.part = 0;
-  if (a.parts_o > 1) {
+  if constexpr (SPLIT) {
     w.part = (int)(id % (unsigned)a.parts_o);
     id /= (unsigned)a.parts_o;
   }
@@ -96,7 +97,7 @@ __device__ __forceinline__ Work work_at(const AttnArgs& a, unsigned id, int tile
     w.n[h] = w.sp.tile >= 0 && first < w.sp.len_q && keys > 0 ? (keys + 127) / 128 : 0;
   }
   w.j0 = 0;
-  if (a.parts_o > 1) {                                       // an even share of the longer half's key tiles
+  if constexpr (SPLIT) {                                     // an even share of the longer half's key tiles
     const int most = w.n[0] > w.n[1] ? w.n[0] : w.n[1];
     w.j0 = most * w.part / a.parts_o;
     const int j1 = most * (w.part + 1) / a.parts_o;
@@ -109,7 +110,7 @@ __device__ __forceinline__ Work work_at(const AttnArgs& a, unsigned id, int tile
   return w;
 }
 
-template <int DP, bool BF16>
+template <int DP, bool BF16, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
     attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                          const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttnArgs a, int tiles) {
@@ -146,6 +147,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   fence_after();
   const uint32_t tmem = b.tmem;
+  pdl_wait();
+  pdl_trigger();
 
   // The tile after the k-th, for every role alike: -1 none, -2 a wait gave up.  Whole warps.
   auto next_tile = [&](int k) {
@@ -171,7 +174,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           break;
         }
         if (lane == 0) ask_for_work(b.next + (k & 1), b.next_full + (k & 1));
-        const Work w = work_at(a, (unsigned)id, tiles);
+        const Work w = work_at<SPLIT>(a, (unsigned)id, tiles);
         const int kv_head = w.head / (a.H / a.Hk), nmax = w.n[0] > w.n[1] ? w.n[0] : w.n[1];
         for (int i = 0; i < 2 * nmax && ok; ++i, ++it) {     // K0, V0, K1, V1, ...
           const uint32_t st = it % C::kStages, ph = (it / C::kStages) & 1u;
@@ -226,7 +229,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t it = 0, s_count[2] = {0, 0}, items[2] = {0, 0};     // ring position; tiles and work items of each half
       int id = (int)blockIdx.x;
       for (int k = 0;; ++k) {
-        const Work w = work_at(a, (unsigned)id, tiles);
+        const Work w = work_at<SPLIT>(a, (unsigned)id, tiles);
         const int nmax = w.n[0] > w.n[1] ? w.n[0] : w.n[1];
         if (nmax > 0) {
           auto tile_at = [&](uint32_t i) { return ring + (i % C::kStages) * C::kTile; };
@@ -315,7 +318,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t s_count = 0, items = 0;
     int id = (int)blockIdx.x;
     for (int k = 0;; ++k) {
-      const Work w = work_at(a, (unsigned)id, tiles);
+      const Work w = work_at<SPLIT>(a, (unsigned)id, tiles);
       const int n = h == 0 ? w.n[0] : w.n[1];
       const int row = w.row0 + h * 128 + (warp & 3) * 32 + lane;         // within the sequence
       const int keys = !a.causal ? w.sp.len_k : (row + w.offset + 1 < w.sp.len_k ? row + w.offset + 1 : w.sp.len_k);   // that this query sees
@@ -426,11 +429,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int e = 0; e < 32; ++e) o[e] = 0;
           }
           if (!exists) continue;
-          if (a.parts_o > 1) store32_f32(part_row(a.partial, w.part, a.B, a.H, a.Sq, a.D, w.sp.batch, w.head, row), c * 32, a.D, o, inv);
+          if constexpr (SPLIT) store32_f32(part_row(a.partial, w.part, a.B, a.H, a.Sq, a.D, w.sp.batch, w.head, row), c * 32, a.D, o, inv);
           else store32<BF16>(out, c * 32, a.D, o, inv, wide);
         }
         if (exists) {
-          float* lse = a.parts_o > 1 ? a.partial_lse + (int64_t)w.part * a.B * a.H * a.Sq : a.lse;
+          float* lse = SPLIT ? a.partial_lse + (int64_t)w.part * a.B * a.H * a.Sq : a.lse;
           lse[stat_row(a, w.sp.batch, w.head) + w.sp.first_q + row] = none ? -INFINITY : m * a.scale + logf(l);
         }
       }
@@ -454,12 +457,16 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 __global__ void __launch_bounds__(1024) attention_order_kernel(const __grid_constant__ AttnArgs a) {
+  pdl_wait();
+  pdl_trigger();
   write_order(a.cu_q, a.nseq, a.Sq, 256, false, a.order_q);
 }
 
 // The parts of one row joined: lse = log(sum of exp(lse_part)), o = sum of exp(lse_part - lse) o_part.  Sixteen lanes per row.
 template <bool BF16>
 __global__ void __launch_bounds__(256) attention_join_kernel(const __grid_constant__ AttnArgs a) {
+  pdl_wait();
+  pdl_trigger();
   const int sub = threadIdx.x & 15;
   const int64_t rows = (int64_t)a.B * a.H * a.Sq, r = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 4;
   if (r >= rows) return;
@@ -496,14 +503,14 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const __grid_consta
   if (sub == 0) a.lse[r] = top == -INFINITY ? -INFINITY : top + logf(sum);
 }
 
-template <int DP, bool BF16>
+template <int DP, bool BF16, bool SPLIT>
 cudaError_t launch(const AttnArgs& a, cudaStream_t stream) {
   using C = Fwd<DP>;
   CUtensorMap mq, mk, mv;
   if (!make_map(&mq, a.q, BF16, a.D, a.H, a.Sq, a.B)) return cudaErrorInvalidValue;
   if (a.Sk == 0) mk = mv = mq;                               // no key is ever loaded
   else if (!make_map(&mk, a.k, BF16, a.D, a.Hk, a.Sk, a.B) || !make_map(&mv, a.v, BF16, a.D, a.Hk, a.Sk, a.B)) return cudaErrorInvalidValue;
-  auto kernel = attention_fwd_kernel<DP, BF16>;
+  auto kernel = attention_fwd_kernel<DP, BF16, SPLIT>;
   static thread_local bool configured[64] = {false};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -517,16 +524,18 @@ cudaError_t launch(const AttnArgs& a, cudaStream_t stream) {
   const int64_t ctas = tiles * a.H * a.B * a.parts_o;
   if (ctas > INT32_MAX) return cudaErrorInvalidValue;
   if (a.cu_q != nullptr) {
-    attention_order_kernel<<<1, 1024, 0, stream>>>(a);
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    if ((e = launch_pdl(attention_order_kernel, dim3(1), dim3(1024), 0, stream, a)) != cudaSuccess) return e;
   }
-  kernel<<<(unsigned)ctas, kThreads, C::kSmem, stream>>>(mq, mk, mv, a, (int)tiles);
-  e = cudaGetLastError();
-  if (e != cudaSuccess || a.parts_o == 1) return e;
+  e = launch_pdl(kernel, dim3((unsigned)ctas), dim3(kThreads), C::kSmem, stream, mq, mk, mv, a, (int)tiles);
+  if (e != cudaSuccess || !SPLIT) return e;
   const int64_t blocks = ((int64_t)a.B * a.H * a.Sq + 15) / 16;
   if (blocks > INT32_MAX) return cudaErrorInvalidValue;
-  attention_join_kernel<BF16><<<(unsigned)blocks, 256, 0, stream>>>(a);
-  return cudaGetLastError();
+  return launch_pdl(attention_join_kernel<BF16>, dim3((unsigned)blocks), dim3(256), 0, stream, a);
+}
+
+template <int DP, bool BF16>
+cudaError_t launch_type(const AttnArgs& a, cudaStream_t stream) {
+  return a.parts_o > 1 ? launch<DP, BF16, true>(a, stream) : launch<DP, BF16, false>(a, stream);
 }
 
 }  // namespace
@@ -553,8 +562,8 @@ AttnScratch plan_attention_forward(AttnArgs& a, int sm_count) {
 cudaError_t launch_attention_forward(const AttnArgs& a, cudaStream_t stream) {
   if (a.B <= 0 || a.H <= 0 || a.Sq <= 0) return cudaSuccess;
   if (a.Hk <= 0 || a.H % a.Hk != 0 || a.D <= 0 || a.D % 8 != 0 || a.D > kAttnMaxDim || a.Sk < 0 || a.parts_o < 1) return cudaErrorInvalidValue;
-  if (a.D <= 64) return a.is_bf16 ? launch<64, true>(a, stream) : launch<64, false>(a, stream);
-  return a.is_bf16 ? launch<128, true>(a, stream) : launch<128, false>(a, stream);
+  if (a.D <= 64) return a.is_bf16 ? launch_type<64, true>(a, stream) : launch_type<64, false>(a, stream);
+  return a.is_bf16 ? launch_type<128, true>(a, stream) : launch_type<128, false>(a, stream);
 }
 
 }  // namespace pccl
