@@ -142,7 +142,7 @@ __device__ __forceinline__ F2 decode2(const F2& c, const F2& unit) {
   if constexpr (SIGNED) {
     float x, y;
     split(c, x, y);
-    return unit * (f2(fabsf(x), fabsf(y)) * c);
+    return unit * f2(fabsf(x) * x, fabsf(y) * y);
   } else {
     const F2 c2 = c * c;
     return unit * (c2 * c2);
@@ -171,37 +171,34 @@ __device__ __forceinline__ float root_hw(float x) {
 // the root lies within 2^-16 of a whole number, the comparison moves it to the right neighbour all the same, but for noise
 // within 2^-16 of 0 or 1.
 template <bool SIGNED>
-__device__ __forceinline__ void encode2(const F2& x, const F2& inv, const F2& u, float& r0, float& r1) {
+__device__ __forceinline__ void encode2(const F2& x, const F2& inv, const F2& u, bool zeros, float& r0, float& r1) {
   constexpr float top = SIGNED ? 127.f : 255.f;
   float x0, x1, y0, y1;
   split(x, x0, x1);
-  const F2 y = (f2(fabsf(x0), fabsf(x1)) * inv) * f2(SIGNED ? kSigned : kUnsigned);
-  split(y, y0, y1);
-  y0 = root_hw(y0);
-  y1 = root_hw(y1);
+  split((x * inv) * f2(SIGNED ? kSigned : kUnsigned), y0, y1);
+  float c0 = root_hw(fabsf(y0)), c1 = root_hw(fabsf(y1));
   if constexpr (!SIGNED) {
-    y0 = root_hw(y0);
-    y1 = root_hw(y1);
+    c0 = root_hw(c0);
+    c1 = root_hw(c1);
   }
-  const F2 c = f2(__fadd_rz(y0, 8388608.f), __fadd_rz(y1, 8388608.f)) + f2(-8388608.f);
-  const F2 c1 = c + f2(1.f), lo = power2<SIGNED>(c);
-  const F2 minus = f2(-1.f);
-  const F2 step = u * fma2(lo, minus, power2<SIGNED>(c1)), part = fma2(lo, minus, y);     // times -1 is exact: a subtraction
-  float s0, s1, p0, p1, a0, a1, b0, b1;
+  const F2 c = f2(__fadd_rz(c0, 8388608.f), __fadd_rz(c1, 8388608.f)) + f2(-8388608.f);
+  const F2 next = c + f2(1.f), lo = power2<SIGNED>(c);
+  const F2 step = u * fma2(lo, f2(-1.f), power2<SIGNED>(next));           // times -1 is exact: a subtraction
+  float l0, l1, s0, s1, a0, a1, b0, b1;
+  split(lo, l0, l1);
   split(step, s0, s1);
-  split(part, p0, p1);
   split(c, a0, a1);
-  split(c1, b0, b1);
-  a0 = fminf(s0 < p0 ? b0 : a0, top);
-  a1 = fminf(s1 < p1 ? b1 : a1, top);
+  split(next, b0, b1);
+  a0 = fminf(s0 < __fsub_rn(fabsf(y0), l0) ? b0 : a0, top);
+  a1 = fminf(s1 < __fsub_rn(fabsf(y1), l1) ? b1 : a1, top);
   if constexpr (SIGNED) {
     r0 = copysignf(a0, x0) + 12582912.f;
     r1 = copysignf(a1, x1) + 12582912.f;
   } else {
-    float i0, i1;
-    split(inv, i0, i1);                                          // both halves are the block's
-    r0 = (x0 > 0.f && i0 > 0.f ? fmaxf(a0, 1.f) : a0) + 8388608.f;
-    r1 = (x1 > 0.f && i0 > 0.f ? fmaxf(a1, 1.f) : a1) + 8388608.f;
+    // not below 1 where x is not zero (its bits as a number, at most 1) and the block is not held as zeros
+    const uint32_t most = zeros ? 0u : 1u;
+    r0 = __uint_as_float(max(__float_as_uint(a0 + 8388608.f), 0x4B000000u + min(__float_as_uint(x0), most)));
+    r1 = __uint_as_float(max(__float_as_uint(a1 + 8388608.f), 0x4B000000u + min(__float_as_uint(x1), most)));
   }
 }
 __device__ __forceinline__ uint32_t bytes4(float a, float b, float c, float d) {
@@ -214,21 +211,70 @@ __device__ __forceinline__ float noise_lo(uint32_t h) { return __uint_as_float((
 
 // The block's largest size: sizes are not negative, so their bits are in the order of their values, infinities and NaN on top.
 __device__ __forceinline__ float block_max(const F2* x) {
-  uint32_t m = 0;
+  float top = 0.f;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     float a, b;
     split(x[i], a, b);
-    m = max(m, max(__float_as_uint(fabsf(a)), __float_as_uint(fabsf(b))));
+    asm("max.NaN.abs.f32 %0, %0, %1, %2;" : "+f"(top) : "f"(a), "f"(b));
   }
+  uint32_t m = __float_as_uint(fabsf(top));
   m = __reduce_max_sync(0xffffffffu, m);
   const float f = __uint_as_float(m);
   return m >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : (f < kLeast ? 0.f : f);
 }
 
+// Where a block lies, and what is read of it.  The loads of a warp's next block are on their way while it works on this one.
+template <bool BITS8>
+struct Block {
+  int k;                                                       // tensor
+  int64_t at;                                                  // place of the lane's first element within it
+  uint64_t sblk;                                               // place within the state
+  bool whole;                                                  // 256 elements on vector boundaries; the same for the whole warp
+  Raw8 g, p;
+  uint2 cm, cv;                                                // 8 bits
+  float m_scale, v_scale;
+};
+template <int PT>
+__device__ __forceinline__ void* weights_of(const AdamTensor& t) {
+  return PT == kAdamF32 ? t.param : static_cast<void*>(t.master);
+}
 template <int PT, int GT, bool BITS8, int MAX>
-__global__ void __launch_bounds__(kThreads, 4) adamw_multi_kernel(const __grid_constant__ AdamMultiArgs a,
-                                                               const __grid_constant__ Table<MAX> table) {
+__device__ __forceinline__ void fetch(const AdamMultiArgs& a, const Table<MAX>& table, uint32_t blk, int k, Block<BITS8>& x) {
+  // the last tensor that starts at or before this block: mostly the last block's, else one behind it
+  if (k + 1 < table.count && table.t[k + 1].first <= blk) {
+    int hi = table.count;
+    while (hi - k > 1) {
+      const int mid = (k + hi) >> 1;
+      if (table.t[mid].first <= blk) k = mid;
+      else hi = mid;
+    }
+  }
+  const AdamTensor& t = table.t[k];
+  const int lane = threadIdx.x & 31;
+  x.k = k;
+  x.at = (int64_t)(blk - t.first) * kAdamBlock + lane * 8;
+  x.sblk = a.first_block + blk;
+  const void* weights = weights_of<PT>(t);
+  const uintptr_t bad = (reinterpret_cast<uintptr_t>(weights) & 31u) | (reinterpret_cast<uintptr_t>(t.grad) & (GT == kAdamF32 ? 31u : 15u)) |
+                        (PT == kAdamF32 ? 0u : reinterpret_cast<uintptr_t>(t.param) & 15u);
+  x.whole = bad == 0 && x.at - lane * 8 + kAdamBlock <= t.n;
+  if (x.whole) {
+    load8<GT>(t.grad, x.at, x.g);
+    load8<kAdamF32>(weights, x.at, x.p);
+  }
+  if constexpr (BITS8) {                                       // the state's blocks are whole: behind a tensor's end they hold zeros
+    const uint64_t si = x.sblk * kAdamBlock + (uint64_t)lane * 8;
+    x.cm = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.m) + si));
+    x.cv = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.v) + si));
+    x.m_scale = a.m_scale[x.sblk];
+    x.v_scale = a.v_scale[x.sblk];
+  }
+}
+
+template <int PT, int GT, bool BITS8, int MAX>
+__global__ void __launch_bounds__(kThreads, BITS8 ? 4 : 3) adamw_multi_kernel(const __grid_constant__ AdamMultiArgs a,
+                                                                              const __grid_constant__ Table<MAX> table) {
   pdl_wait();
   pdl_trigger();
   const int lane = threadIdx.x & 31;
@@ -239,92 +285,83 @@ __global__ void __launch_bounds__(kThreads, 4) adamw_multi_kernel(const __grid_c
     gs = clip >= 1.f ? gs : gs * clip;                   // a norm that is NaN makes every gradient NaN
   }
   const uint32_t warps = gridDim.x * (kThreads / 32);
-  int k = 0;
-  for (uint32_t blk = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); blk < a.blocks; blk += warps) {
-    // the last tensor that starts at or before this block: its tensor is at or behind the last block's
-    int hi = table.count;
-    while (hi - k > 1) {
-      const int mid = (k + hi) >> 1;
-      if (table.t[mid].first <= blk) k = mid;
-      else hi = mid;
-    }
-    const AdamTensor& t = table.t[k];
-    const int64_t at = (int64_t)(blk - t.first) * kAdamBlock + lane * 8;       // place within the tensor
-    const uint64_t sblk = a.first_block + blk;
-    const uint64_t si = sblk * kAdamBlock + (uint64_t)lane * 8;                // place within the state
-    void* weights = PT == kAdamF32 ? t.param : static_cast<void*>(t.master);
-    const uintptr_t bad = (reinterpret_cast<uintptr_t>(weights) & 31u) | (reinterpret_cast<uintptr_t>(t.grad) & (GT == kAdamF32 ? 31u : 15u)) |
-                          (PT == kAdamF32 ? 0u : reinterpret_cast<uintptr_t>(t.param) & 15u);
-    const bool whole = bad == 0 && at - lane * 8 + kAdamBlock <= t.n;          // the same for the whole warp
-    // ---- loads
+  uint32_t blk = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+  if (blk >= a.blocks) return;
+  Block<BITS8> x;
+  fetch<PT, GT, BITS8, MAX>(a, table, blk, 0, x);
+  for (;;) {
+    const AdamTensor& t = table.t[x.k];
+    void* weights = weights_of<PT>(t);
+    const int64_t at = x.at;
+    const uint64_t sblk = x.sblk, si = sblk * kAdamBlock + (uint64_t)lane * 8;
+    const bool whole = x.whole;
     float g[8], p[8];
-    F2 m[4], v[4];                                                             // pairs of neighbours
-    float m_unit = 0.f, v_unit = 0.f;
+    F2 m[4], v[4];                                             // pairs of neighbours
+    if constexpr (BITS8) {
+      decode8<true>(x.cm, __fmul_rn(x.m_scale, kSignedUnit), m);
+      decode8<false>(x.cv, __fmul_rn(x.v_scale, kUnsignedUnit), v);
+    }
     if (whole) {
-      Raw8 rg, rp, rm, rv;
-      load8<GT>(t.grad, at, rg);
-      load8<kAdamF32>(weights, at, rp);
-      if constexpr (BITS8) {
-        const uint2 cm = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.m) + si));
-        const uint2 cv = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.v) + si));
-        m_unit = __fmul_rn(a.m_scale[sblk], kSignedUnit);
-        v_unit = __fmul_rn(a.v_scale[sblk], kUnsignedUnit);
-        decode8<true>(cm, m_unit, m);
-        decode8<false>(cv, v_unit, v);
-      } else {
+      widen<GT>(x.g, g);
+      widen<kAdamF32>(x.p, p);
+      if constexpr (!BITS8) {
+        Raw8 rm, rv;
         load8<kAdamF32>(a.m, (int64_t)si, rm);
         load8<kAdamF32>(a.v, (int64_t)si, rv);
-        float x[8], y[8];
-        widen<kAdamF32>(rm, x);
-        widen<kAdamF32>(rv, y);
+        float y[8], z[8];
+        widen<kAdamF32>(rm, y);
+        widen<kAdamF32>(rv, z);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          m[i] = f2(x[2 * i], x[2 * i + 1]);
-          v[i] = f2(y[2 * i], y[2 * i + 1]);
+          m[i] = f2(y[2 * i], y[2 * i + 1]);
+          v[i] = f2(z[2 * i], z[2 * i + 1]);
         }
       }
-      widen<GT>(rg, g);
-      widen<kAdamF32>(rp, p);
     } else {
-      float x[8], y[8];
+      float y[8], z[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const bool on = at + i < t.n;
         g[i] = on ? load1<GT>(t.grad, at + i) : 0.f;
         p[i] = on ? static_cast<const float*>(weights)[at + i] : 0.f;
         if constexpr (!BITS8) {
-          x[i] = on ? static_cast<const float*>(a.m)[si + i] : 0.f;
-          y[i] = on ? static_cast<const float*>(a.v)[si + i] : 0.f;
+          y[i] = on ? static_cast<const float*>(a.m)[si + i] : 0.f;
+          z[i] = on ? static_cast<const float*>(a.v)[si + i] : 0.f;
         }
       }
-      if constexpr (BITS8) {                                     // the state's blocks are whole: behind a tensor's end they hold zeros
-        m_unit = __fmul_rn(a.m_scale[sblk], kSignedUnit);
-        v_unit = __fmul_rn(a.v_scale[sblk], kUnsignedUnit);
-        decode8<true>(*reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.m) + si), m_unit, m);
-        decode8<false>(*reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.v) + si), v_unit, v);
-      } else {
+      if constexpr (!BITS8) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          m[i] = f2(x[2 * i], x[2 * i + 1]);
-          v[i] = f2(y[2 * i], y[2 * i + 1]);
+          m[i] = f2(y[2 * i], y[2 * i + 1]);
+          v[i] = f2(z[2 * i], z[2 * i + 1]);
         }
       }
     }
+    blk += warps;
+    const bool more = blk < a.blocks;
+    if constexpr (!BITS8) {
+      if (more) fetch<PT, GT, BITS8, MAX>(a, table, blk, x.k, x);
+    }
     // ---- the step
-    const F2 keep = f2(1.f - a.lr * t.decay);
+    const F2 keep = f2(1.f - a.lr * t.decay), rate = f2(-a.lr * a.bias1);
+    const bool tiny_eps = a.eps < 1e-15f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const F2 x = f2(g[2 * i], g[2 * i + 1]) * f2(gs);
-      m[i] = f2(a.beta1) * m[i] + f2(a.one_minus_beta1) * x;
-      v[i] = f2(a.beta2) * v[i] + f2(a.one_minus_beta2) * (x * x);
+      const F2 y = f2(g[2 * i], g[2 * i + 1]) * f2(gs);
+      m[i] = f2(a.beta1) * m[i] + f2(a.one_minus_beta1) * y;
+      v[i] = f2(a.beta2) * v[i] + f2(a.one_minus_beta2) * (y * y);
       // the update's root and quotient are the hardware's (a few units in the last place of the update, not of the parameter)
       float a0, a1;
       split(v[i] * f2(a.bias2), a0, a1);
-      asm("sqrt.approx.f32 %0, %0;" : "+f"(a0));                 // v may be below 2^-126 where eps is 0
-      asm("sqrt.approx.f32 %0, %0;" : "+f"(a1));
+      if (tiny_eps) {                                          // a v below 2^-126 counts
+        asm("sqrt.approx.f32 %0, %0;" : "+f"(a0));
+        asm("sqrt.approx.f32 %0, %0;" : "+f"(a1));
+      } else {
+        a0 = root_hw(a0);
+        a1 = root_hw(a1);
+      }
       split(f2(a0, a1) + f2(a.eps), a0, a1);
-      const F2 q = m[i] * f2(a.lr * a.bias1) * f2(rcp_hw(a0), rcp_hw(a1));
-      split(fma2(f2(p[2 * i], p[2 * i + 1]), keep, q * f2(-1.f)), p[2 * i], p[2 * i + 1]);
+      split(fma2(f2(p[2 * i], p[2 * i + 1]), keep, m[i] * rate * f2(rcp_hw(a0), rcp_hw(a1))), p[2 * i], p[2 * i + 1]);
     }
     // ---- states
     uint32_t cm[2] = {0u, 0u}, cv[2] = {0u, 0u};
@@ -336,8 +373,8 @@ __global__ void __launch_bounds__(kThreads, 4) adamw_multi_kernel(const __grid_c
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint32_t n0 = mix(base + 2 * i), n1 = mix(base + 2 * i + 1);
-        encode2<true>(m[i], f2(im), f2(noise_hi(n0), noise_hi(n1)) + f2(-1.f), km[2 * i], km[2 * i + 1]);
-        encode2<false>(v[i], f2(iv), f2(noise_lo(n0), noise_lo(n1)) + f2(-1.f), kv[2 * i], kv[2 * i + 1]);
+        encode2<true>(m[i], f2(im), f2(noise_hi(n0), noise_hi(n1)) + f2(-1.f), false, km[2 * i], km[2 * i + 1]);
+        encode2<false>(v[i], f2(iv), f2(noise_lo(n0), noise_lo(n1)) + f2(-1.f), !(iv > 0.f), kv[2 * i], kv[2 * i + 1]);
       }
       for (int i = 0; i < 2; ++i) {
         cm[i] = bytes4(km[4 * i], km[4 * i + 1], km[4 * i + 2], km[4 * i + 3]);
@@ -380,6 +417,8 @@ __global__ void __launch_bounds__(kThreads, 4) adamw_multi_kernel(const __grid_c
         }
       }
     }
+    if (!more) break;
+    if constexpr (BITS8) fetch<PT, GT, BITS8, MAX>(a, table, blk, x.k, x);
   }
 }
 
@@ -408,7 +447,7 @@ cudaError_t launch(const AdamMultiArgs& a, const AdamTensor* tensors, int count,
   Table<MAX> table;
   memcpy(table.t, tensors, sizeof(AdamTensor) * (size_t)count);
   table.count = count;
-  const uint32_t need = (a.blocks + kThreads / 32 - 1) / (kThreads / 32), most = (uint32_t)sm_count * 4;
+  const uint32_t need = (a.blocks + kThreads / 32 - 1) / (kThreads / 32), most = (uint32_t)sm_count * (BITS8 ? 4 : 3);
   return launch_pdl(adamw_multi_kernel<PT, GT, BITS8, MAX>, dim3(need < most ? need : most), dim3(kThreads), 0, s, a, table);
 }
 template <int PT, int GT>
