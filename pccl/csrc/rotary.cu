@@ -23,7 +23,7 @@ namespace pccl {
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kForward = 128, kBackward = 256;               // threads of a block
 
 // Four elements of 16 bits, in a register pair.
 template <bool BF16>
@@ -153,11 +153,11 @@ __device__ __forceinline__ int share_of(const RotaryArgs& a, uint32_t& block, ui
 
 // ---------------------------------------------------------------- forward
 template <bool BF16, bool NEIGHBOURS, int L>
-__global__ void __launch_bounds__(kThreads) rotary_forward_kernel(const __grid_constant__ RotaryArgs a) {
+__global__ void __launch_bounds__(kForward) rotary_forward_kernel(const __grid_constant__ RotaryArgs a) {
   pdl_wait();
   pdl_trigger();
   constexpr int U = 4;
-  constexpr uint32_t groups = kThreads / L;
+  constexpr uint32_t groups = kForward / L;
   const Columns col = columns<NEIGHBOURS>(threadIdx.x & (L - 1), a.half, a.D);
   const float inv_d = 1.f / (float)a.D;
   uint32_t block, blocks;
@@ -171,45 +171,41 @@ __global__ void __launch_bounds__(kThreads) rotary_forward_kernel(const __grid_c
     load_w4(a.w[which], a.w_type, col.c0, w);
     load_w4(a.w[which], a.w_type, col.c1, w + 4);
   }
-  // a group: one chunk of heads in one row after another; all groups of a block take equally many steps, because the
-  // exchanges want whole warps
-  const uint64_t items = (uint64_t)rows * chunks;
-  for (uint64_t i0 = (uint64_t)block * groups; i0 < items; i0 += (uint64_t)blocks * groups) {
-    const uint64_t i = i0 + threadIdx.x / L;
-    const bool exists = i < items;
-    const uint32_t row = exists ? (uint32_t)(chunks == 1 ? i : i / chunks) : 0, chunk = exists ? (uint32_t)(i - (uint64_t)row * chunks) : 0;
-    const Item it = item_at(a, which, row, chunk);
-    const int h1 = exists && col.on ? it.h1 : it.h0;
-    Angles t;
-    load_angles(t, a, position(a, it), col);
-    for (int r = 0; r < a.heads_per_item; r += U) {
-      uint2 q[U][2];
+  // a group: one chunk of heads in one row; groups without one go through the exchanges with the others
+  const uint64_t items = (uint64_t)rows * chunks, i = (uint64_t)block * groups + threadIdx.x / L;
+  const bool exists = i < items;
+  const uint32_t row = exists ? (uint32_t)(chunks == 1 ? i : i / chunks) : 0, chunk = exists ? (uint32_t)(i - (uint64_t)row * chunks) : 0;
+  const Item it = item_at(a, which, row, chunk);
+  const int h1 = exists && col.on ? it.h1 : it.h0;
+  Angles t;
+  load_angles(t, a, position(a, it), col);
+  for (int r = 0; r < a.heads_per_item; r += U) {
+    uint2 q[U][2];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int h = it.h0 + r + u;
-        const uint16_t* p = row_at(tx, it.b, it.s, h);
-        q[u][0] = h < h1 ? *reinterpret_cast<const uint2*>(p + col.c0) : make_uint2(0, 0);
-        q[u][1] = h < h1 ? *reinterpret_cast<const uint2*>(p + col.c1) : make_uint2(0, 0);
-      }
+    for (int u = 0; u < U; ++u) {
+      const int h = it.h0 + r + u;
+      const uint16_t* p = row_at(tx, it.b, it.s, h);
+      q[u][0] = h < h1 ? *reinterpret_cast<const uint2*>(p + col.c0) : make_uint2(0, 0);
+      q[u][1] = h < h1 ? *reinterpret_cast<const uint2*>(p + col.c1) : make_uint2(0, 0);
+    }
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (r + u >= a.heads_per_item) break;
-        const int h = it.h0 + r + u;
-        float x[8];
-        unpack4<BF16>(q[u][0], x);
-        unpack4<BF16>(q[u][1], x + 4);
-        float ss = 0.f;
+    for (int u = 0; u < U; ++u) {
+      if (r + u >= a.heads_per_item) break;
+      const int h = it.h0 + r + u;
+      float x[8];
+      unpack4<BF16>(q[u][0], x);
+      unpack4<BF16>(q[u][1], x + 4);
+      float ss = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
-        const float rs = rsqrtf(fmaf(group_sum<L>(ss), inv_d, a.eps));
+      for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
+      const float rs = rsqrtf(fmaf(group_sum<L>(ss), inv_d, a.eps));
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] *= rs * w[e];
-        rotate<NEIGHBOURS, false>(x, t, col.turned);
-        if (h < h1) {
-          uint16_t* p = row_at(ty, it.b, it.s, h);
-          *reinterpret_cast<uint2*>(p + col.c0) = pack4<BF16>(x);
-          *reinterpret_cast<uint2*>(p + col.c1) = pack4<BF16>(x + 4);
-        }
+      for (int e = 0; e < 8; ++e) x[e] *= rs * w[e];
+      rotate<NEIGHBOURS, false>(x, t, col.turned);
+      if (h < h1) {
+        uint16_t* p = row_at(ty, it.b, it.s, h);
+        *reinterpret_cast<uint2*>(p + col.c0) = pack4<BF16>(x);
+        *reinterpret_cast<uint2*>(p + col.c1) = pack4<BF16>(x + 4);
       }
     }
   }
@@ -217,12 +213,12 @@ __global__ void __launch_bounds__(kThreads) rotary_forward_kernel(const __grid_c
 
 // ---------------------------------------------------------------- backward
 template <bool BF16, bool NEIGHBOURS, int L>
-__global__ void __launch_bounds__(kThreads) rotary_backward_kernel(const __grid_constant__ RotaryArgs a) {
-  __shared__ float sums[kThreads * 8];
+__global__ void __launch_bounds__(kBackward, 2) rotary_backward_kernel(const __grid_constant__ RotaryArgs a) {
+  __shared__ float sums[kBackward * 8];
   pdl_wait();
   pdl_trigger();
-  constexpr int U = 2;
-  constexpr uint32_t groups = kThreads / L;
+  constexpr int U = 4;
+  constexpr uint32_t groups = kBackward / L;
   const Columns col = columns<NEIGHBOURS>(threadIdx.x & (L - 1), a.half, a.D);
   const float inv_d = 1.f / (float)a.D;
   uint32_t block, blocks;
@@ -298,7 +294,7 @@ __global__ void __launch_bounds__(kThreads) rotary_backward_kernel(const __grid_
     }
   }
   __syncthreads();
-  for (int c = threadIdx.x; c < a.D; c += kThreads) {
+  for (int c = threadIdx.x; c < a.D; c += kBackward) {
     float s = 0.f;
     for (int g = 0; g < (int)groups; ++g) s += sums[g * L * 8 + c];
     a.partial[(int64_t)blockIdx.x * a.D + c] = s;
@@ -306,7 +302,7 @@ __global__ void __launch_bounds__(kThreads) rotary_backward_kernel(const __grid_
 }
 
 // dw[c] = sum of the blocks' shares: 32 columns per block, eight warps that each add up every eighth share.
-__global__ void __launch_bounds__(kThreads) rotary_weights_kernel(const __grid_constant__ RotaryArgs a, int blocks) {
+__global__ void __launch_bounds__(kBackward) rotary_weights_kernel(const __grid_constant__ RotaryArgs a, int blocks) {
   __shared__ float sums[8][32];
   pdl_wait();
   pdl_trigger();
@@ -329,10 +325,10 @@ int lanes_of(int D) { return D <= 64 ? 8 : (D <= 128 ? 16 : 32); }
 
 template <bool BF16, bool NEIGHBOURS, int L>
 cudaError_t launch(const RotaryArgs& a, bool backward, int blocks, cudaStream_t s) {
-  if (!backward) return launch_pdl(rotary_forward_kernel<BF16, NEIGHBOURS, L>, dim3(blocks), dim3(kThreads), 0, s, a);
-  const cudaError_t e = launch_pdl(rotary_backward_kernel<BF16, NEIGHBOURS, L>, dim3(blocks), dim3(kThreads), 0, s, a);
+  if (!backward) return launch_pdl(rotary_forward_kernel<BF16, NEIGHBOURS, L>, dim3(blocks), dim3(kForward), 0, s, a);
+  const cudaError_t e = launch_pdl(rotary_backward_kernel<BF16, NEIGHBOURS, L>, dim3(blocks), dim3(kBackward), 0, s, a);
   if (e != cudaSuccess) return e;
-  return launch_pdl(rotary_weights_kernel, dim3((a.D + 31) / 32, 2), dim3(kThreads), 0, s, a, blocks);
+  return launch_pdl(rotary_weights_kernel, dim3((a.D + 31) / 32, 2), dim3(kBackward), 0, s, a, blocks);
 }
 template <bool BF16, bool NEIGHBOURS>
 cudaError_t launch_lanes(const RotaryArgs& a, bool backward, int blocks, cudaStream_t s) {
@@ -352,15 +348,17 @@ cudaError_t launch_any(const RotaryArgs& a, bool backward, int blocks, cudaStrea
 }  // namespace
 
 int rotary_blocks(RotaryArgs& a, bool backward, int sm_count) {
-  const int lanes = lanes_of(a.D), groups = kThreads / lanes;
+  const int lanes = lanes_of(a.D), groups = (backward ? kBackward : kForward) / lanes;
   const int64_t rows = (int64_t)a.B * a.S;
-  const int64_t most = (int64_t)sm_count * (backward ? 4 : 8);
-  // up to sixteen heads per item where that still gives every SM four blocks, else fewer: a short call wants many groups
+  // Heads per item: as many of a row as possible share its angles, but every SM wants eight blocks (forward: one item per group), or
+  // two blocks that walk over six items or more (backward).  8192 rows of 16 + 16 heads of 128, backward: 16 heads 55.2 us, 8 heads 51.8;
+  // of 32 + 32: 91.5 and 94.6.  Forward: 16 heads 28.0 and 50.0, 8 heads 28.9 and 51.7.
+  const int64_t most = backward ? (int64_t)sm_count * 2 : INT32_MAX, want = (int64_t)sm_count * groups * (backward ? 12 : 8);
   int hpi = 16;
   for (;; hpi /= 2) {
     a.heads_per_item = hpi;
     for (int i = 0; i < 2; ++i) a.chunks[i] = (a.H[i] + hpi - 1) / hpi;
-    if (hpi == 1 || rows * (a.chunks[0] + a.chunks[1]) >= (int64_t)sm_count * 4 * groups) break;
+    if (hpi == 1 || rows * (a.chunks[0] + a.chunks[1]) >= want) break;
   }
   int64_t need[2];
   for (int i = 0; i < 2; ++i) need[i] = (rows * a.chunks[i] + groups - 1) / groups;
