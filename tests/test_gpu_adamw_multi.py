@@ -46,6 +46,8 @@ SIZES = [[1], [256], [255, 257], [1, 2, 3, 100003, 5, 4096, 31], [7] * 900, [204
 def test_states_in_32_bits_match_formula(types, sizes, shift):
     from pccl.ops.optim import adamw_state, adamw_step
 
+    if len(sizes) > 100 and (types != (BF, BF) or shift):
+        pytest.skip("the long list once")
     params, grads, masters = _lists(sizes, *types, 1, shift)
     decay = [0.1 * (i % 3) for i in range(len(sizes))]
     state = adamw_state(params, 32)
@@ -70,6 +72,35 @@ def test_states_in_32_bits_match_formula(types, sizes, shift):
             assert torch.all((w.double() - want).abs() <= 4 * f * b.abs() + 24 * f * upd.abs() + slack + tiny)
             if w is not p:
                 assert torch.equal(p, w.to(p.dtype))
+
+
+def test_moments_are_rounded_product_by_product():
+    """b1 m and (1 - b1) g are rounded to 32 bits before they are added, so that the codes of 8-bit states hang on the formula alone."""
+    import numpy as np
+
+    from pccl.ops.optim import adamw_state, adamw_step
+
+    f = lambda x: float(np.float32(x))                                            # noqa: E731
+    g = torch.Generator(device=DEV).manual_seed(8)
+    n = 256 * 300
+    for bits in (32, 8):
+        grad = torch.randn(n, device=DEV, generator=g) * 1e-3
+        state = adamw_state([grad], bits)
+        for step in (1, 2):
+            m, v = (x.clone() for x in state.dequantize())
+            full = adamw_state([grad], 32)
+            full.exp_avg.copy_(m)
+            full.exp_avg_sq.copy_(v)
+            p = torch.zeros(n, device=DEV)
+            adamw_step([p], [grad], full, step=step, **HYPER)
+            assert torch.equal(full.exp_avg, m * f(0.9) + grad * f(1 - 0.9))
+            assert torch.equal(full.exp_avg_sq, v * f(0.95) + (grad * grad) * f(1 - 0.95))
+            adamw_step([p], [grad], state, step=step, **HYPER)
+            if bits == 8:
+                assert torch.equal(state.exp_avg_scale, full.exp_avg.abs().view(-1, 256).amax(1))
+                assert torch.equal(state.exp_avg_sq_scale, full.exp_avg_sq.view(-1, 256).amax(1))
+            else:
+                assert torch.equal(state.exp_avg, full.exp_avg)
 
 
 @pytest.mark.parametrize("types", [(BF, BF), (F32, F32), (FP, F32)], ids=str)
