@@ -86,6 +86,9 @@ def parse_args():
                     help="GELU backward as the epilogue of the data-gradient GEMM in front of it (library GEMM only)")
     ap.add_argument("--dynamic-tiles", type=int, default=int(os.environ.get("PCCL_DYNAMIC_TILES", "-1")),
                     help="library GEMM hands tiles out at run time: 1 on, 0 off, -1 on when N > 1")
+    ap.add_argument("--attention", default="sdpa", choices=["sdpa", "pccl"],
+                    help="library arm: attention core through torch's scaled_dot_product_attention or on the library's kernels")
+    ap.add_argument("--optim-bits", type=int, default=32, choices=[8, 32], help="library arm: bits of both Adam moments")
     ap.add_argument("--no-e2e", action="store_true")
     ap.add_argument("--no-baseline", action="store_true", help="library arm only: skip the NCCL+cuBLAS arm and vs_baseline")
     ap.add_argument("--no-raw", action="store_true", help="skip the raw-collective rows")
@@ -165,7 +168,8 @@ def run_arm(args, impl: str, ctx: dict, native_gemm: bool = False, e2e: bool = T
                          fused_gelu_gemm=(library and bool(args.fused_gelu_gemm)), overlap_wgrad=bool(args.overlap_wgrad),
                          native_gemm=(library and native_gemm), fused_gelu_bwd_gemm=bool(args.fused_gelu_bwd),
                          dynamic_tiles=None if args.dynamic_tiles < 0 else bool(args.dynamic_tiles),
-                         copy_engine_gather=(library and args.gather == "copy_engine"))
+                         copy_engine_gather=(library and args.gather == "copy_engine"),
+                         native_attention=(library and args.attention == "pccl"), optim_bits=args.optim_bits if library else 32)
     host_tokens, dev_tokens = ctx["host_tokens"], ctx["dev_tokens"]
 
     def step_device(i):
@@ -207,7 +211,7 @@ def run_arm(args, impl: str, ctx: dict, native_gemm: bool = False, e2e: bool = T
         "engine": {"fused_ag_gemm": bool(engine.fused_ag_gemm), "fused_gelu_gemm": bool(engine.fused_gelu_gemm),
                    "overlap_wgrad": bool(engine.overlap_wgrad), "native_gemm": bool(engine.native_gemm),
                    "fused_gelu_bwd_gemm": bool(engine.fused_gelu_bwd_gemm), "dynamic_tiles": bool(engine.dynamic_tiles),
-                   "copy_engine_gather": bool(engine.copy_engine_gather)},
+                   "copy_engine_gather": bool(engine.copy_engine_gather), "native_attention": bool(engine.native_attention)},
     }
     if e2e and not args.no_e2e:
         step_host(0)                                    # host path once, untimed
@@ -328,7 +332,9 @@ def main() -> None:
                 "model": cfg.name, "layers": cfg.n_layer, "d_model": cfg.d_model, "heads": cfg.n_head,
                 "ffn": cfg.d_ff, "vocab": cfg.vocab, "params": cfg.num_params(),
                 "global_batch": world * mb, "micro_batch_per_gpu": mb, "seq_len": S,
-                "parallelism": f"zero3-dp{world}", "optimizer": "AdamW fp32 master+moments, grad-norm clip 1.0",
+                "parallelism": f"zero3-dp{world}", "optimizer": "AdamW fp32 master" + ("+moments" if args.impl == "nccl" or args.optim_bits == 32 else ", 8-bit moments") +
+                             ", grad-norm clip 1.0",
+                "attention": "this repository's kernels" if main_arm["engine"]["native_attention"] else "scaled_dot_product_attention",
                 "algorithm": args.algorithm, "lanes": args.lanes, "nvls": bool(args.nvls),
                 "gemm": "tcgen05 (this repository)" if main_arm["engine"]["native_gemm"] else
                         ("cuBLAS for the plain products, tcgen05 (this repository) for the fused ones that are switched on"
