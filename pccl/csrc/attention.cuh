@@ -307,6 +307,12 @@ __device__ __forceinline__ void zero_rows(const AttnTensor& t, int head, int fir
   }
 }
 
+// Eight words to a 32-byte boundary.
+__device__ __forceinline__ void store_words(void* p, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]),
+               "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
 // 32 accumulator columns of one row, times f, as 16-bit elements; only columns below D exist.  wide: the row starts on a
 // 32-byte boundary, and a store of 32 bytes writes one whole sector.
 template <bool BF16>
@@ -318,9 +324,7 @@ __device__ __forceinline__ void store32(uint16_t* row, int col0, int D, const ui
     for (int e = 0; e < 8; ++e) w[e] = pack2<BF16>(__uint_as_float(r[v * 16 + 2 * e]) * f, __uint_as_float(r[v * 16 + 2 * e + 1]) * f);
     const int col = col0 + v * 16;
     if (wide && col + 16 <= D) {
-      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(row + col), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
-                   "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
-                   : "memory");
+      store_words(row + col, w);
     } else {
       if (col < D) *reinterpret_cast<uint4*>(row + col) = make_uint4(w[0], w[1], w[2], w[3]);
       if (col + 8 < D) *reinterpret_cast<uint4*>(row + col + 8) = make_uint4(w[4], w[5], w[6], w[7]);

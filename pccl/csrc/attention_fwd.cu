@@ -550,7 +550,7 @@ AttnScratch plan_attention_forward(AttnArgs& a, int sm_count) {
     a.parts_o = (int)(room < most ? room : most);
     if (a.parts_o < 1) a.parts_o = 1;
   }
-  AttnScratch need = {0, 0, 0, 0};
+  AttnScratch need = {0, 0, 0, 0, 0};
   if (a.cu_q != nullptr) need.order_q = max_tiles(a.Sq, a.nseq, 256);
   if (a.parts_o > 1) {
     need.partial_lse = (int64_t)a.parts_o * a.B * a.H * a.Sq;
