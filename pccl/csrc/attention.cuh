@@ -260,7 +260,9 @@ __device__ __forceinline__ void write_order(const int* cu, int nseq, int limit, 
     for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
     return n;
   };
-  const int most = (int)((limit + rows - 1) / rows);
+  int most = 0;                                                // the longest sequence's tiles
+  for (int s = lane; s < nseq; s += 32) most = max(most, tiles_of(s));
+  most = __reduce_max_sync(0xffffffffu, most);
   for (int level = warp + 1; level <= most; level += warps) {
     int64_t at = above(level + 1);
     for (int s0 = 0; s0 < nseq && at < entries; s0 += 32) {

@@ -32,7 +32,7 @@ struct AttnArgs {
   int2* order_q;                     // packed: which sequence and which of its tiles each tile number stands for (scratch; forward:
   int2* order_k;                     // order_q; backward: both)
   int causal;
-  int zero_tail;                     // packed: rows behind the last sequence are set to 0 (lse: -inf); else they are left alone
+  int zero_tail;                     // packed: rows behind the last sequence are set to 0; else they are left alone (lse there is -inf)
   float scale;
   int* error;
   // Work split over a long axis (not for packed sequences), where there are too few tiles for the device: the parts of one

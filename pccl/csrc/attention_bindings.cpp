@@ -175,6 +175,12 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_backward(const at::Tens
   TORCH_CHECK(dq_.has_value() == dk_.has_value() && dq_.has_value() == dv_.has_value(), "dq, dk and dv are given together or not at all");
   const std::initializer_list<at::Tensor> inputs = {dout, q, k, v, out};
   at::Tensor dq = output(dq_, q, "dq", inputs), dk = output(dk_, k, "dk", inputs), dv = output(dv_, v, "dv", inputs);
+  auto apart = [](const at::Tensor& x, const at::Tensor& y) {
+    const auto o = at::get_overlap_status(x, y);
+    return o != at::MemOverlapStatus::Full && o != at::MemOverlapStatus::Partial;
+  };
+  TORCH_CHECK(apart(dq, dk) && apart(dq, dv) && apart(dk, dv), "dq, dk and dv must not overlap each other");
+  TORCH_CHECK(s.B <= 65535, "the backward pass takes up to 65535 batch entries");
   a.dq = view(dq, "dq", q, s.B, s.Sq, s.H, s.D);
   a.dk = view(dk, "dk", q, s.B, s.Sk, s.Hk, s.D);
   a.dv = view(dv, "dv", q, s.B, s.Sk, s.Hk, s.D);

@@ -400,11 +400,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!ok) break;
       if (w.sp.tile < 0) {                                             // behind the last sequence
-        if (a.zero_tail) {
-          zero_rows(a.o, w.head, w.sp.first_q, 256, a.Sq, a.D, threadIdx.x, 256);
-          const int r = w.sp.first_q + (int)threadIdx.x;
-          if (r < a.Sq) a.lse[stat_row(a, 0, w.head) + r] = -INFINITY;
-        }
+        if (a.zero_tail) zero_rows(a.o, w.head, w.sp.first_q, 256, a.Sq, a.D, threadIdx.x, 256);
+        const int r = w.sp.first_q + (int)threadIdx.x;
+        if (r < a.Sq) a.lse[stat_row(a, 0, w.head) + r] = -INFINITY;
       } else {
         const bool exists = row < w.sp.len_q, wide = rows_are_wide(a.o);
         const bool none = l == 0.f;                                    // no key is seen (scores that are NaN leave l NaN)

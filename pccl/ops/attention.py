@@ -11,14 +11,18 @@ Layout.  ``q`` is ``[batch, rows, heads, dim]``, ``k`` and ``v`` are ``[batch, k
 ``h // (heads // key heads)``).  Only the last dimension has to be contiguous: views into a packed projection are read where
 they lie (16-byte boundaries, strides that are multiples of 8 elements).  Packed sequences are ``[rows, heads, dim]`` with the
 starts of the sequences and the end of the last one in ``cu_seqlens_q`` (and ``cu_seqlens_k``; left out, it is the same), int32
-on the device, not decreasing; they are read there, so the host waits for nothing.  Rows behind the last sequence belong to
-none: results that are allocated here hold 0 there (``lse``: -inf), tensors given by the caller keep what they held.
+on the device, from 0 on and not decreasing; they are read there, so the host waits for nothing (starts that break this give
+results that mean nothing, within the tensors).  Rows behind the last sequence belong to none: results that are allocated here
+hold 0 there (``lse``: -inf), tensors given by the caller keep what they held.
 
 Masks.  ``causal``: query i sees the keys up to ``i + (key rows - query rows)`` of its sequence, so that the last query sees the
 last key.  A query that sees no key has an output of 0, an ``lse`` of -inf, and adds nothing to any gradient.
 
 These are plain functions like those of ``pccl.ops.gemm``: they record nothing for autograd.  Results are the same bits from
-call to call (no atomic additions).  Outputs must not overlap inputs.
+call to call (no atomic additions).  Outputs must not overlap inputs or each other.  Probabilities and score gradients are rounded
+to the inputs' type for the products that they enter: with fp16 a score gradient above 65504 becomes infinite, as it does in
+``dout``.  The backward pass of a batch (not of packed sequences) keeps its score gradients in up to 1 GiB of memory while it
+runs, and computes them twice where they would take more.
 """
 from __future__ import annotations
 

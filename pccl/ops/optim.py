@@ -75,7 +75,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], st
 
     ``step`` counts from 1.  ``weight_decay`` is one number, or one for each tensor.  Gradients are multiplied by
     ``grad_scale``, and with ``max_grad_norm`` > 0 scaled down where their norm, ``sqrt(total_sq_norm) * grad_scale``, is above
-    it; ``total_sq_norm`` is a device scalar (``pccl._C.sq_norm`` adds to one, ranks may add theirs), read on the device."""
+    it; ``total_sq_norm`` is a device scalar (``pccl._C.sq_norm`` adds to one, ranks may add theirs), read on the device.  All other
+    numbers are the call's own: a captured call replays with the ``step``, ``lr`` and noise that it was captured with."""
     decay = [float(weight_decay)] if isinstance(weight_decay, (int, float)) else [float(w) for w in weight_decay]
     _C().adamw_multi(list(params), list(grads), None if masters is None else list(masters), state.exp_avg, state.exp_avg_sq,
                      state.exp_avg_scale, state.exp_avg_sq_scale, decay, step, lr, beta1, beta2, eps, grad_scale, max_grad_norm,

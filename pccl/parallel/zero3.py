@@ -319,6 +319,9 @@ class Zero3Engine:
         cfg, C = self.cfg, self.C
         if cu_seqlens is not None and not (self.native_attention and cfg.qk_norm_rope):
             raise ValueError("packed documents need native_attention and a configuration with qk_norm_rope")
+        if cu_seqlens is not None and (cu_seqlens.device != self.device or cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1
+                                       or cu_seqlens.numel() < 2 or not cu_seqlens.is_contiguous()):
+            raise ValueError("cu_seqlens must be a contiguous 1-D int32 tensor of at least two starts on the engine's device")
         if tokens.device.type != "cuda":
             if self._tokens_dev is None or self._tokens_dev.shape != tokens.shape:
                 self._tokens_dev = torch.empty(tokens.shape, dtype=torch.int64, device=self.device)

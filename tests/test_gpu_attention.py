@@ -192,7 +192,7 @@ def test_packed_outputs_of_the_caller_keep_the_rows_behind():
     _out, lse = attention_forward(q, k, v, cu_seqlens_q=cq, out=new[0])
     attention_backward(dout, q, k, v, new[0], lse, cu_seqlens_q=cq, dq=new[1], dk=new[2], dv=new[3])
     ref, _ = attention_forward(q, k, v, cu_seqlens_q=cq)
-    assert torch.equal(new[0][:140], ref[:140])
+    assert torch.equal(new[0][:140], ref[:140]) and torch.all(lse[:, 140:] == -math.inf)
     for x in new:
         assert torch.all(x[140:] == 7.0) and not torch.any(x[:140] == 7.0)
 
@@ -297,6 +297,54 @@ def test_captured_calls_and_other_streams():
     check_errors()
 
 
+def test_first_call_of_a_process_may_be_captured():
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    code = """
+import torch
+from pccl.ops.attention import attention_backward, attention_forward, check_errors
+from pccl.ops.rotary import qk_norm_rope_forward, rotary_table
+from pccl.ops.optim import adamw_state, adamw_step
+x = torch.randn(1, 300, 6, 64, device="cuda", dtype=torch.bfloat16)
+w = torch.ones(64, device="cuda", dtype=torch.bfloat16)
+cos, sin = rotary_table(300, 64, device="cuda")
+p = torch.ones(1000, device="cuda"); st = adamw_state([p], 8)
+def run():
+    q, k = qk_norm_rope_forward(x[:, :, :4], x[:, :, 4:5], w, w, cos, sin)
+    out, lse = attention_forward(q, k, x[:, :, 5:6])
+    g = attention_backward(out, q, k, x[:, :, 5:6], out, lse)
+    return (q, k, out, lse, *g)
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    got = run()
+    adamw_step([p], [p * 0.5], st, step=1, lr=0.1)
+g.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, run()))
+assert float(p.max()) < 1.0
+check_errors()
+print("fine")
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).resolve().parent.parent, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stderr[-2000:]
+
+
+def test_score_gradients_kept_or_computed_twice():
+    """Two heads of 2049 rows keep their score gradients in memory, three hundred (1.4 GiB) compute them twice."""
+    from pccl.ops.attention import attention_backward
+
+    q, k, v, dout = _inputs(1, 2049, 2049, 2, 2, 64, BF, 30)
+    out, lse = _given(q, k, v, True, 0.125)
+    want = _oracle(q[0], k[0], v[0], _visible(2049, 2049, True), 0.125, dout[0], out[0], lse[0])
+    for n in (1, 150):
+        got = attention_backward(*(t.expand(n, *t.shape[1:]).contiguous() for t in (dout, q, k, v, out)), lse.expand(n, 2, 2049).contiguous())
+        for x, (w, t), what in zip(got, want, ("dq", "dk", "dv")):
+            _close(x[0], w, t, what)
+            assert torch.equal(x[0], x[n - 1])
+
+
 def test_empty_calls():
     from pccl.ops.attention import attention_backward, attention_forward
 
@@ -368,6 +416,8 @@ def test_refusals():
         lambda: attention_backward(q, q, k, k, q, lse.double()),
         lambda: attention_backward(q[:, :, :2], q, k, k, q, lse),
         lambda: attention_backward(q, q, k, k, q, lse, dq=torch.empty_like(q)),
+        lambda: (lambda x: attention_backward(q, q, k, k, q, lse, dq=torch.empty_like(q), dk=x, dv=x))(torch.empty_like(k)),
+        lambda: (lambda x: attention_backward(x, q, k, k, q, lse, dq=x, dk=torch.empty_like(k), dv=torch.empty_like(k)))(torch.empty_like(q)),
     ]
     for i, call in enumerate(bad):
         with pytest.raises(RuntimeError):
