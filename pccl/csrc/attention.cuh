@@ -118,17 +118,19 @@ __device__ __forceinline__ void commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
-// d[128, 128] = a b^T, both tiles contracted along their DP columns.
+// Columns of a head in steps of 16, as the products take them: the rest of a tile's DP columns is zeros.
+__device__ __forceinline__ int steps_of(int D) { return (D + 15) / 16; }
+// d[128, 128] = a b^T, both tiles contracted along their first `steps` x 16 columns.
 template <int DP>
-__device__ __forceinline__ void mma_columns(uint32_t d, uint32_t a_addr, uint32_t b_addr, uint32_t id) {
+__device__ __forceinline__ void mma_columns(uint32_t d, uint32_t a_addr, uint32_t b_addr, uint32_t id, int steps) {
   const uint32_t a = desc_k(a_addr), b = desc_k(b_addr);
 #pragma unroll
   for (int k = 0; k < DP / 16; ++k) {
     const uint32_t off = (k >> 2) * (kBlockBytes >> 4) + (k & 3) * (32 >> 4);
-    mma_ss(d, a + off, b + off, id, k > 0 ? 1u : 0u);
+    if (k == 0 || k < steps) mma_ss(d, a + off, b + off, id, k > 0 ? 1u : 0u);
   }
 }
-// d[128, DP] (+)= a b, a: 128 x 128 of 16 bits in tensor memory, b: a tile contracted along its 128 rows, in steps of 16 of
+// d[128, columns of id] (+)= a b, a: 128 x 128 of 16 bits in tensor memory, b: a tile contracted along its 128 rows, in steps of 16 of
 // which this takes [FROM, TO).  GROUP steps of a lie side by side (8 columns each), the next GROUP from STRIDE columns further on.
 template <int FROM, int TO, int GROUP, int STRIDE>
 __device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a, uint32_t b_addr, uint32_t id, bool accumulate) {

@@ -292,7 +292,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     } else if (warp == kCompute + 1) {
       // ---------------------------------------------------------- products
-      constexpr uint32_t id_s = idesc(BF16, 128, false), id_o = idesc(BF16, DP, true);
+      constexpr uint32_t id_s = idesc(BF16, 128, false);
+      const int steps = steps_of(a.D);
+      const uint32_t id_o = idesc(BF16, steps * 16, true);
       const uint32_t k_addr = smem_u32(smem), v_addr = k_addr + C::kTile;
       const uint32_t q_ring = smem_u32(smem + C::kQ), do_ring = smem_u32(smem + C::kDo);
       bool ok = true;
@@ -307,7 +309,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t m = n + (uint32_t)i;
             if (!wait_warp(b.q_full + m % C::kNq, (m / C::kNq) & 1u, abort_flag)) return false;
             if (elect()) {
-              mma_columns<DP>(tmem + C::kS, k_addr, q_at(m), id_s);
+              mma_columns<DP>(tmem + C::kS, k_addr, q_at(m), id_s, steps);
               commit(&b.s);
               if (i + 1 == w.total) commit(&b.k_empty);
             }
@@ -318,7 +320,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t m = n + (uint32_t)i;
             if (!wait_warp(b.do_full + m % C::kNdo, (m / C::kNdo) & 1u, abort_flag)) return false;
             if (elect()) {
-              mma_columns<DP>(tmem + C::kDp, v_addr, do_at(m), id_s);
+              mma_columns<DP>(tmem + C::kDp, v_addr, do_at(m), id_s, steps);
               commit(&b.dp);
               if (i + 1 == w.total) commit(&b.v_empty);
             }
@@ -752,7 +754,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     } else if (warp == kCompute + 1) {
       // ---------------------------------------------------------- products
-      constexpr uint32_t id_s = idesc(BF16, 128, false), id_o = idesc(BF16, DP, true);
+      constexpr uint32_t id_s = idesc(BF16, 128, false);
+      const int steps = steps_of(a.D);
+      const uint32_t id_o = idesc(BF16, steps * 16, true);
       const uint32_t q_addr = smem_u32(smem), do_addr = q_addr + C::kTile;
       const uint32_t k_ring = smem_u32(smem + C::kKRing), v_ring = smem_u32(smem + C::kVRing);
       bool ok = true;
@@ -765,7 +769,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t m = n + (uint32_t)j;
             if (!wait_warp(b.k_full + m % C::kK, (m / C::kK) & 1u, abort_flag)) return false;
             if (elect()) {
-              mma_columns<DP>(tmem + C::kS + (m & 1) * 128, q_addr, k_ring + (m % C::kK) * C::kTile, id_s);
+              mma_columns<DP>(tmem + C::kS + (m & 1) * 128, q_addr, k_ring + (m % C::kK) * C::kTile, id_s, steps);
               commit(b.s + (m & 1));
               if (j + 1 == w.n) commit(&b.q_empty);
             }
@@ -776,7 +780,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t m = n + (uint32_t)j;
             if (!wait_warp(b.v_full + m % C::kV, (m / C::kV) & 1u, abort_flag)) return false;
             if (elect()) {
-              mma_columns<DP>(tmem + C::kDp, do_addr, v_ring + (m % C::kV) * C::kTile, id_s);
+              mma_columns<DP>(tmem + C::kDp, do_addr, v_ring + (m % C::kV) * C::kTile, id_s, steps);
               commit(&b.dp);
               commit(b.v_empty + m % C::kV);
               if (j + 1 == w.n) commit(&b.do_empty);
@@ -1101,7 +1105,7 @@ __global__ void __launch_bounds__(320, 1)
     }
   } else if (warp == 9) {
     // ------------------------------------------------------------ products
-    constexpr uint32_t id_o = idesc(BF16, DP, true) | (1u << 15);             // both operands contracted along their rows
+    const uint32_t id_o = idesc(BF16, steps_of(a.D) * 16, true) | (1u << 15);      // both operands contracted along their rows
     const uint32_t ring = smem_u32(smem);
     bool ok = true;
     uint32_t it = 0;

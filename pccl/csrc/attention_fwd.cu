@@ -223,7 +223,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     } else if (warp == 9) {
       // ---------------------------------------------------------- products
-      constexpr uint32_t id_s = idesc(BF16, 128, false), id_o = idesc(BF16, DP, true);
+      constexpr uint32_t id_s = idesc(BF16, 128, false);
+      const int steps = steps_of(a.D);
+      const uint32_t id_o = idesc(BF16, steps * 16, true);
       const uint32_t q_addr = smem_u32(smem), ring = smem_u32(smem + C::kRing);
       bool ok = true;
       uint32_t it = 0, s_count[2] = {0, 0}, items[2] = {0, 0};     // ring position; tiles and work items of each half
@@ -236,7 +238,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           auto loaded = [&](uint32_t i) { return wait_warp(b.full + i % C::kStages, (i / C::kStages) & 1u, abort_flag); };
           auto scores = [&](int h, int j) {
             if (elect()) {
-              mma_columns<DP>(tmem + C::kS + h * 128, q_addr + h * C::kTile, tile_at(it + 2 * j), id_s);
+              mma_columns<DP>(tmem + C::kS + h * 128, q_addr + h * C::kTile, tile_at(it + 2 * j), id_s, steps);
               commit(b.s + h);
               if (j + 1 == w.n[h]) commit(b.q_empty + h);    // the queries are not read again
             }
