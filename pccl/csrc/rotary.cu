@@ -16,6 +16,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "act.cuh"
 #include "pdl.cuh"
 #include "rotary.h"
 
@@ -25,36 +26,72 @@ namespace {
 
 constexpr int kForward = 128, kBackward = 256;               // threads of a block
 
-// Four elements of 16 bits, in a register pair.
+// A lane's eight elements: the first and the second members of its four pairs, two and two for the packed arithmetic.
+struct Pairs {
+  F2 a[2], b[2];
+};
 template <bool BF16>
-__device__ __forceinline__ void unpack4(const uint2& q, float* f) {
-  const uint32_t w[2] = {q.x, q.y};
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    if constexpr (BF16) {
-      f[2 * i] = __uint_as_float(w[i] << 16);
-      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    } else {
-      const float2 x = __half22float2(*reinterpret_cast<const __half2*>(w + i));
-      f[2 * i] = x.x;
-      f[2 * i + 1] = x.y;
-    }
+__device__ __forceinline__ void widen(uint32_t w, float& lo, float& hi) {
+  if constexpr (BF16) {
+    lo = __uint_as_float(w << 16);
+    hi = __uint_as_float(w & 0xffff0000u);
+  } else {
+    const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    lo = x.x;
+    hi = x.y;
   }
 }
 template <bool BF16>
-__device__ __forceinline__ uint2 pack4(const float* f) {
-  uint32_t w[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    if constexpr (BF16) {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
-      w[i] = *reinterpret_cast<const uint32_t*>(&h);
-    } else {
-      const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
-      w[i] = *reinterpret_cast<const uint32_t*>(&h);
-    }
+__device__ __forceinline__ uint32_t narrow(float lo, float hi) {
+  if constexpr (BF16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
   }
-  return make_uint2(w[0], w[1]);
+}
+// From the elements in the order of the columns (c0 on, c1 on) and back.
+template <bool NEIGHBOURS>
+__device__ __forceinline__ void pair_up(const float* e, Pairs& p) {
+  if constexpr (NEIGHBOURS) {
+    p.a[0] = f2(e[0], e[2]), p.a[1] = f2(e[4], e[6]);
+    p.b[0] = f2(e[1], e[3]), p.b[1] = f2(e[5], e[7]);
+  } else {
+    p.a[0] = f2(e[0], e[1]), p.a[1] = f2(e[2], e[3]);
+    p.b[0] = f2(e[4], e[5]), p.b[1] = f2(e[6], e[7]);
+  }
+}
+template <bool NEIGHBOURS>
+__device__ __forceinline__ void take_apart(const Pairs& p, float* e) {
+  if constexpr (NEIGHBOURS) {
+    split(p.a[0], e[0], e[2]), split(p.a[1], e[4], e[6]);
+    split(p.b[0], e[1], e[3]), split(p.b[1], e[5], e[7]);
+  } else {
+    split(p.a[0], e[0], e[1]), split(p.a[1], e[2], e[3]);
+    split(p.b[0], e[4], e[5]), split(p.b[1], e[6], e[7]);
+  }
+}
+template <bool BF16, bool NEIGHBOURS>
+__device__ __forceinline__ void unpack(const uint2& x, const uint2& y, Pairs& p) {
+  float e[8];
+  widen<BF16>(x.x, e[0], e[1]);
+  widen<BF16>(x.y, e[2], e[3]);
+  widen<BF16>(y.x, e[4], e[5]);
+  widen<BF16>(y.y, e[6], e[7]);
+  pair_up<NEIGHBOURS>(e, p);
+}
+template <bool BF16, bool NEIGHBOURS>
+__device__ __forceinline__ void store(uint16_t* x, uint16_t* y, const Pairs& p) {
+  float e[8];
+  take_apart<NEIGHBOURS>(p, e);
+  *reinterpret_cast<uint2*>(x) = make_uint2(narrow<BF16>(e[0], e[1]), narrow<BF16>(e[2], e[3]));
+  *reinterpret_cast<uint2*>(y) = make_uint2(narrow<BF16>(e[4], e[5]), narrow<BF16>(e[6], e[7]));
+}
+__device__ __forceinline__ float dot(const Pairs& x, const Pairs& y) {
+  float lo, hi;
+  split(fma2(x.a[0], y.a[0], fma2(x.a[1], y.a[1], fma2(x.b[0], y.b[0], x.b[1] * y.b[1]))), lo, hi);
+  return lo + hi;
 }
 template <int L>
 __device__ __forceinline__ float group_sum(float v) {
@@ -95,8 +132,17 @@ __device__ __forceinline__ Columns columns(int l, int half, int D) {
   c.c1 = apart ? half + l * 4 : l * 8 + 4;
   return c;
 }
+template <bool NEIGHBOURS>
+__device__ __forceinline__ void load_weights(const RotaryArgs& a, int which, const Columns& col, Pairs& w) {
+  float e[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (col.on) {
+    load_w4(a.w[which], a.w_type, col.c0, e);
+    load_w4(a.w[which], a.w_type, col.c1, e + 4);
+  }
+  pair_up<NEIGHBOURS>(e, w);
+}
 struct Angles {
-  float c[4], s[4];
+  F2 c[2], s[2];
 };
 __device__ __forceinline__ void load_angles(Angles& t, const RotaryArgs& a, int64_t pos, const Columns& col) {
   const bool known = pos >= 0 && pos < a.table;
@@ -109,21 +155,20 @@ __device__ __forceinline__ void load_angles(Angles& t, const RotaryArgs& a, int6
       s = *reinterpret_cast<const float4*>(a.sin + pos * a.half + col.angle);
     }
   }
-  t.c[0] = c.x, t.c[1] = c.y, t.c[2] = c.z, t.c[3] = c.w;
-  t.s[0] = s.x, t.s[1] = s.y, t.s[2] = s.z, t.s[3] = s.w;
+  t.c[0] = f2(c.x, c.y), t.c[1] = f2(c.z, c.w);
+  t.s[0] = f2(s.x, s.y), t.s[1] = f2(s.z, s.w);
 }
-// x[0..4) and x[4..8) of a lane turned by its angles (forward), or back.
-template <bool NEIGHBOURS, bool BACK>
-__device__ __forceinline__ void rotate(float* x, const Angles& t, bool turned) {
+// A lane's pairs turned by its angles (forward), or back.  Where not all columns are turned, those that are not (cos 1, or NaN for
+// an unknown position) keep clear of what their neighbours hold.
+template <bool BACK>
+__device__ __forceinline__ void rotate(Pairs& p, const Angles& t, bool all, bool turned) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float& a = x[NEIGHBOURS ? 2 * i : i];
-    float& b = x[NEIGHBOURS ? 2 * i + 1 : 4 + i];
-    const float s = BACK ? -t.s[i] : t.s[i];
-    // columns that are not turned (cos 1, or NaN for an unknown position) keep clear of what their neighbours hold
-    const float y = fmaf(a, t.c[i], turned ? -b * s : 0.f), z = fmaf(b, t.c[i], turned ? a * s : 0.f);
-    a = y;
-    b = z;
+  for (int i = 0; i < 2; ++i) {
+    const F2 s = BACK ? t.s[i] : t.s[i] * f2(-1.f), n = BACK ? t.s[i] * f2(-1.f) : t.s[i];
+    F2 x = p.b[i] * s, y = p.a[i] * n;
+    if (!all && !turned) x = y = f2(0.f);
+    p.a[i] = fma2(p.a[i], t.c[i], x);
+    p.b[i] = fma2(p.b[i], t.c[i], y);
   }
 }
 
@@ -160,17 +205,13 @@ __global__ void __launch_bounds__(kForward) rotary_forward_kernel(const __grid_c
   constexpr uint32_t groups = kForward / L;
   const Columns col = columns<NEIGHBOURS>(threadIdx.x & (L - 1), a.half, a.D);
   const float inv_d = 1.f / (float)a.D;
+  const bool all = 2 * a.half == a.D;
   uint32_t block, blocks;
   const int which = share_of(a, block, blocks);
   const RotaryTensor &tx = a.x[which], &ty = a.y[which];
   const uint32_t rows = (uint32_t)a.B * (uint32_t)a.S, chunks = (uint32_t)a.chunks[which];
-  float w[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) w[e] = 0.f;
-  if (col.on) {
-    load_w4(a.w[which], a.w_type, col.c0, w);
-    load_w4(a.w[which], a.w_type, col.c1, w + 4);
-  }
+  Pairs w;
+  load_weights<NEIGHBOURS>(a, which, col, w);
   // a group: one chunk of heads in one row; groups without one go through the exchanges with the others
   const uint64_t items = (uint64_t)rows * chunks, i = (uint64_t)block * groups + threadIdx.x / L;
   const bool exists = i < items;
@@ -192,20 +233,18 @@ __global__ void __launch_bounds__(kForward) rotary_forward_kernel(const __grid_c
     for (int u = 0; u < U; ++u) {
       if (r + u >= a.heads_per_item) break;
       const int h = it.h0 + r + u;
-      float x[8];
-      unpack4<BF16>(q[u][0], x);
-      unpack4<BF16>(q[u][1], x + 4);
-      float ss = 0.f;
+      Pairs x;
+      unpack<BF16, NEIGHBOURS>(q[u][0], q[u][1], x);
+      const F2 rs = f2(rsqrtf(fmaf(group_sum<L>(dot(x, x)), inv_d, a.eps)));
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
-      const float rs = rsqrtf(fmaf(group_sum<L>(ss), inv_d, a.eps));
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] *= rs * w[e];
-      rotate<NEIGHBOURS, false>(x, t, col.turned);
+      for (int i = 0; i < 2; ++i) {
+        x.a[i] = x.a[i] * (rs * w.a[i]);
+        x.b[i] = x.b[i] * (rs * w.b[i]);
+      }
+      rotate<false>(x, t, all, col.turned);
       if (h < h1) {
         uint16_t* p = row_at(ty, it.b, it.s, h);
-        *reinterpret_cast<uint2*>(p + col.c0) = pack4<BF16>(x);
-        *reinterpret_cast<uint2*>(p + col.c1) = pack4<BF16>(x + 4);
+        store<BF16, NEIGHBOURS>(p + col.c0, p + col.c1, x);
       }
     }
   }
@@ -221,17 +260,15 @@ __global__ void __launch_bounds__(kBackward, 2) rotary_backward_kernel(const __g
   constexpr uint32_t groups = kBackward / L;
   const Columns col = columns<NEIGHBOURS>(threadIdx.x & (L - 1), a.half, a.D);
   const float inv_d = 1.f / (float)a.D;
+  const bool all = 2 * a.half == a.D;
   uint32_t block, blocks;
   const int which = share_of(a, block, blocks);
   const RotaryTensor &tx = a.x[which], &td = a.dy[which], &ty = a.y[which];
   const uint32_t rows = (uint32_t)a.B * (uint32_t)a.S, chunks = (uint32_t)a.chunks[which];
-  float w[8], dw[8];
+  Pairs w, dw;
+  load_weights<NEIGHBOURS>(a, which, col, w);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) w[e] = dw[e] = 0.f;
-  if (col.on) {
-    load_w4(a.w[which], a.w_type, col.c0, w);
-    load_w4(a.w[which], a.w_type, col.c1, w + 4);
-  }
+  for (int i = 0; i < 2; ++i) dw.a[i] = dw.b[i] = f2(0.f);
   const uint64_t items = (uint64_t)rows * chunks;
   for (uint64_t i0 = (uint64_t)block * groups; i0 < items; i0 += (uint64_t)blocks * groups) {
     const uint64_t i = i0 + threadIdx.x / L;
@@ -256,30 +293,31 @@ __global__ void __launch_bounds__(kBackward, 2) rotary_backward_kernel(const __g
       for (int u = 0; u < U; ++u) {
         if (r + u >= a.heads_per_item) break;
         const int h = it.h0 + r + u;
-        float x[8], g[8];
-        unpack4<BF16>(qx[u][0], x);
-        unpack4<BF16>(qx[u][1], x + 4);
-        unpack4<BF16>(qd[u][0], g);
-        unpack4<BF16>(qd[u][1], g + 4);
-        rotate<NEIGHBOURS, true>(g, t, col.turned);          // the gradient behind the weights
-        float ss = 0.f, dot = 0.f;
+        Pairs x, g;
+        unpack<BF16, NEIGHBOURS>(qx[u][0], qx[u][1], x);
+        unpack<BF16, NEIGHBOURS>(qd[u][0], qd[u][1], g);
+        rotate<true>(g, t, all, col.turned);                 // the gradient behind the weights
+        const F2 rs = f2(rsqrtf(fmaf(group_sum<L>(dot(x, x)), inv_d, a.eps)));
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
-        const float rs = rsqrtf(fmaf(group_sum<L>(ss), inv_d, a.eps));
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          x[e] *= rs;
-          if (h < h1) dw[e] = fmaf(g[e], x[e], dw[e]);
-          g[e] *= w[e];
-          dot = fmaf(g[e], x[e], dot);
+        for (int i = 0; i < 2; ++i) {
+          x.a[i] = x.a[i] * rs;
+          x.b[i] = x.b[i] * rs;
+          if (h < h1) {                                      // behind the last head an unknown position's NaN stands in g
+            dw.a[i] = fma2(g.a[i], x.a[i], dw.a[i]);
+            dw.b[i] = fma2(g.b[i], x.b[i], dw.b[i]);
+          }
+          g.a[i] = g.a[i] * w.a[i];
+          g.b[i] = g.b[i] * w.b[i];
         }
-        dot = group_sum<L>(dot) * inv_d;
+        const F2 mean = f2(group_sum<L>(dot(g, x)) * -inv_d);
         if (h < h1) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) g[e] = rs * fmaf(-x[e], dot, g[e]);
+          for (int i = 0; i < 2; ++i) {
+            g.a[i] = rs * fma2(x.a[i], mean, g.a[i]);
+            g.b[i] = rs * fma2(x.b[i], mean, g.b[i]);
+          }
           uint16_t* p = row_at(ty, it.b, it.s, h);
-          *reinterpret_cast<uint2*>(p + col.c0) = pack4<BF16>(g);
-          *reinterpret_cast<uint2*>(p + col.c1) = pack4<BF16>(g + 4);
+          store<BF16, NEIGHBOURS>(p + col.c0, p + col.c1, g);
         }
       }
     }
@@ -287,10 +325,12 @@ __global__ void __launch_bounds__(kBackward, 2) rotary_backward_kernel(const __g
   // the block's groups in order
   const int at = (threadIdx.x / L) * (L * 8);
   if (col.on) {
+    float e[8];
+    take_apart<NEIGHBOURS>(dw, e);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      sums[at + col.c0 + e] = dw[e];
-      sums[at + col.c1 + e] = dw[4 + e];
+    for (int i = 0; i < 4; ++i) {
+      sums[at + col.c0 + i] = e[i];
+      sums[at + col.c1 + i] = e[4 + i];
     }
   }
   __syncthreads();
@@ -309,8 +349,15 @@ __global__ void __launch_bounds__(kBackward) rotary_weights_kernel(const __grid_
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.x * 32 + lane, which = blockIdx.y;
   const int first = which ? a.q_blocks : 0, last = which ? blocks : a.q_blocks;
   float s = 0.f;
-  if (c < a.D)
-    for (int b = first + warp; b < last; b += 8) s += a.partial[(int64_t)b * a.D + c];
+  if (c < a.D) {
+    for (int b = first + warp; b < last; b += 64) {          // eight loads on their way at once
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = b + i * 8 < last ? a.partial[(int64_t)(b + i * 8) * a.D + c] : 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s += x[i];
+    }
+  }
   sums[warp][lane] = s;
   __syncthreads();
   if (warp == 0 && c < a.D) {
