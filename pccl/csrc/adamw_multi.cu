@@ -281,9 +281,19 @@ __device__ __forceinline__ void fetch(const AdamMultiArgs& a, const Table<MAX>& 
   }
 }
 
+// A warp's 256 numbers, written by neighbouring lanes in turn: eight neighbours of each lane.
+__device__ __forceinline__ void exchange(const float* s, float* x) {
+  __syncwarp();
+  const float4 a = reinterpret_cast<const float4*>(s)[(threadIdx.x & 31) * 2], b = reinterpret_cast<const float4*>(s)[(threadIdx.x & 31) * 2 + 1];
+  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
+  x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+  __syncwarp();
+}
+
 template <int PT, int GT, bool BITS8, int MAX>
 __global__ void __launch_bounds__(kThreads, BITS8 ? 4 : 3) adamw_multi_kernel(const __grid_constant__ AdamMultiArgs a,
                                                                               const __grid_constant__ Table<MAX> table) {
+  __shared__ __align__(16) float stage[kThreads / 32][kAdamBlock];
   pdl_wait();
   pdl_trigger();
   const int lane = threadIdx.x & 31;
@@ -313,37 +323,34 @@ __global__ void __launch_bounds__(kThreads, BITS8 ? 4 : 3) adamw_multi_kernel(co
     if (whole) {
       widen<GT>(x.g, g);
       widen<kAdamF32>(x.p, p);
-      if constexpr (!BITS8) {
-        Raw8 rm, rv;
-        load8<kAdamF32>(a.m, (int64_t)si, rm);
-        load8<kAdamF32>(a.v, (int64_t)si, rv);
-        float y[8], z[8];
-        widen<kAdamF32>(rm, y);
-        widen<kAdamF32>(rv, z);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          m[i] = f2(y[2 * i], y[2 * i + 1]);
-          v[i] = f2(z[2 * i], z[2 * i + 1]);
-        }
-      }
     } else {
-      float y[8], z[8];
+      // off vector boundaries, or a tensor's end: neighbouring lanes read neighbouring elements, and change them for eight in a row
+      const int64_t first = at - lane * 8;
+      float* s = stage[threadIdx.x >> 5];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const bool on = at + i < t.n;
-        g[i] = on ? load1<GT>(t.grad, at + i) : 0.f;
-        p[i] = on ? static_cast<const float*>(weights)[at + i] : 0.f;
-        if constexpr (!BITS8) {
-          y[i] = on ? static_cast<const float*>(a.m)[si + i] : 0.f;
-          z[i] = on ? static_cast<const float*>(a.v)[si + i] : 0.f;
-        }
+        const int64_t e = first + i * 32 + lane;
+        s[i * 32 + lane] = e < t.n ? load1<GT>(t.grad, e) : 0.f;
       }
-      if constexpr (!BITS8) {
+      exchange(s, g);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          m[i] = f2(y[2 * i], y[2 * i + 1]);
-          v[i] = f2(z[2 * i], z[2 * i + 1]);
-        }
+      for (int i = 0; i < 8; ++i) {
+        const int64_t e = first + i * 32 + lane;
+        s[i * 32 + lane] = e < t.n ? static_cast<const float*>(weights)[e] : 0.f;
+      }
+      exchange(s, p);
+    }
+    if constexpr (!BITS8) {
+      Raw8 rm, rv;
+      load8<kAdamF32>(a.m, (int64_t)si, rm);
+      load8<kAdamF32>(a.v, (int64_t)si, rv);
+      float y[8], z[8];
+      widen<kAdamF32>(rm, y);
+      widen<kAdamF32>(rv, z);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        m[i] = f2(y[2 * i], y[2 * i + 1]);
+        v[i] = f2(z[2 * i], z[2 * i + 1]);
       }
     }
     blk += warps;
@@ -398,33 +405,34 @@ __global__ void __launch_bounds__(kThreads, BITS8 ? 4 : 3) adamw_multi_kernel(co
       __stcs(reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.v) + si), make_uint2(cv[0], cv[1]));
     }
     // ---- stores
+    if constexpr (!BITS8) {                                    // behind a tensor's end: zeros, as they were
+      float y[8], z[8];
+      unpair(m, y);
+      unpair(v, z);
+      store32(static_cast<float*>(a.m) + si, y);
+      store32(static_cast<float*>(a.v) + si, z);
+    }
     if (whole) {
-      if constexpr (!BITS8) {
-        float x[8], y[8];
-        unpair(m, x);
-        unpair(v, y);
-        store32(static_cast<float*>(a.m) + si, x);
-        store32(static_cast<float*>(a.v) + si, y);
-      }
       store32(static_cast<float*>(weights) + at, p);
       if constexpr (PT != kAdamF32)
         *reinterpret_cast<uint4*>(static_cast<uint16_t*>(t.param) + at) =
             make_uint4(narrow2<PT>(p[0], p[1]), narrow2<PT>(p[2], p[3]), narrow2<PT>(p[4], p[5]), narrow2<PT>(p[6], p[7]));
     } else {
-      float x[8], y[8];
-      unpair(m, x);
-      unpair(v, y);
+      const int64_t first = at - lane * 8;
+      float* s = stage[threadIdx.x >> 5];
+      reinterpret_cast<float4*>(s)[lane * 2] = make_float4(p[0], p[1], p[2], p[3]);
+      reinterpret_cast<float4*>(s)[lane * 2 + 1] = make_float4(p[4], p[5], p[6], p[7]);
+      __syncwarp();
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        if (at + i < t.n) {
-          if constexpr (!BITS8) {
-            static_cast<float*>(a.m)[si + i] = x[i];
-            static_cast<float*>(a.v)[si + i] = y[i];
-          }
-          static_cast<float*>(weights)[at + i] = p[i];
-          if constexpr (PT != kAdamF32) store1<PT>(t.param, at + i, p[i]);
+        const int64_t e = first + i * 32 + lane;
+        if (e < t.n) {
+          const float y = s[i * 32 + lane];
+          static_cast<float*>(weights)[e] = y;
+          if constexpr (PT != kAdamF32) store1<PT>(t.param, e, y);
         }
       }
+      __syncwarp();
     }
     if (!more) break;
     if constexpr (BITS8) fetch<PT, GT, BITS8, MAX>(a, table, blk, x.k, x);
