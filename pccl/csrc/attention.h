@@ -40,9 +40,6 @@ struct AttnArgs {
   int parts_o, parts_dq, parts_dkv;  // 1: not split
   float* partial;
   float* partial_lse;                // forward: lse of each part, [part][batch][head][row]
-  // Backward: the score gradients as the dk/dv kernel makes them, 128 x 128 tiles of 16 bits, for dq; nullptr: dq computes them again.
-  uint16_t* ds;
-  int64_t ds_tiles;                  // of one head
 };
 
 constexpr int kAttnMaxDim = 128;     // columns of a head: a multiple of 8 up to this
@@ -51,7 +48,6 @@ constexpr int kAttnMaxDim = 128;     // columns of a head: a multiple of 8 up to
 struct AttnScratch {
   int64_t partial, partial_lse;
   int64_t order_q, order_k;          // entries
-  int64_t ds;                        // elements
 };
 AttnScratch plan_attention_forward(AttnArgs& a, int sm_count);
 AttnScratch plan_attention_backward(AttnArgs& a, int sm_count);

@@ -189,11 +189,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_backward(const at::Tens
   a.delta = delta.data_ptr<float>();
   a.zero_tail = !dq_.has_value();
   const AttnScratch need = plan_attention_backward(a, at::cuda::getCurrentDeviceProperties()->multiProcessorCount);
-  at::Tensor partial, order, ds;
-  if (need.ds > 0) {
-    ds = at::empty({need.ds}, q.options());
-    a.ds = reinterpret_cast<uint16_t*>(ds.data_ptr());
-  }
+  at::Tensor partial, order;
   if (need.order_q > 0) {
     order = at::empty({2 * (need.order_q + need.order_k)}, q.options().dtype(at::kInt));
     a.order_q = reinterpret_cast<int2*>(order.data_ptr<int>());

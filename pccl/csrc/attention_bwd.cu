@@ -1,12 +1,12 @@
 // Attention, backward pass: a kernel for the row sums <do_i, o_i>, one for dk and dv, one for dq (attention.h has the formulas,
 // attention.cuh the tiles).
 //
-// Two kernels share the work so that every gradient has one owner: a CTA keeps 128 keys (dk, dv) or some queries (dq) and walks
-// over the others, and its sums stay in tensor memory until they are complete: no atomic additions of a whole dq per key tile, and
-// results are the same bits from run to run.  The heads of a group are walked over one after the other by the CTA that owns their
-// shared key head.  For dq there are two forms.  Either the dk/dv kernel leaves its score gradients, rounded to 16 bits as its
-// own product reads them, in memory, and dq = dS K is one product behind it; or, for packed sequences and where those tiles would
-// take more than 1 GiB, dq computes scores and do v^T again: seven products instead of five.
+// Two kernels share the work so that every gradient has one owner: a CTA keeps 128 keys (dk, dv) or 128 queries (dq) and walks
+// over the others, and its sums stay in tensor memory until they are complete.  Scores and do v^T are computed twice, seven
+// products instead of five; what is saved are fp32 atomic additions of a whole dq per key tile, and results are the same bits
+// from run to run.  (Leaving the score gradients in memory for dq instead was tried: 2 to 4 % faster for 4 x 2048 x 16 heads, up to 50 %
+// slower for small calls, and up to 1 GiB of memory.)  The heads of a group are walked over one after the other by the CTA that
+// owns their shared key head.
 //
 //   warps 0-7   probabilities and score gradients: two warpgroups, each with half of a tile's 128 columns
 //   warp 8      TMA; asks for the next tile of the grid (attention.cuh)
@@ -18,6 +18,12 @@
 //   S(i) | P(i): dv += P^T dO, S(i+1) | dS(i): dk += dS^T Q, dP(i+1) | ...
 // dq: S = Q K^T and dP = dO V^T as in the forward pass, dq += dS K; S is kept twice, so that its next tile is ready when the
 // exponentials of the last one are done.
+//
+// What bounds it.  4 x 2048 x 16 heads of 128 causal take 250 us, 687 TFLOP/s by the five products that the formulas need and 960
+// by the seven computed: row sums 10 us (6.4 TB/s), dk and dv 132, dq 103.  With the exponentials and conversions left out the
+// products alone take 110 and 87: tensor memory holds four or five 128 x 128 accumulators and no more, so a product waits for its
+// operand's conversion at every tile, with one tile of the other chain in between.  Sixteen compute warps for eight: no faster.  The
+// clock is at 1.69 GHz by the power limit.  16 heads of 4096 223 us (768 TFLOP/s), heads of 64 199.
 #include "attention.cuh"
 
 namespace pccl {
@@ -29,7 +35,6 @@ using namespace attn;
 constexpr int kCompute = 8;                     // warps that make probabilities and score gradients, 512 / kCompute columns each
 constexpr int kCols = 512 / kCompute;
 constexpr int kThreads = kCompute * 32 + 128;
-constexpr int64_t kKeepBytes = (int64_t)1 << 30;                // of score gradients that are kept in memory for dq
 
 // ---------------------------------------------------------------- row sums
 // delta_i = <do_i, o_i>: sixteen lanes per row.  One read of both tensors.
@@ -108,25 +113,6 @@ struct DkvBars {
   int abort;
 };
 static_assert(sizeof(DkvBars) <= 512, "the barriers' part of shared memory");
-
-// Score gradients in memory: the tiles of a head by key tile, each with the query tiles that see it (from first on).  A tile is
-// [group of 16 queries][key][16 queries]: a warp's lanes, a key each, then write 1 KiB in a row (rows of 128 queries per key were 45 us
-// slower for 4 x 2048 x 16 heads), and the copy engine moves it as one piece of 32 KiB.  The halves of a key's 32 bytes change
-// places where bit 2 of the key is set: the 32-byte swizzle that the product expects of an operand of such rows.
-__host__ __device__ __forceinline__ int64_t ds_first(const AttnArgs& a, int64_t kt) {
-  if (!a.causal) return 0;
-  const int64_t x = kt * 128 - ((int64_t)a.Sk - a.Sq);       // the first query that sees the tile's first key
-  return x > 0 ? x / 128 : 0;
-}
-// Tiles of a head before those of key tile kt.  first(k) = max(0, k - c) with c the rows between, in tiles, rounded up.
-__host__ __device__ __forceinline__ int64_t ds_before(const AttnArgs& a, int64_t kt) {
-  const int64_t tiles = ((int64_t)a.Sq + 127) / 128;
-  if (!a.causal) return kt * tiles;
-  const int64_t off = (int64_t)a.Sk - a.Sq, c = off >= 0 ? (off + 127) / 128 : -(-off / 128);
-  if (c < 0) return kt * tiles - (kt * (kt - 1) / 2 - kt * c);
-  const int64_t m = kt - 1 - c > 0 ? kt - 1 - c : 0;
-  return kt * tiles - m * (m + 1) / 2;
-}
 
 // The keys of one tile number, and the query tiles that see one of them: per_head of them from tile `first` on, for each head
 // of the group.  Of that sequence of steps, `total` from i0 on are this part's.
@@ -414,17 +400,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       const DkvWork w = dkv_work_at<SPLIT>(a, (unsigned)id);
       const int key = w.key0 + (warp & 3) * 32 + lane;
       int tile = w.first + (w.per_head > 0 ? w.i0 % w.per_head : 0);            // query tile within its head
-      // where this thread's part of the next score gradients goes
-      uint16_t* ds_out = nullptr;
-      if (a.ds != nullptr && w.total > 0) {
-        const int64_t head = (int64_t)w.sp.batch * a.H + w.kv_head * group + w.i0 / w.per_head;
-        ds_out = a.ds + (head * a.ds_tiles + ds_before(a, w.sp.tile) + tile - w.first) * 16384 + (g * (kCols / 16) * 128 + (warp & 3) * 32 + lane) * 16;
-      }
       for (int i = 0; i < w.total; ++i, ++n) {
         const float* st = reinterpret_cast<const float*>(smem + C::kStat) + (n & 1) * 256 + g * kCols;
         const int q0 = tile * 128 + g * kCols;
-        const bool head_ends = ++tile == w.first + w.per_head;
-        if (head_ends) tile = w.first;
+        if (++tile == w.first + w.per_head) tile = w.first;
         const int hidden = a.causal ? key - w.offset - q0 : 0;               // this key is not seen by the first so many queries
         const bool masked = a.causal && w.key0 + (warp & 3) * 32 + 31 - w.offset - q0 > 0;
         if (!(ok = wait_warp(b.stat_full + (n & 1), (n >> 1) & 1u, abort_flag))) break;
@@ -488,19 +467,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             wd[e + 1] = pack2<BF16>(x[2], x[3]);
           }
           tmem_st16(t_dp + c * 16, wd);
-          if (ds_out != nullptr) {
-            // keys that do not exist: what stands here is not even finite for sure
-            const bool there = key < w.sp.len_k, turned = (lane & 4) != 0;
-#pragma unroll
-            for (int v = 0; v < 2; ++v) {
-              uint32_t x[8];
-#pragma unroll
-              for (int e = 0; e < 8; ++e) x[e] = there ? (turned ? wd[v * 8 + (e ^ 4)] : wd[v * 8 + e]) : 0u;
-              store_words(ds_out + (c * 2 + v) * 2048, x);
-            }
-          }
         }
-        if (ds_out != nullptr) ds_out += (head_ends ? a.ds_tiles - w.per_head + 1 : 1) * 16384;
         tmem_wait_st();
         fence_before();
         __syncwarp();
@@ -949,253 +916,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// ---------------------------------------------------------------- dq from score gradients in memory
-// dq = dS K for 256 queries per CTA, two accumulators that share the key tiles, kept twice so that the end of one tile overlaps
-// the next.  dS lies transposed, [key][query], and is read as it lies.  A stream of 32 KiB tiles into a ring of six; bound by
-// the memory that dS comes from.
-template <int DP>
-struct Dsq {
-  static constexpr int kStages = 6;
-  static constexpr uint32_t kTile = 2 * kBlockBytes;         // of a ring slot: a tile of dS; key tiles of 64 columns leave half empty
-  static constexpr uint32_t kKeyBytes = (DP / 64) * kBlockBytes;
-  static constexpr uint32_t kBars = kStages * kTile;
-  static constexpr uint32_t kSmem = kBars + 512 + 1024;
-  static constexpr int kReaders = 10;                        // of the next tile's number: all warps
-};
-struct DsqBars {
-  Handle next[2];
-  uint64_t next_full[2], next_empty[2], full[6], empty[6], out_full[2], out_empty[2], drain;
-  uint32_t tmem;
-  int abort;
-};
-static_assert(sizeof(DsqBars) <= 512, "the barriers' part of shared memory");
-
-// The first operand: rows of 32 bytes, eight of them 256 bytes, groups of 16 queries 4096 bytes apart, 32-byte swizzle.
-constexpr uint32_t kDescHi32 = (256u >> 4) | (1u << 14) | (6u << 29);
-__device__ __forceinline__ uint32_t desc_rows32(uint32_t addr) { return ((addr & 0x3FFFFu) >> 4) + ((4096u >> 4) << 16); }
-__device__ __forceinline__ void mma_rows32(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t id, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "mov.b64 da, {%1, %5};\n\t"
-      "mov.b64 db, {%2, %6};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}"
-      ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(id), "r"(accumulate), "r"(kDescHi32), "r"(kDescHi)
-      : "memory");
-}
-
-struct DsqWork {
-  int batch, head, row0, part, j0, n[2];                     // key tiles of each half, from j0 on
-};
-template <bool SPLIT>
-__device__ __forceinline__ DsqWork dsq_work_at(const AttnArgs& a, unsigned id, int tiles) {
-  DsqWork w;
-  w.part = 0;
-  if constexpr (SPLIT) {
-    w.part = (int)(id % (unsigned)a.parts_dq);
-    id /= (unsigned)a.parts_dq;
-  }
-  const unsigned heads = (unsigned)(a.B * a.H), bh = id % heads;
-  const int t = (int)(id / heads);
-  w.head = (int)(bh % (unsigned)a.H);
-  w.batch = (int)(bh / (unsigned)a.H);
-  w.row0 = (a.causal ? tiles - 1 - t : t) * 256;                              // most keys first
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int first = w.row0 + h * 128, last = first + 127 < a.Sq - 1 ? first + 127 : a.Sq - 1;
-    const int keys = !a.causal ? a.Sk : (last + a.Sk - a.Sq + 1 < a.Sk ? last + a.Sk - a.Sq + 1 : a.Sk);
-    w.n[h] = first < a.Sq && keys > 0 ? (keys + 127) / 128 : 0;
-  }
-  w.j0 = 0;
-  if constexpr (SPLIT) {
-    const int most = w.n[0] > w.n[1] ? w.n[0] : w.n[1];
-    w.j0 = most * w.part / a.parts_dq;
-    const int j1 = most * (w.part + 1) / a.parts_dq;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int end = w.n[h] < j1 ? w.n[h] : j1;
-      w.n[h] = end > w.j0 ? end - w.j0 : 0;
-    }
-  }
-  return w;
-}
-
-template <int DP, bool BF16, bool SPLIT>
-__global__ void __launch_bounds__(320, 1)
-    attention_dsq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ AttnArgs a, int tiles) {
-  using C = Dsq<DP>;
-  extern __shared__ unsigned char smem_raw[];
-  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  DsqBars& b = *reinterpret_cast<DsqBars*>(smem + C::kBars);
-  volatile int* abort_flag = &b.abort;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < C::kStages; ++i) {
-      mbar_init(b.full + i, 1);
-      mbar_init(b.empty + i, 1);
-    }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(b.next_full + i, 1);
-      mbar_init(b.next_empty + i, C::kReaders);
-      mbar_init(b.out_full + i, 1);
-      mbar_init(b.out_empty + i, 8);
-    }
-    mbar_init(&b.drain, 1);
-    b.abort = 0;
-    fence_mbar_init();
-  }
-  if (warp == 9) tmem_alloc(&b.tmem, 512);
-  fence_before();
-  __syncthreads();
-  fence_after();
-  const uint32_t tmem = b.tmem;
-  pdl_wait();
-  pdl_trigger();
-
-  auto next_tile = [&](int k) {
-    if (!wait_warp(b.next_full + (k & 1), (k >> 1) & 1u, abort_flag)) return -2;
-    const int id = work_taken(b.next + (k & 1));
-    __syncwarp();
-    if (lane == 0) mbar_arrive(b.next_empty + (k & 1));
-    return id;
-  };
-  auto fail = [&](int code) {
-    if (lane == 0) {
-      atomicCAS(a.error, 0, code);
-      *abort_flag = 1;
-    }
-  };
-
-  if (warp == 8) {
-    // ------------------------------------------------------------ loads, and the tiles to come
-    bool ok = true;
-    uint32_t it = 0;
-    int id = (int)blockIdx.x;
-    for (int k = 0; ok; ++k) {
-      if (k >= 2 && !(ok = wait_warp(b.next_empty + (k & 1), ((k >> 1) - 1) & 1u, abort_flag))) break;
-      if (lane == 0) ask_for_work(b.next + (k & 1), b.next_full + (k & 1));
-      const DsqWork w = dsq_work_at<SPLIT>(a, (unsigned)id, tiles);
-      const int kv_head = w.head / (a.H / a.Hk), nmax = w.n[0] > w.n[1] ? w.n[0] : w.n[1];
-      const int64_t head_tiles = ((int64_t)w.batch * a.H + w.head) * a.ds_tiles;
-      for (int j = 0; j < nmax && ok; ++j) {
-        const int kt = w.j0 + j;
-        const int64_t tile0 = head_tiles + ds_before(a, kt) - ds_first(a, kt) + w.row0 / 128;
-#pragma unroll
-        for (int what = 0; what < 3; ++what) {               // dS of the two halves, then the keys
-          if (what < 2 && j >= w.n[what]) continue;
-          const uint32_t st = it % C::kStages;
-          if (!(ok = wait_warp(b.empty + st, ((it / C::kStages) & 1u) ^ 1u, abort_flag))) break;
-          ++it;
-          if (lane == 0) {
-            unsigned char* dst = smem + st * C::kTile;
-            mbar_expect_tx(b.full + st, what < 2 ? C::kTile : C::kKeyBytes);
-            if (what < 2) bulk_load(dst, a.ds + (tile0 + what) * 16384, C::kTile, b.full + st);
-            else load_tile<DP>(dst, &map_k, kv_head, kt * 128, w.batch, b.full + st);
-          }
-        }
-      }
-      if (!ok) break;
-      id = next_tile(k);
-      ok = id != -2;
-      if (id < 0) break;
-    }
-    if (!ok) {
-      fail(kErrLoad);
-      for (int i = 0; i < 1000; ++i) __nanosleep(1000);      // which copies are on their way is not known: the time that they can take
-    }
-  } else if (warp == 9) {
-    // ------------------------------------------------------------ products
-    const uint32_t id_o = idesc(BF16, steps_of(a.D) * 16, true) | (1u << 15);      // both operands contracted along their rows
-    const uint32_t ring = smem_u32(smem);
-    bool ok = true;
-    uint32_t it = 0;
-    int id = (int)blockIdx.x;
-    for (int k = 0; ok; ++k) {
-      const DsqWork w = dsq_work_at<SPLIT>(a, (unsigned)id, tiles);
-      const int nmax = w.n[0] > w.n[1] ? w.n[0] : w.n[1], buf = k & 1;
-      // these accumulators' last sums have been read
-      if (!(ok = wait_warp(b.out_empty + buf, ((k >> 1) & 1u) ^ 1u, abort_flag))) break;
-      fence_after();
-      for (int j = 0; j < nmax; ++j) {
-        const int count = (j < w.n[0] ? 1 : 0) + (j < w.n[1] ? 1 : 0) + 1;
-        for (int i = 0; i < count && ok; ++i) ok = wait_warp(b.full + (it + i) % C::kStages, ((it + i) / C::kStages) & 1u, abort_flag);
-        if (!ok) break;
-        const uint32_t keys = ring + ((it + count - 1) % C::kStages) * C::kTile;
-        if (elect()) {
-          uint32_t s = it;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (j >= w.n[h]) continue;
-            const uint32_t da = desc_rows32(ring + (s % C::kStages) * C::kTile), db = desc_mn(keys);
-#pragma unroll
-            for (int x = 0; x < 8; ++x)
-              mma_rows32(tmem + buf * 256 + h * 128, da + x * (512 >> 4), db + x * (2048 >> 4), id_o, (j > 0 || x > 0) ? 1u : 0u);
-            ++s;
-          }
-          for (int i = 0; i < count; ++i) commit(b.empty + (it + i) % C::kStages);
-          if (j + 1 == nmax) commit(b.out_full + buf);
-        }
-        __syncwarp();
-        it += (uint32_t)count;
-      }
-      if (!ok) break;
-      if (nmax == 0) {                                       // nothing to multiply: the others go by the same count
-        if (elect()) commit(b.out_full + buf);
-        __syncwarp();
-      }
-      id = next_tile(k);
-      ok = id != -2;
-      if (id < 0) break;
-    }
-    if (!ok) fail(kErrMma);
-    __syncwarp();
-    if (elect()) commit(&b.drain);
-    __syncwarp();
-    mbar_wait(&b.drain, 0, kWaitNs);
-  } else {
-    // ------------------------------------------------------------ results: four warps per half
-    const int h = warp >> 2;
-    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const bool wide = rows_are_wide(a.dq);
-    bool ok = true;
-    int id = (int)blockIdx.x;
-    for (int k = 0; ok; ++k) {
-      const DsqWork w = dsq_work_at<SPLIT>(a, (unsigned)id, tiles);
-      const int buf = k & 1, row = w.row0 + h * 128 + (warp & 3) * 32 + lane, n = h == 0 ? w.n[0] : w.n[1];
-      if (!(ok = wait_warp(b.out_full + buf, (k >> 1) & 1u, abort_flag))) break;
-      fence_after();
-      const bool exists = row < a.Sq;
-      uint16_t* out = row_ptr(a.dq, w.batch, w.head, row);
-#pragma unroll
-      for (int c = 0; c < DP / 32; ++c) {
-        uint32_t o[32];
-#pragma unroll
-        for (int e = 0; e < 32; ++e) o[e] = 0;
-        if (n > 0) {
-          tmem_ld32(tmem + buf * 256 + h * 128 + lanes + c * 32, o);
-          tmem_wait_ld(o);
-        }
-        if (!exists) continue;
-        if constexpr (SPLIT) store32_f32(part_row(a.partial, w.part, a.B, a.H, a.Sq, a.D, w.batch, w.head, row), c * 32, a.D, o, a.scale);
-        else store32<BF16>(out, c * 32, a.D, o, a.scale, wide);
-      }
-      fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(b.out_empty + buf);
-      id = next_tile(k);
-      ok = id != -2;
-      if (id < 0) break;
-    }
-    if (!ok) fail(kErrCompute);
-  }
-  fence_before();
-  __syncthreads();
-  if (warp == 9) {
-    fence_after();
-    tmem_free(tmem, 512);
-  }
-}
-
 // A gradient from its parts, added up in order: dst = sum of `parts` arrays of [batch][head][row][D].  Sixteen lanes per row.
 template <bool BF16>
 __global__ void __launch_bounds__(256) attention_sum_kernel(const float* partial, int parts, AttnTensor dst, int B, int H, int S, int D) {
@@ -1261,15 +981,6 @@ cudaError_t launch_dq(const CUtensorMap& mq, const CUtensorMap& mk, const CUtens
                     (int)tiles, beside);
 }
 
-template <int DP, bool BF16, bool SPLIT>
-cudaError_t launch_dsq(const CUtensorMap& mk, const AttnArgs& a, cudaStream_t stream) {
-  const cudaError_t e = allow_smem<attention_dsq_kernel<DP, BF16, SPLIT>>(Dsq<DP>::kSmem);
-  if (e != cudaSuccess) return e;
-  const int64_t tiles = ((int64_t)a.Sq + 255) / 256, ctas = tiles * a.H * a.B * a.parts_dq;
-  if (ctas > INT32_MAX) return cudaErrorInvalidValue;
-  return launch_pdl(attention_dsq_kernel<DP, BF16, SPLIT>, dim3((unsigned)ctas), dim3(320), Dsq<DP>::kSmem, stream, mk, a, (int)tiles);
-}
-
 template <int DP, bool BF16>
 cudaError_t launch(const AttnArgs& a, cudaStream_t stream) {
   const bool packed = a.cu_q != nullptr;
@@ -1300,9 +1011,7 @@ cudaError_t launch(const AttnArgs& a, cudaStream_t stream) {
     }
   }
   if (a.Sq > 0) {
-    cudaError_t e;
-    if (a.ds != nullptr) e = a.parts_dq > 1 ? launch_dsq<DP, BF16, true>(mk, a, stream) : launch_dsq<DP, BF16, false>(mk, a, stream);
-    else e = a.parts_dq > 1 ? launch_dq<DP, BF16, true>(mq, mk, mv, mdo, a, stream) : launch_dq<DP, BF16, false>(mq, mk, mv, mdo, a, stream);
+    cudaError_t e = a.parts_dq > 1 ? launch_dq<DP, BF16, true>(mq, mk, mv, mdo, a, stream) : launch_dq<DP, BF16, false>(mq, mk, mv, mdo, a, stream);
     if (e != cudaSuccess) return e;
     if (a.parts_dq > 1 && (e = add_parts<BF16>(a.partial, a.parts_dq, a.dq, a.B, a.H, a.Sq, a.D, stream)) != cudaSuccess) return e;
   }
@@ -1311,13 +1020,16 @@ cudaError_t launch(const AttnArgs& a, cudaStream_t stream) {
 
 }  // namespace
 
-// Tiles are split where they alone leave SMs without work, into parts of two key tiles (dq) or four steps (dk, dv) or more.  A group
-// of many heads on few key heads makes few and long tiles: those are cut until there are two for each SM.  Both kernels use the
-// same memory for their parts, one after the other.  Score gradients are kept for dq where they take 1 GiB or less.
+// Tiles are split where they alone leave SMs without work and the longest walk is of sixteen steps or more, into parts of four steps
+// or more: the parts' sums take another launch each and part the kernels for dk, dv and dq, about eight steps' time.  A group of many
+// heads on few key heads makes few and long tiles: those are cut until there are two for each SM.  Both kernels use the same
+// memory for their parts, one after the other.  Measured, whole / split (us): 2048 x 16 heads on one key head (18 parts for dk, dv)
+// 443 / 116; 256 queries on 4096 keys, 8 heads (8 for dq) 63 / 43; 1021 on 4093, 16 heads on 4 of 80 (2 for dk, dv) 132 / 122; 2 x 1000,
+// 12 heads on 3 (6 for dk, dv) 54 / 51.  Below the line, in two parts: 128 queries on 1024 keys, 4 heads (dq) 16.7 / 14.9;
+// 512 x 4 heads (dq) 14.0 / 16.1, (dk, dv) 24.6; 1024 x 8 heads (dq) 24.1 / 27.9.
 AttnScratch plan_attention_backward(AttnArgs& a, int sm_count) {
   a.parts_dq = a.parts_dkv = 1;
-  a.ds_tiles = 0;
-  AttnScratch need = {0, 0, 0, 0, 0};
+  AttnScratch need = {0, 0, 0, 0};
   if (a.cu_q != nullptr) {
     need.order_q = max_tiles(a.Sq, a.nseq, 128);
     need.order_k = max_tiles(a.Sk, a.nseq, 128);
@@ -1325,19 +1037,13 @@ AttnScratch plan_attention_backward(AttnArgs& a, int sm_count) {
   }
   if (a.Sq <= 0 || a.Sk <= 0 || a.B <= 0) return need;
   const int64_t q_tiles = ((int64_t)a.Sq + 127) / 128, k_tiles = ((int64_t)a.Sk + 127) / 128;
-  const int64_t all = ds_before(a, k_tiles), bytes = all * a.B * a.H * 32768;
-  const bool keep = bytes <= kKeepBytes;
-  if (keep) {
-    a.ds_tiles = all;
-    need.ds = bytes / 2;
-  }
-  const int64_t dq = (keep ? (q_tiles + 1) / 2 : q_tiles) * a.H * a.B, dkv = k_tiles * a.Hk * a.B, steps = q_tiles * (a.H / a.Hk);
-  auto parts = [](int64_t room, int64_t most) {
-    const int64_t p = room < most ? room : most;
-    return (int)(p > 1 ? p : 1);
+  const int64_t dq = q_tiles * a.H * a.B, dkv = k_tiles * a.Hk * a.B, steps = q_tiles * (a.H / a.Hk);
+  auto parts = [](int64_t room, int64_t steps) {
+    const int64_t p = room < steps / 4 ? room : steps / 4;
+    return steps >= 16 && p > 1 ? (int)p : 1;
   };
-  if (dq < sm_count) a.parts_dq = parts(sm_count / dq, k_tiles / 2);
-  if (dkv < sm_count) a.parts_dkv = parts((a.H > a.Hk ? 2 : 1) * sm_count / dkv, steps / 4);
+  if (dq < sm_count) a.parts_dq = parts(sm_count / dq, k_tiles);
+  if (dkv < sm_count) a.parts_dkv = parts((a.H > a.Hk ? 2 : 1) * sm_count / dkv, steps);
   const int64_t dq_floats = a.parts_dq > 1 ? (int64_t)a.parts_dq * a.B * a.H * a.Sq * a.D : 0;
   const int64_t dkv_floats = a.parts_dkv > 1 ? (int64_t)2 * a.parts_dkv * a.B * a.Hk * a.Sk * a.D : 0;
   need.partial = dq_floats > dkv_floats ? dq_floats : dkv_floats;

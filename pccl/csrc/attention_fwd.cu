@@ -11,13 +11,14 @@
 // the order of issue, so S0(j+1) may be written over P0(j), and a finished S0(j+1) says that O0 holds the sum up to j.
 // P is handed over in two halves, so that its product begins while the other half is still in its exponentials.
 //
-// What bounds it.  With the softmax left out, the products alone run at 1373 TFLOP/s on 16 heads of 16384 causal (0.84 of the
-// measured rate: both operands of Q K^T come from shared memory, 128 bytes per cycle for 128 x 128 tiles); with it 1171.  The exponentials
-// are not the limit: without them the same call takes as long, and moving a quarter of them to the multiply-add units as a
-// polynomial made it slower (939 -> 997 us).  The chain product - maximum - exponentials - product is.
-// Shorter sequences pay for the start and the end of each tile: 4 x 2048 x 16 heads of 128 causal 86.6 us (794 TFLOP/s), 70 without
-// softmax.  The grid's tiles are taken over at run time (attention.cuh), so that the loads of the next tile overlap the end of
-// the last: 97.8 -> 87.1 us there; one CTA per tile and two passes over the scores in tensor memory: 105.
+// What bounds it.  16 heads of 16384 causal take 870 us, 1265 TFLOP/s; with the softmax left out the products alone take 735
+// (1495 TFLOP/s, 0.91 of the measured rate: both operands of Q K^T come from shared memory, 128 bytes per cycle for 128 x 128 tiles).
+// The exponentials are not the limit: without them the same call takes as long, and moving a quarter of them to the
+// multiply-add units as a polynomial made it slower (928 us).  The chain product - maximum - exponentials - product is, and
+// the clock, which the power limit takes down to 1.69 GHz.
+// Shorter sequences pay for the start and the end of each tile: 4 x 2048 x 16 heads of 128 causal 82 us (838 TFLOP/s), 63
+// without softmax; heads of 64 69 us.  The grid's tiles are taken over at run time (attention.cuh), so that the loads of the next
+// tile overlap the end of the last: one CTA per tile took a seventh longer, two passes over the scores in tensor memory a quarter.
 //
 // The running maximum only follows the true one when it has fallen behind by a factor of 2^8: sums and products are then at
 // most 2^8 times larger than with the true maximum, far inside fp32 and inside the range of 16-bit probabilities, and O, which
@@ -540,17 +541,20 @@ cudaError_t launch_type(const AttnArgs& a, cudaStream_t stream) {
 
 }  // namespace
 
-// A tile's keys are split where the tiles alone leave SMs without work: into as many parts as the device has room for, of two
-// key tiles or more.
+// A tile's keys are split where the tiles alone leave SMs without work, into as many parts as the device has room for, of four
+// key tiles or more; the join takes another launch.  Measured, whole / split (us): 1021 queries on 4093 keys, 16 heads of 80
+// (2 parts) 60 / 45; 256 on 4096, 8 heads (8 parts) 61 / 24, in 16 parts 27; 128 on 1024, 4 heads (2 parts) 15.2 / 13.9, in 8 parts
+// 11.6.  Causal calls, whose tiles are of different lengths, gain little or nothing near the line: 1024 x 8 heads (2 parts)
+// 20.4 / 21.9; below it, in parts of two tiles, 512 x 4 heads 11.6 / 12.9.
 AttnScratch plan_attention_forward(AttnArgs& a, int sm_count) {
   a.parts_o = 1;
   const int64_t tiles = ((int64_t)a.Sq + 255) / 256 * a.H * a.B, key_tiles = ((int64_t)a.Sk + 127) / 128;
   if (a.cu_q == nullptr && tiles > 0 && tiles < sm_count) {
-    const int64_t room = sm_count / tiles, most = key_tiles / 2;
+    const int64_t room = sm_count / tiles, most = key_tiles / 4;
     a.parts_o = (int)(room < most ? room : most);
     if (a.parts_o < 1) a.parts_o = 1;
   }
-  AttnScratch need = {0, 0, 0, 0, 0};
+  AttnScratch need = {0, 0, 0, 0};
   if (a.cu_q != nullptr) need.order_q = max_tiles(a.Sq, a.nseq, 256);
   if (a.parts_o > 1) {
     need.partial_lse = (int64_t)a.parts_o * a.B * a.H * a.Sq;

@@ -3,8 +3,12 @@
 // A row of one head is held by a group of 8, 16 or 32 lanes.  A lane holds four pairs: columns 4l and half + 4l on (two loads
 // of 8 bytes), or 8l on where the pairs are neighbours; lanes behind the rotated columns hold eight of the others.  So the
 // rotation stays within a lane, and the sum over the row takes the only exchanges.  A group takes several heads of the same row
-// one after the other, because they share the angles, with the loads of a few heads in flight.  One read and one write of the
-// data; bound by HBM.
+// one after the other, because they share the angles, with the loads of a few heads in flight.  One read and one write of the data.
+//
+// What bounds it.  8192 rows of 16 + 16 heads of 128, bf16: forward 26.9 us (5.0 TB/s: 0.76 of the measured copy rate), backward
+// 48.1 (4.2 TB/s); 32 + 32 heads 48.3 (5.6 TB/s) and 85.2 (4.7 TB/s).  A call of this length is never far from its start and its end;
+// behind that are the instructions: the issue slots are two thirds full in the forward pass, which is why the arithmetic is on
+// pairs of 32-bit numbers.
 //
 // The backward pass computes the norms again (its x is read for the gradient anyway).  A group sums its share of a weight's
 // gradient in registers over all its rows, a block (of queries, or of keys) adds up its groups in order, and a second small
@@ -398,8 +402,8 @@ int rotary_blocks(RotaryArgs& a, bool backward, int sm_count) {
   const int lanes = lanes_of(a.D), groups = (backward ? kBackward : kForward) / lanes;
   const int64_t rows = (int64_t)a.B * a.S;
   // Heads per item: as many of a row as possible share its angles, but every SM wants eight blocks (forward: one item per group), or
-  // two blocks that walk over six items or more (backward).  8192 rows of 16 + 16 heads of 128, backward: 16 heads 55.2 us, 8 heads 51.8;
-  // of 32 + 32: 91.5 and 94.6.  Forward: 16 heads 28.0 and 50.0, 8 heads 28.9 and 51.7.
+  // two blocks that walk over six items or more (backward).  8192 rows of 16 + 16 heads of 128, 16 / 8 / 4 heads per item: backward
+  // 51.1 / 48.0 / 51.6 us, forward 26.9 / 27.7 / 29.8; of 32 + 32 heads 85.2 / 88.4 / 95.2 and 48.3 / 49.6 / 54.6.
   const int64_t most = backward ? (int64_t)sm_count * 2 : INT32_MAX, want = (int64_t)sm_count * groups * (backward ? 12 : 8);
   int hpi = 16;
   for (;; hpi /= 2) {

@@ -309,6 +309,8 @@ def positions_of(cfg: GPTConfig, batch: int, seq: int, device, tables=None, cu_s
 
         tables = rotary_table(cfg.seq_len, cfg.head_dim, cfg.rope_theta, device)
     pos = Positions(*tables)
+    if cu_seqlens is None and seq > pos.cos.shape[0]:
+        raise ValueError(f"sequences of {seq} tokens have positions that the table of {pos.cos.shape[0]} does not hold")
     if cu_seqlens is not None:
         # tokens behind the last document count on from its end, within the table
         t = torch.arange(batch * seq, dtype=torch.int32, device=device)

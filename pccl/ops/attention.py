@@ -21,8 +21,7 @@ last key.  A query that sees no key has an output of 0, an ``lse`` of -inf, and 
 These are plain functions like those of ``pccl.ops.gemm``: they record nothing for autograd.  Results are the same bits from
 call to call (no atomic additions).  Outputs must not overlap inputs or each other.  Probabilities and score gradients are rounded
 to the inputs' type for the products that they enter: with fp16 a score gradient above 65504 becomes infinite, as it does in
-``dout``.  The backward pass of a batch (not of packed sequences) keeps its score gradients in up to 1 GiB of memory while it
-runs, and computes them twice where they would take more.
+``dout``.
 """
 from __future__ import annotations
 

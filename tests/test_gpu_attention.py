@@ -331,8 +331,7 @@ print("fine")
     assert r.returncode == 0 and "fine" in r.stdout, r.stderr[-2000:]
 
 
-def test_score_gradients_kept_or_computed_twice():
-    """Two heads of 2049 rows keep their score gradients in memory, three hundred (1.4 GiB) compute them twice."""
+def test_many_batch_entries_give_the_same_bits():
     from pccl.ops.attention import attention_backward
 
     q, k, v, dout = _inputs(1, 2049, 2049, 2, 2, 64, BF, 30)
@@ -343,6 +342,41 @@ def test_score_gradients_kept_or_computed_twice():
         for x, (w, t), what in zip(got, want, ("dq", "dk", "dv")):
             _close(x[0], w, t, what)
             assert torch.equal(x[0], x[n - 1])
+
+
+@pytest.mark.parametrize("case", [(37, 37, 4, 2, 64, True, BF), (20, 150, 2, 2, 80, True, FP), (140, 30, 3, 1, 128, False, BF), (90, 33, 2, 1, 64, True, BF)], ids=str)
+def test_gradient_against_differences(case):
+    """The sum of out * dout, moved along a direction, against the gradients.  The formula in 64 bits is differenced; the kernel's
+    gradient may be off by its roundings, the formula's by what the rounded output makes of the row sums."""
+    from pccl.ops.attention import attention_backward
+
+    Sq, Sk, H, Hk, D, causal, dtype = case
+    q, k, v, dout = _inputs(1, Sq, Sk, H, Hk, D, dtype, 40)
+    scale, see = D ** -0.5, _visible(Sq, Sk, causal)
+    out, lse = _given(q, k, v, causal, scale)
+    got = attention_backward(dout, q, k, v, out, lse, causal=causal)
+    G, up = H // Hk, lambda x: x[0].double().transpose(0, 1)                     # noqa: E731
+
+    def f(q, k, v):
+        s = ((q @ k.repeat_interleave(G, 0).transpose(1, 2)) * scale).masked_fill(~see, -math.inf)
+        return (s.softmax(-1).nan_to_num(0.0) @ v.repeat_interleave(G, 0))        # a query that sees nothing has an output of zero
+
+    x, d = [up(q), up(k), up(v)], up(dout)
+    exact = f(*x).transpose(0, 1)
+    near = _oracle(q[0], k[0], v[0], see, scale, dout[0], out[0], lse[0])
+    true = _oracle(q[0], k[0], v[0], see, scale, dout[0], exact, _oracle(q[0], k[0], v[0], see, scale)[2])
+    gen = torch.Generator(device=DEV).manual_seed(41)
+    for i, what in enumerate(("dq", "dk", "dv")):
+        e = torch.randn(x[i].shape, dtype=torch.float64, device=DEV, generator=gen)
+        h = 1e-5
+        move = lambda t: [t * e + y if j == i else y for j, y in enumerate(x)]    # noqa: E731,B023
+        want = float(((f(*move(h)) - f(*move(-h))) * d).sum() / (2 * h))
+        along = lambda g: float((g.double().transpose(0, 1) * e).sum())           # noqa: E731,B023
+        # central differences: h^2 times a third derivative, 2^-53 / h times the sum's size
+        step = 1e-6 * (1 + float((f(*x).abs() * d.abs()).sum()))
+        assert abs(along(true[i][0]) - want) <= step, f"{what}: the formula"
+        off = float((near[i][1].transpose(0, 1) * e.abs()).sum()) + abs(along(near[i][0]) - along(true[i][0]))
+        assert abs(along(got[i][0]) - want) <= off + step, what
 
 
 def test_empty_calls():
