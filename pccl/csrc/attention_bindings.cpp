@@ -1,5 +1,4 @@
 // Python bindings of attention.
-#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
@@ -12,6 +11,7 @@
 
 #include "attention.h"
 #include "comm.h"
+#include "overlap.h"
 
 namespace py = pybind11;
 using namespace pccl;
@@ -123,10 +123,8 @@ Shape fill(AttnArgs& a, const at::Tensor& q, const at::Tensor& k, const at::Tens
 // An output: the caller's tensor, or a new one.
 at::Tensor output(const std::optional<at::Tensor>& given, const at::Tensor& like, const char* name, std::initializer_list<at::Tensor> inputs) {
   if (!given.has_value()) return at::empty(like.sizes(), like.options());
-  at::assert_no_internal_overlap(*given);
-  for (const at::Tensor& t : inputs)
-    TORCH_CHECK(at::get_overlap_status(*given, t) != at::MemOverlapStatus::Full && at::get_overlap_status(*given, t) != at::MemOverlapStatus::Partial,
-                name, " must not overlap an input");
+  TORCH_CHECK(distinct(*given), name, " must not overlap itself");
+  for (const at::Tensor& t : inputs) TORCH_CHECK(share(*given, t) == Share::kNone, name, " must not overlap an input");
   return *given;
 }
 
@@ -173,13 +171,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_backward(const at::Tens
                   lse.dim() == (s.packed ? 2 : 3) && lse.size(-1) == s.Sq && lse.size(-2) == s.H && (s.packed || lse.size(0) == s.B),
               "lse must be what the forward pass returned");
   TORCH_CHECK(dq_.has_value() == dk_.has_value() && dq_.has_value() == dv_.has_value(), "dq, dk and dv are given together or not at all");
-  const std::initializer_list<at::Tensor> inputs = {dout, q, k, v, out};
+  const std::initializer_list<at::Tensor> inputs = {dout, q, k, v, out, lse};
   at::Tensor dq = output(dq_, q, "dq", inputs), dk = output(dk_, k, "dk", inputs), dv = output(dv_, v, "dv", inputs);
-  auto apart = [](const at::Tensor& x, const at::Tensor& y) {
-    const auto o = at::get_overlap_status(x, y);
-    return o != at::MemOverlapStatus::Full && o != at::MemOverlapStatus::Partial;
-  };
-  TORCH_CHECK(apart(dq, dk) && apart(dq, dv) && apart(dk, dv), "dq, dk and dv must not overlap each other");
+  TORCH_CHECK(share(dq, dk) == Share::kNone && share(dq, dv) == Share::kNone && share(dk, dv) == Share::kNone,
+              "dq, dk and dv must not overlap each other");
   TORCH_CHECK(s.B <= 65535, "the backward pass takes up to 65535 batch entries");
   a.dq = view(dq, "dq", q, s.B, s.Sq, s.H, s.D);
   a.dk = view(dk, "dk", q, s.B, s.Sk, s.Hk, s.D);

@@ -1,5 +1,4 @@
 // Python bindings of the query/key norms with rotation.
-#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
@@ -10,6 +9,7 @@
 #include <tuple>
 
 #include "comm.h"
+#include "overlap.h"
 #include "rotary.h"
 
 namespace py = pybind11;
@@ -39,12 +39,14 @@ RotaryTensor view(const at::Tensor& t, const char* name, const at::Tensor& q, co
   return v;
 }
 
-// An output: the caller's tensor, which may be exactly one of the inputs (a row is read before it is written), or a new one.
-at::Tensor output(const std::optional<at::Tensor>& given, const at::Tensor& like, const char* name, std::initializer_list<at::Tensor> inputs) {
+// An output: the caller's tensor, which may be exactly one of its own inputs (a row is read before it is written) but shares nothing
+// with those of the other heads, or a new one.
+at::Tensor output(const std::optional<at::Tensor>& given, const at::Tensor& like, const char* name, std::initializer_list<at::Tensor> own,
+                  std::initializer_list<at::Tensor> others) {
   if (!given.has_value()) return at::empty(like.sizes(), like.options());
-  at::assert_no_internal_overlap(*given);
-  for (const at::Tensor& t : inputs)
-    TORCH_CHECK(at::get_overlap_status(*given, t) != at::MemOverlapStatus::Partial, name, " must not partly overlap an input");
+  TORCH_CHECK(distinct(*given), name, " must not overlap itself");
+  for (const at::Tensor& t : own) TORCH_CHECK(share(*given, t) != Share::kSome, name, " must not partly overlap an input");
+  for (const at::Tensor& t : others) TORCH_CHECK(share(*given, t) == Share::kNone, name, " must not overlap an input of the other heads");
   return *given;
 }
 
@@ -109,7 +111,8 @@ std::tuple<at::Tensor, at::Tensor> qk_norm_rope_forward(const at::Tensor& q, con
   RotaryArgs a;
   const Shape s = fill(a, q, k, qw, kw, cos, sin, positions, eps, interleaved);
   c10::cuda::CUDAGuard guard(q.device());
-  at::Tensor qo = output(q_out, q, "q_out", {q}), ko = output(k_out, k, "k_out", {k});
+  at::Tensor qo = output(q_out, q, "q_out", {q}, {k}), ko = output(k_out, k, "k_out", {k}, {q});
+  TORCH_CHECK(share(qo, ko) == Share::kNone, "q_out and k_out must not overlap");
   a.y[0] = view(qo, "q_out", q, s, a.H[0]);
   a.y[1] = view(ko, "k_out", q, s, a.H[1]);
   if (s.B * s.S == 0 || a.H[0] + a.H[1] == 0) return {qo, ko};
@@ -127,7 +130,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> qk_norm_rope_backward
   c10::cuda::CUDAGuard guard(q.device());
   a.dy[0] = view(dq, "dq", q, s, a.H[0]);
   a.dy[1] = view(dk, "dk", q, s, a.H[1]);
-  at::Tensor qo = output(dq_in, q, "dq_in", {dq, q}), ko = output(dk_in, k, "dk_in", {dk, k});
+  at::Tensor qo = output(dq_in, q, "dq_in", {dq, q}, {dk, k}), ko = output(dk_in, k, "dk_in", {dk, k}, {dq, q});
+  TORCH_CHECK(share(qo, ko) == Share::kNone, "dq_in and dk_in must not overlap");
   a.y[0] = view(qo, "dq_in", q, s, a.H[0]);
   a.y[1] = view(ko, "dk_in", q, s, a.H[1]);
   at::Tensor dqw = dqw_.has_value() ? *dqw_ : at::empty_like(qw), dkw = dkw_.has_value() ? *dkw_ : at::empty_like(kw);
@@ -135,7 +139,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> qk_norm_rope_backward
     TORCH_CHECK(w->is_cuda() && w->device() == q.device() && w->is_contiguous() && w->dim() == 1 && w->numel() == s.D &&
                     w->scalar_type() == qw.scalar_type(),
                 "dq_weight and dk_weight must look like the weights");
-  TORCH_CHECK(at::get_overlap_status(dqw, dkw) == at::MemOverlapStatus::No, "dq_weight and dk_weight must not overlap");
+  TORCH_CHECK(share(dqw, dkw) == Share::kNone, "dq_weight and dk_weight must not overlap");
   a.dw[0] = dqw.data_ptr();
   a.dw[1] = dkw.data_ptr();
   if (s.B * s.S == 0 || a.H[0] + a.H[1] == 0) {

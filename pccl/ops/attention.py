@@ -19,9 +19,9 @@ Masks.  ``causal``: query i sees the keys up to ``i + (key rows - query rows)`` 
 last key.  A query that sees no key has an output of 0, an ``lse`` of -inf, and adds nothing to any gradient.
 
 These are plain functions like those of ``pccl.ops.gemm``: they record nothing for autograd.  Results are the same bits from
-call to call (no atomic additions).  Outputs must not overlap inputs or each other.  Probabilities and score gradients are rounded
-to the inputs' type for the products that they enter: with fp16 a score gradient above 65504 becomes infinite, as it does in
-``dout``.
+call to call (no atomic additions).  Outputs must not overlap inputs or each other (views that lie in each other's range are
+told apart where their strides are equal).  ``scale`` is positive.  Probabilities and score gradients are rounded to the
+inputs' type for the products that they enter: with fp16 a score gradient above 65504 becomes infinite, as it does in ``dout``.
 """
 from __future__ import annotations
 

@@ -457,3 +457,28 @@ def test_refusals():
         with pytest.raises(RuntimeError):
             call()
             pytest.fail(f"call {i} was taken")
+
+
+def test_outputs_between_the_inputs():
+    """Views into one packed tensor: refused where an output touches an input, taken where it lies beside them."""
+    from pccl.ops.attention import attention_backward, attention_forward
+
+    x = torch.randn(2, 40, 8, 64, device=DEV).to(BF)                              # q 0-3, k 4, v 5, room 6 and 7
+    q, k, v = x[:, :, :4], x[:, :, 4:5], x[:, :, 5:6]
+    kept = x.clone()
+    for h in (0, 1, 2, 3, 4):
+        with pytest.raises(RuntimeError, match="overlap"):
+            attention_forward(q, k, v, out=x[:, :, h:h + 4])
+    with pytest.raises(RuntimeError, match="overlap"):
+        attention_forward(q, k, v, out=x.view(-1)[:2 * 40 * 256].view(2, 40, 4, 64))
+    with pytest.raises(RuntimeError, match="overlap"):
+        attention_forward(q[:1], k[:1], v[:1], out=torch.as_strided(torch.zeros(1 << 14, device=DEV, dtype=BF), (1, 40, 4, 64), (0, 256, 8, 1)))
+    out, lse = attention_forward(x[:, :, :2], k, v)
+    o = x[:, :, 6:8]
+    assert torch.equal(attention_forward(x[:, :, :2], k, v, out=o)[0], out) and torch.equal(x[:, :, :6], kept[:, :, :6])
+    g = torch.zeros(2, 40, 4, 64, device=DEV, dtype=BF)
+    want = attention_backward(out, x[:, :, :2], k, v, out, lse)
+    got = attention_backward(out, x[:, :, :2], k, v, out, lse, dq=g[:, :, :2], dk=g[:, :, 2:3], dv=g[:, :, 3:])
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with pytest.raises(RuntimeError, match="overlap"):
+        attention_backward(out, x[:, :, :2], k, v, out, lse, dq=g[:, :, :2], dk=g[:, :, 1:2], dv=g[:, :, 3:])

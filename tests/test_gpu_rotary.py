@@ -210,3 +210,20 @@ def test_refusals():
         with pytest.raises(RuntimeError):
             call()
             pytest.fail(f"call {i} was taken")
+
+
+def test_outputs_between_the_inputs():
+    from pccl.ops.rotary import qk_norm_rope_backward, qk_norm_rope_forward, rotary_table
+
+    x = torch.randn(2, 20, 6, 64, device=DEV).to(BF)                              # q 0-1, k 2, room 3 to 5
+    q, k = x[:, :, :2], x[:, :, 2:3]
+    w = torch.ones(64, device=DEV, dtype=BF)
+    tab = rotary_table(20, 64, device=DEV)
+    want = qk_norm_rope_forward(q, k, w, w, *tab)
+    for bad in (dict(q_out=x[:, :, 1:3]), dict(q_out=x[:, :, 2:4]), dict(k_out=x[:, :, 1:2]), dict(q_out=x[:, :, 3:5], k_out=x[:, :, 4:5])):
+        with pytest.raises(RuntimeError, match="overlap"):
+            qk_norm_rope_forward(q, k, w, w, *tab, **bad)
+    with pytest.raises(RuntimeError, match="overlap"):
+        qk_norm_rope_backward(*want, q, k, w, w, *tab, dq_in=x[:, :, 1:3])
+    got = qk_norm_rope_forward(q, k, w, w, *tab, q_out=x[:, :, 3:5], k_out=x[:, :, 2:3])
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
