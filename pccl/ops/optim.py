@@ -15,12 +15,12 @@ from typing import List, Optional, Sequence, Tuple, Union
 
 import torch
 
+from .. import build_kernels        # an import inside _C() would cost every call 0.6 us, of 7 for a small one
+
 BLOCK = 256
 
 
 def _C():
-    from .. import build_kernels
-
     return build_kernels.load()
 
 
