@@ -8,9 +8,10 @@
 // its own table.  Streaming: 28 bytes per parameter with states in 32 bits and a 16-bit gradient and parameter beside the 32-bit
 // copy, 16 bytes with states in 8 bits.
 //
-// What bounds it.  308 million parameters: with states in 32 bits 1377 us, 6.26 TB/s (0.95 of the measured copy rate); tensors off
-// vector boundaries 1497.  In 8 bits 999 us, 4.93 TB/s: the codes cost 85 instructions for each element, and the issue slots are three
-// quarters full; misaligned 1658.  Reading the states back (adamw_dequantize) 458 us, 6.72 TB/s.
+// What bounds it.  308 million parameters: with states in 32 bits 1382 us, 6.24 TB/s (0.95 of the measured copy rate); tensors off
+// vector boundaries 1402.  With three blocks on an SM, more loads on their way, 1404; with four 1590.  In 8 bits 955 us, 5.16 TB/s: the
+// codes cost about 80 instructions for each element, and the issue slots are three quarters full; misaligned 1277.  Reading the
+// states back (adamw_dequantize) 458 us, 6.72 TB/s.
 //
 // 8-bit states.  A block keeps the size A of its largest value in 32 bits and a code c per element:
 //   m = sign * A (c / 127)^2,  v = A (c / 255)^4
@@ -99,11 +100,17 @@ __device__ __forceinline__ void load8(const void* base, int64_t i, Raw8& r) {
   if constexpr (TYPE == kAdamF32) load32(static_cast<const float*>(base) + i, r);
   else r.a = __ldcs(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + i));
 }
+// One element as it lies in memory, and its value.
 template <int TYPE>
-__device__ __forceinline__ float load1(const void* base, int64_t i) {
-  if constexpr (TYPE == kAdamF32) return static_cast<const float*>(base)[i];
-  else if constexpr (TYPE == kAdamBf16) return __bfloat162float(static_cast<const __nv_bfloat16*>(base)[i]);
-  else return __half2float(static_cast<const __half*>(base)[i]);
+__device__ __forceinline__ uint32_t load_bits(const void* base, int64_t i) {
+  if constexpr (TYPE == kAdamF32) return static_cast<const uint32_t*>(base)[i];
+  else return static_cast<const uint16_t*>(base)[i];
+}
+template <int TYPE>
+__device__ __forceinline__ float from_bits(uint32_t w) {
+  if constexpr (TYPE == kAdamF32) return __uint_as_float(w);
+  else if constexpr (TYPE == kAdamBf16) return __uint_as_float(w << 16);
+  else return __half2float(__ushort_as_half((unsigned short)w));
 }
 template <int TYPE>
 __device__ __forceinline__ uint32_t narrow2(float a, float b) {
@@ -252,6 +259,19 @@ template <int PT>
 __device__ __forceinline__ void* weights_of(const AdamTensor& t) {
   return PT == kAdamF32 ? t.param : static_cast<void*>(t.master);
 }
+// Off vector boundaries, or at a tensor's end: neighbouring lanes read neighbouring elements.
+template <int PT, int GT, bool BITS8>
+__device__ __forceinline__ void fetch_ragged(const AdamTensor& t, Block<BITS8>& x) {
+  uint32_t g[8], p[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int64_t e = x.at - (threadIdx.x & 31) * 7 + i * 32;
+    g[i] = e < t.n ? load_bits<GT>(t.grad, e) : 0u;
+    p[i] = e < t.n ? static_cast<const uint32_t*>(weights_of<PT>(t))[e] : 0u;
+  }
+  x.g = {make_uint4(g[0], g[1], g[2], g[3]), make_uint4(g[4], g[5], g[6], g[7])};
+  x.p = {make_uint4(p[0], p[1], p[2], p[3]), make_uint4(p[4], p[5], p[6], p[7])};
+}
 template <int PT, int GT, bool BITS8, int MAX>
 __device__ __forceinline__ void fetch(const AdamMultiArgs& a, const Table<MAX>& table, uint32_t blk, int k, Block<BITS8>& x) {
   // the last tensor that starts at or before this block: mostly the last block's, else one behind it
@@ -275,6 +295,8 @@ __device__ __forceinline__ void fetch(const AdamMultiArgs& a, const Table<MAX>& 
   if (x.whole) {
     load8<GT>(t.grad, x.at, x.g);
     load8<kAdamF32>(weights, x.at, x.p);
+  } else {
+    fetch_ragged<PT, GT>(t, x);
   }
   if constexpr (BITS8) {                                       // the state's blocks are whole: behind a tensor's end they hold zeros
     const uint64_t si = x.sblk * kAdamBlock + (uint64_t)lane * 8;
@@ -285,17 +307,22 @@ __device__ __forceinline__ void fetch(const AdamMultiArgs& a, const Table<MAX>& 
   }
 }
 
-// A warp's 256 numbers, written by neighbouring lanes in turn: eight neighbours of each lane.
-__device__ __forceinline__ void exchange(const float* s, float* x) {
+// A warp's 256 numbers: from those of neighbouring lanes in turn, one to a word, to eight neighbours of each lane.
+template <int TYPE>
+__device__ __forceinline__ void exchange(float* s, const Raw8& r, float* x) {
+  const int lane = threadIdx.x & 31;
+  const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s[i * 32 + lane] = from_bits<TYPE>(w[i]);
   __syncwarp();
-  const float4 a = reinterpret_cast<const float4*>(s)[(threadIdx.x & 31) * 2], b = reinterpret_cast<const float4*>(s)[(threadIdx.x & 31) * 2 + 1];
+  const float4 a = reinterpret_cast<const float4*>(s)[lane * 2], b = reinterpret_cast<const float4*>(s)[lane * 2 + 1];
   x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
   x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
   __syncwarp();
 }
 
 template <int PT, int GT, bool BITS8, int MAX>
-__global__ void __launch_bounds__(kThreads, BITS8 ? 4 : 3) adamw_multi_kernel(const __grid_constant__ AdamMultiArgs a,
+__global__ void __launch_bounds__(kThreads, BITS8 ? 4 : 2) adamw_multi_kernel(const __grid_constant__ AdamMultiArgs a,
                                                                               const __grid_constant__ Table<MAX> table) {
   __shared__ __align__(16) float stage[kThreads / 32][kAdamBlock];
   pdl_wait();
@@ -320,7 +347,11 @@ __global__ void __launch_bounds__(kThreads, BITS8 ? 4 : 3) adamw_multi_kernel(co
     const bool whole = x.whole;
     float g[8], p[8];
     F2 m[4], v[4];                                             // pairs of neighbours
-    if constexpr (BITS8) {
+    Raw8 rm, rv;
+    if constexpr (!BITS8) {
+      load8<kAdamF32>(a.m, (int64_t)si, rm);
+      load8<kAdamF32>(a.v, (int64_t)si, rv);
+    } else {
       decode8<true>(x.cm, __fmul_rn(x.m_scale, kSignedUnit), m);
       decode8<false>(x.cv, __fmul_rn(x.v_scale, kUnsignedUnit), v);
     }
@@ -328,26 +359,10 @@ __global__ void __launch_bounds__(kThreads, BITS8 ? 4 : 3) adamw_multi_kernel(co
       widen<GT>(x.g, g);
       widen<kAdamF32>(x.p, p);
     } else {
-      // off vector boundaries, or a tensor's end: neighbouring lanes read neighbouring elements, and change them for eight in a row
-      const int64_t first = at - lane * 8;
-      float* s = stage[threadIdx.x >> 5];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int64_t e = first + i * 32 + lane;
-        s[i * 32 + lane] = e < t.n ? load1<GT>(t.grad, e) : 0.f;
-      }
-      exchange(s, g);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int64_t e = first + i * 32 + lane;
-        s[i * 32 + lane] = e < t.n ? static_cast<const float*>(weights)[e] : 0.f;
-      }
-      exchange(s, p);
+      exchange<GT>(stage[threadIdx.x >> 5], x.g, g);           // for eight in a row
+      exchange<kAdamF32>(stage[threadIdx.x >> 5], x.p, p);
     }
     if constexpr (!BITS8) {
-      Raw8 rm, rv;
-      load8<kAdamF32>(a.m, (int64_t)si, rm);
-      load8<kAdamF32>(a.v, (int64_t)si, rv);
       float y[8], z[8];
       widen<kAdamF32>(rm, y);
       widen<kAdamF32>(rv, z);
@@ -468,7 +483,7 @@ cudaError_t launch(const AdamMultiArgs& a, const AdamTensor* tensors, int count,
   Table<MAX> table;
   memcpy(table.t, tensors, sizeof(AdamTensor) * (size_t)count);
   table.count = count;
-  const uint32_t need = (a.blocks + kThreads / 32 - 1) / (kThreads / 32), most = (uint32_t)sm_count * (BITS8 ? 4 : 3);
+  const uint32_t need = (a.blocks + kThreads / 32 - 1) / (kThreads / 32), most = (uint32_t)sm_count * (BITS8 ? 4 : 2);
   return launch_pdl(adamw_multi_kernel<PT, GT, BITS8, MAX>, dim3(need < most ? need : most), dim3(kThreads), 0, s, a, table);
 }
 template <int PT, int GT>
