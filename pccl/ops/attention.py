@@ -17,6 +17,9 @@ hold 0 there (``lse``: -inf), tensors given by the caller keep what they held.
 
 Masks.  ``causal``: query i sees the keys up to ``i + (key rows - query rows)`` of its sequence, so that the last query sees the
 last key.  A query that sees no key has an output of 0, an ``lse`` of -inf, and adds nothing to any gradient.
+What is not finite in a hidden place (a value in the forward pass, any input in the backward pass) may make results of rows up
+to 127 away from it NaN, because a probability of 0 is multiplied with it, as in the formula.  Nothing passes from one packed
+sequence to another.
 
 These are plain functions like those of ``pccl.ops.gemm``: they record nothing for autograd.  Results are the same bits from
 call to call (no atomic additions).  Outputs must not overlap inputs or each other (views that lie in each other's range are
