@@ -274,3 +274,27 @@ def test_refusals():
         adamw_state([p], 16)
     adamw_step([], [], st, step=1, **HYPER)
     adamw_step([mk(0), p], [mk(0), g], st, step=1, **HYPER)                        # an empty tensor has no part in the state
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_more_than_2_31_elements(bits):
+    """The end of a long tensor, and the tensor behind it, change as they do alone (the first step reads no codes)."""
+    from pccl.ops.optim import adamw_state, adamw_step
+
+    n = (1 << 31) + 773
+    if torch.cuda.mem_get_info()[0] < 44 << 30:
+        pytest.skip("needs 44 GiB")
+    p, g = torch.zeros(n, device=DEV), torch.zeros(n, device=DEV, dtype=BF)
+    q, h = torch.randn(1000, device=DEV), torch.randn(1000, device=DEV).to(BF)
+    p[-773:].copy_(torch.randn(773, device=DEV))
+    g[-773:].copy_(torch.randn(773, device=DEV))
+    few, few_grads = [p[-773:].clone(), q.clone()], [g[-773:].clone(), h]
+    state, own = adamw_state([p, q], bits), adamw_state(few, bits)
+    adamw_step([p, q], [g, h], state, step=1, **HYPER)
+    adamw_step(few, few_grads, own, step=1, **HYPER)
+    assert torch.equal(p[-773:], few[0]) and torch.equal(q, few[1]) and float(p[:-773].abs().max()) == 0.0
+    if bits == 8:
+        assert torch.equal(state.exp_avg_scale[-8:], own.exp_avg_scale) and torch.equal(state.exp_avg_sq_scale[-8:], own.exp_avg_sq_scale)
+        assert float(state.exp_avg_scale[:-8].abs().max()) == 0.0
+    else:
+        assert torch.equal(state.exp_avg[-2048:], own.exp_avg) and torch.equal(state.exp_avg_sq[-2048:], own.exp_avg_sq)

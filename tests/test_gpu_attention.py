@@ -482,3 +482,24 @@ def test_outputs_between_the_inputs():
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     with pytest.raises(RuntimeError, match="overlap"):
         attention_backward(out, x[:, :, :2], k, v, out, lse, dq=g[:, :, :2], dk=g[:, :, 1:2], dv=g[:, :, 3:])
+
+
+def test_offsets_beyond_32_bits():
+    """Rows four million elements apart: the last one's offset is above 2^31 elements.  The same bits as from contiguous tensors."""
+    from pccl.ops.attention import attention_backward, attention_forward
+
+    S, step = 600, 1 << 22
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GiB")
+    far, grads = (torch.empty((S - 1) * step + 512, device=DEV, dtype=BF) for _ in range(2))
+    cut = lambda x, at: torch.as_strided(x, (1, S, 1, 128), (S * step, step, 128, 1), at)    # noqa: E731
+    q, k, v, dout = _inputs(1, S, S, 1, 1, 128, BF, 50)
+    views = [cut(far, 128 * i) for i in range(4)]
+    for x, y in zip(views, (q, k, v, dout)):
+        x.copy_(y)
+    out, lse = attention_forward(q, k, v)
+    got, got_lse = attention_forward(*views[:3], out=cut(grads, 384))
+    assert torch.equal(got, out) and torch.equal(got_lse, lse)
+    want = attention_backward(dout, q, k, v, out, lse)
+    near = attention_backward(views[3], *views[:3], got, lse, dq=cut(grads, 0), dk=cut(grads, 128), dv=cut(grads, 256))
+    assert all(torch.equal(a, b) for a, b in zip(near, want))

@@ -227,3 +227,23 @@ def test_outputs_between_the_inputs():
         qk_norm_rope_backward(*want, q, k, w, w, *tab, dq_in=x[:, :, 1:3])
     got = qk_norm_rope_forward(q, k, w, w, *tab, q_out=x[:, :, 3:5], k_out=x[:, :, 2:3])
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_offsets_beyond_32_bits():
+    from pccl.ops.rotary import qk_norm_rope_backward, qk_norm_rope_forward, rotary_table
+
+    S, step = 600, 1 << 22
+    if torch.cuda.mem_get_info()[0] < 12 << 30:
+        pytest.skip("needs 12 GiB")
+    far = torch.empty((S - 1) * step + 512, device=DEV, dtype=BF)
+    cut = lambda at: torch.as_strided(far, (S, 1, 128), (step, 128, 1), at)                  # noqa: E731
+    q, k, dq, dk = (torch.randn(S, 1, 128, device=DEV).to(BF) for _ in range(4))
+    w, tab = torch.rand(128, device=DEV) + 0.5, rotary_table(S, 128, device=DEV)
+    want = qk_norm_rope_forward(q, k, w, w, *tab)
+    grad = qk_norm_rope_backward(dq, dk, q, k, w, w, *tab)
+    for i, x in enumerate((q, k, dq, dk)):
+        cut(128 * i).copy_(x)
+    got = qk_norm_rope_backward(cut(256), cut(384), cut(0), cut(128), w, w, *tab, dq_in=cut(256), dk_in=cut(384))
+    assert all(torch.equal(a, b) for a, b in zip(got, grad))
+    got = qk_norm_rope_forward(cut(0), cut(128), w, w, *tab, q_out=cut(0), k_out=cut(128))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
