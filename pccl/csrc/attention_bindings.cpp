@@ -11,6 +11,7 @@
 
 #include "attention.h"
 #include "comm.h"
+#include "fresh.h"
 #include "overlap.h"
 
 namespace py = pybind11;
@@ -122,7 +123,7 @@ Shape fill(AttnArgs& a, const at::Tensor& q, const at::Tensor& k, const at::Tens
 
 // An output: the caller's tensor, or a new one.
 at::Tensor output(const std::optional<at::Tensor>& given, const at::Tensor& like, const char* name, std::initializer_list<at::Tensor> inputs) {
-  if (!given.has_value()) return at::empty(like.sizes(), like.options());
+  if (!given.has_value()) return fresh(like.sizes(), like.scalar_type(), like);
   TORCH_CHECK(distinct(*given), name, " must not overlap itself");
   for (const at::Tensor& t : inputs) TORCH_CHECK(share(*given, t) == Share::kNone, name, " must not overlap an input");
   return *given;
@@ -136,19 +137,18 @@ std::tuple<at::Tensor, at::Tensor> attention_forward(const at::Tensor& q, const 
   c10::cuda::CUDAGuard guard(q.device());
   at::Tensor out = output(out_, q, "out", {q, k, v});
   a.o = view(out, "out", q, s.B, s.Sq, s.H, s.D);
-  const auto f32 = q.options().dtype(at::kFloat);
-  at::Tensor lse = s.packed ? at::empty({s.H, s.Sq}, f32) : at::empty({s.B, s.H, s.Sq}, f32);
+  at::Tensor lse = s.packed ? fresh({s.H, s.Sq}, at::kFloat, q) : fresh({s.B, s.H, s.Sq}, at::kFloat, q);
   a.lse = lse.data_ptr<float>();
   a.zero_tail = !out_.has_value();
   const AttnScratch need = plan_attention_forward(a, at::cuda::getCurrentDeviceProperties()->multiProcessorCount);
   at::Tensor partial, partial_lse, order;
   if (need.order_q > 0) {
-    order = at::empty({2 * need.order_q}, q.options().dtype(at::kInt));
+    order = fresh({2 * need.order_q}, at::kInt, q);
     a.order_q = reinterpret_cast<int2*>(order.data_ptr<int>());
   }
   if (need.partial > 0) {
-    partial = at::empty({need.partial}, f32);
-    partial_lse = at::empty({need.partial_lse}, f32);
+    partial = fresh({need.partial}, at::kFloat, q);
+    partial_lse = fresh({need.partial_lse}, at::kFloat, q);
     a.partial = partial.data_ptr<float>();
     a.partial_lse = partial_lse.data_ptr<float>();
   }
@@ -180,18 +180,18 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_backward(const at::Tens
   a.dk = view(dk, "dk", q, s.B, s.Sk, s.Hk, s.D);
   a.dv = view(dv, "dv", q, s.B, s.Sk, s.Hk, s.D);
   a.lse = lse.data_ptr<float>();
-  at::Tensor delta = at::empty_like(lse);
+  at::Tensor delta = fresh(lse.sizes(), at::kFloat, q);
   a.delta = delta.data_ptr<float>();
   a.zero_tail = !dq_.has_value();
   const AttnScratch need = plan_attention_backward(a, at::cuda::getCurrentDeviceProperties()->multiProcessorCount);
   at::Tensor partial, order;
   if (need.order_q > 0) {
-    order = at::empty({2 * (need.order_q + need.order_k)}, q.options().dtype(at::kInt));
+    order = fresh({2 * (need.order_q + need.order_k)}, at::kInt, q);
     a.order_q = reinterpret_cast<int2*>(order.data_ptr<int>());
     a.order_k = a.order_q + need.order_q;
   }
   if (need.partial > 0) {
-    partial = at::empty({need.partial}, lse.options());
+    partial = fresh({need.partial}, at::kFloat, q);
     a.partial = partial.data_ptr<float>();
   }
   PCCL_CUDA(launch_attention_backward(a, at::cuda::getCurrentCUDAStream().stream()));

@@ -9,6 +9,7 @@
 #include <tuple>
 
 #include "comm.h"
+#include "fresh.h"
 #include "overlap.h"
 #include "rotary.h"
 
@@ -43,7 +44,7 @@ RotaryTensor view(const at::Tensor& t, const char* name, const at::Tensor& q, co
 // with those of the other heads, or a new one.
 at::Tensor output(const std::optional<at::Tensor>& given, const at::Tensor& like, const char* name, std::initializer_list<at::Tensor> own,
                   std::initializer_list<at::Tensor> others) {
-  if (!given.has_value()) return at::empty(like.sizes(), like.options());
+  if (!given.has_value()) return fresh(like.sizes(), like.scalar_type(), like);
   TORCH_CHECK(distinct(*given), name, " must not overlap itself");
   for (const at::Tensor& t : own) TORCH_CHECK(share(*given, t) != Share::kSome, name, " must not partly overlap an input");
   for (const at::Tensor& t : others) TORCH_CHECK(share(*given, t) == Share::kNone, name, " must not overlap an input of the other heads");
@@ -134,7 +135,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> qk_norm_rope_backward
   TORCH_CHECK(share(qo, ko) == Share::kNone, "dq_in and dk_in must not overlap");
   a.y[0] = view(qo, "dq_in", q, s, a.H[0]);
   a.y[1] = view(ko, "dk_in", q, s, a.H[1]);
-  at::Tensor dqw = dqw_.has_value() ? *dqw_ : at::empty_like(qw), dkw = dkw_.has_value() ? *dkw_ : at::empty_like(kw);
+  at::Tensor dqw = dqw_.has_value() ? *dqw_ : fresh(qw.sizes(), qw.scalar_type(), q), dkw = dkw_.has_value() ? *dkw_ : fresh(kw.sizes(), kw.scalar_type(), q);
   for (const at::Tensor* w : {&dqw, &dkw})
     TORCH_CHECK(w->is_cuda() && w->device() == q.device() && w->is_contiguous() && w->dim() == 1 && w->numel() == s.D &&
                     w->scalar_type() == qw.scalar_type(),
@@ -148,7 +149,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> qk_norm_rope_backward
     return {qo, ko, dqw, dkw};
   }
   const int blocks = rotary_blocks(a, true, at::cuda::getCurrentDeviceProperties()->multiProcessorCount);
-  at::Tensor partial = at::empty({(int64_t)blocks * s.D}, q.options().dtype(at::kFloat));
+  at::Tensor partial = fresh({(int64_t)blocks * s.D}, at::kFloat, q);
   a.partial = partial.data_ptr<float>();
   PCCL_CUDA(launch_rotary_backward(a, blocks, at::cuda::getCurrentCUDAStream().stream()));
   return {qo, ko, dqw, dkw};
