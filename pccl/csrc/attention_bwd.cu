@@ -21,9 +21,11 @@
 //
 // What bounds it.  4 x 2048 x 16 heads of 128 causal take 250 us, 687 TFLOP/s by the five products that the formulas need and 960
 // by the seven computed: row sums 10 us (6.4 TB/s), dk and dv 132, dq 103.  With the exponentials and conversions left out the
-// products alone take 110 and 87: tensor memory holds four or five 128 x 128 accumulators and no more, so a product waits for its
-// operand's conversion at every tile, with one tile of the other chain in between.  Sixteen compute warps for eight: no faster.  The
-// clock is at 1.69 GHz by the power limit.  16 heads of 4096 223 us (768 TFLOP/s), heads of 64 199.
+// products alone take 110 and 87, 1330 and 1260 TFLOP/s, at heads of 64 81 instead of 110 for dk and dv; without the loads of query tiles
+// the whole takes 249.  So most of it is the products that have their first operand in tensor memory and the hand-over of that
+// operand at every tile: tensor memory holds four or five 128 x 128 accumulators and no more.  Sixteen compute warps for
+// eight: 253, at heads of 64 197 instead of 201; a second tile of scores at heads of 64: 199.  The clock is at 1.69 GHz by the
+// power limit.  16 heads of 4096 223 us (768 TFLOP/s), heads of 64 200.
 #include "attention.cuh"
 
 namespace pccl {
