@@ -278,22 +278,37 @@ __device__ __forceinline__ void write_order(const int* cu, int nseq, int limit, 
   const int64_t total = above(1);
   for (int64_t t = total + threadIdx.x; t < entries; t += blockDim.x) order[t] = make_int2(-1, (int)(t - total));
 }
+// What an earlier kernel has written, read where all SMs meet.  For a kernel that reads before its pdl_wait() (the dq kernel): an
+// ordinary load may return what this SM's first-level cache still holds from before that kernel.
+__device__ __forceinline__ int load_past_l1(const int* p) {
+  int v;
+  asm volatile("ld.relaxed.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ float load_past_l1(const float* p) {
+  float v;
+  asm volatile("ld.relaxed.gpu.global.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
+  return v;
+}
+template <bool PAST_L1>
 __device__ __forceinline__ Span find_span(const AttnArgs& a, int t, int rows, bool of_keys) {
-  const int2 e = (of_keys ? a.order_k : a.order_q)[t];
+  auto read = [](const int* p) { return PAST_L1 ? load_past_l1(p) : *p; };
+  const int2* entry = (of_keys ? a.order_k : a.order_q) + t;
+  const int2 e = PAST_L1 ? make_int2(load_past_l1(&entry->x), load_past_l1(&entry->y)) : *entry;
   Span sp;
   sp.batch = 0;
   if (e.x < 0) {
     const int limit = of_keys ? a.Sk : a.Sq;
-    const int64_t first = (int64_t)clamp_start((of_keys ? a.cu_k : a.cu_q)[a.nseq], limit) + (int64_t)e.y * rows;
+    const int64_t first = (int64_t)clamp_start(read((of_keys ? a.cu_k : a.cu_q) + a.nseq), limit) + (int64_t)e.y * rows;
     sp.len_q = sp.len_k = 0;
     sp.tile = -1;
     sp.first_q = sp.first_k = first > limit ? limit : (int)first;
     return sp;
   }
-  sp.first_q = clamp_start(a.cu_q[e.x], a.Sq);
-  sp.len_q = clamp_start(a.cu_q[e.x + 1], a.Sq) - sp.first_q;
-  sp.first_k = clamp_start(a.cu_k[e.x], a.Sk);
-  sp.len_k = clamp_start(a.cu_k[e.x + 1], a.Sk) - sp.first_k;
+  sp.first_q = clamp_start(read(a.cu_q + e.x), a.Sq);
+  sp.len_q = clamp_start(read(a.cu_q + e.x + 1), a.Sq) - sp.first_q;
+  sp.first_k = clamp_start(read(a.cu_k + e.x), a.Sk);
+  sp.len_k = clamp_start(read(a.cu_k + e.x + 1), a.Sk) - sp.first_k;
   if (sp.len_q < 0) sp.len_q = 0;
   if (sp.len_k < 0) sp.len_k = 0;
   sp.tile = e.y;

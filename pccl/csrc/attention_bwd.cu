@@ -133,7 +133,7 @@ __device__ __forceinline__ DkvWork dkv_work_at(const AttnArgs& a, unsigned id) {
   }
   if (a.cu_q != nullptr) {
     w.kv_head = (int)(id % (unsigned)a.Hk);
-    w.sp = find_span(a, (int)(id / (unsigned)a.Hk), 128, true);
+    w.sp = find_span<false>(a, (int)(id / (unsigned)a.Hk), 128, true);
   } else {
     // with a causal mask the first tiles are seen by the most queries: they come first
     const unsigned heads = (unsigned)(a.B * a.Hk), bh = id % heads;
@@ -166,6 +166,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   using C = Dkv<DP>;
   extern __shared__ __align__(1024) unsigned char smem[];   // the swizzled tiles want 1024 bytes; without static variables it starts there
   if ((smem_u32(smem) & 1023u) != 0u) {
+    pdl_wait();                                              // this block too lets the dq kernel in only when the row sums are complete
     if (threadIdx.x == 0) atomicCAS(a.error, 0, kErrLoad);
     return;
   }
@@ -210,7 +211,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   fence_after();
   const uint32_t tmem = b.tmem;
   pdl_wait();
-  pdl_trigger();                                             // behind the wait: see the dq kernel
+  pdl_trigger();                                             // behind the wait of every block: the dq kernel relies on it
 
   // The tile after the k-th, for every role alike: -1 none, -2 a wait gave up.  Whole warps.
   auto next_tile = [&](int k) {
@@ -574,7 +575,7 @@ __device__ __forceinline__ DqWork dq_work_at(const AttnArgs& a, unsigned id, int
   }
   if (a.cu_q != nullptr) {
     w.head = (int)(id % (unsigned)a.H);
-    w.sp = find_span(a, (int)(id / (unsigned)a.H), 128, false);
+    w.sp = find_span<true>(a, (int)(id / (unsigned)a.H), 128, false);
   } else {
     const unsigned heads = (unsigned)(a.B * a.H), bh = id % heads, t = id / heads;
     w.head = (int)(bh % (unsigned)a.H);
@@ -643,8 +644,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   fence_after();
   const uint32_t tmem = b.tmem;
   // beside: the kernel in front is the one for dk and dv, which shares nothing with this one but what both read.  All of that,
-  // the row sums among it, was complete when its blocks let this one's in, so these begin on the SMs that it leaves, and wait
-  // for it at their end.
+  // the row sums among it, was complete when its blocks let this one's in, since each of them has passed its own wait before (or
+  // left behind it), so these begin on the SMs that it leaves, and wait for it at their end.  Completeness is not yet visibility
+  // to this grid, which has not waited: what earlier kernels of the call have written (row sums, tile list) and the other words that it
+  // reads by ordinary loads (lse, starts) are read past the first-level cache, and tiles come by TMA, which does not use it.
   if (!beside) pdl_wait();
 
   // The tile after the k-th, for every role alike: -1 none, -2 a wait gave up.  Whole warps.
@@ -812,9 +815,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       float lse2 = INFINITY, delta = 0.f;
       if (exists) {
         const int64_t at = stat_row(a, w.sp.batch, w.head) + w.sp.first_q + row;
-        const float x = a.lse[at];
+        const float x = load_past_l1(a.lse + at);
         lse2 = x == -INFINITY ? INFINITY : x * kLog2e;
-        delta = a.delta[at];
+        delta = load_past_l1(a.delta + at);
       }
       const int keys = !a.causal ? w.sp.len_k : (row + w.offset + 1 < w.sp.len_k ? row + w.offset + 1 : w.sp.len_k);
       const int keys_all = __shfl_sync(0xffffffffu, keys, 0);

@@ -77,7 +77,7 @@ __device__ __forceinline__ Work work_at(const AttnArgs& a, unsigned id, int tile
   }
   if (a.cu_q != nullptr) {
     w.head = (int)(id % (unsigned)a.H);
-    w.sp = find_span(a, (int)(id / (unsigned)a.H), 256, false);
+    w.sp = find_span<false>(a, (int)(id / (unsigned)a.H), 256, false);
   } else {
     // with a causal mask the last tiles have the most keys: they come first
     const unsigned heads = (unsigned)(a.B * a.H), bh = id % heads, t = id / heads;

@@ -11,6 +11,10 @@
 //   * every block calls pdl_wait(), so a kernel never ends before the ones in front of it;
 //   * pdl_trigger(), which lets the next kernel's blocks in, comes after the block owns all it needs (tensor memory among it):
 //     a block that waits must never hold what a running one still has to acquire.
+// One kernel departs from the first rule: attention's dq kernel, where the dk/dv kernel is right in front of it, waits at its end.  That
+// holds because (a) every block of the dk/dv kernel, also one that gives up, calls pdl_wait() before it triggers or ends, so all that came
+// before it is complete; (b) dq reads nothing that the dk/dv kernel writes and writes nothing that it reads; (c) it reads global
+// memory past the first-level cache only.  A kernel put between the row sums and dk/dv, or an earlier trigger in dk/dv, ends (a).
 // Kernels that wait for other ranks, or for copies that run beside them, are launched the ordinary way.
 #pragma once
 #include <cuda_runtime.h>

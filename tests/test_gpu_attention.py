@@ -503,3 +503,38 @@ def test_offsets_beyond_32_bits():
     want = attention_backward(dout, q, k, v, out, lse)
     near = attention_backward(views[3], *views[:3], got, lse, dq=cut(grads, 0), dk=cut(grads, 128), dv=cut(grads, 256))
     assert all(torch.equal(a, b) for a, b in zip(near, want))
+
+
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("shape", [(1, 300, 2, 64), (1, 700, 16, 128)], ids=str)
+def test_row_sums_of_the_call_in_front_are_not_read(shape, packed):
+    """The kernel for dq begins before the one for dk and dv has ended.  Calls back to back, whose inputs, row sums and tile lists
+    take the same memory and differ from call to call, give the bits of calls that stand alone."""
+    from pccl.ops.attention import attention_backward, attention_forward, check_errors
+
+    B, S, H, D = shape
+    sets = []
+    for seed in range(6):
+        x = list(_inputs(B, S, S, H, H, D, BF, 60 + seed, 1.0 + seed))
+        cu = None
+        if packed:
+            x = [t[0] for t in x]
+            cu = torch.tensor([0, 30 * (seed + 1), 30 * (seed + 1), S - seed], dtype=torch.int32, device=DEV)
+        out, lse = attention_forward(*x[:3], cu_seqlens_q=cu)
+        sets.append((x[3].contiguous(), *(t.contiguous() for t in x[:3]), out, lse, cu))
+    alone = []
+    for s in sets:
+        torch.cuda.synchronize()
+        alone.append([t.clone() for t in attention_backward(*s[:6], cu_seqlens_q=s[6])])
+        torch.cuda.synchronize()
+    here = [None if t is None else t.clone() for t in sets[0]]
+    for _ in range(20):
+        got = []
+        for s in sets:
+            for a, b in zip(here, s):
+                if a is not None:
+                    a.copy_(b)
+            got.append([t.clone() for t in attention_backward(*here[:6], cu_seqlens_q=here[6])])
+        for a, b in zip(alone, got):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
+    check_errors()
