@@ -19,9 +19,14 @@
 // because its root divides.  A value between two codes becomes one of them by chance, in proportion to its distances, so that
 // the mean is exact: rounding to the nearest code would stop an average whose change per step (1 - b2 of it) is below half a
 // step of the code, which at b2 = 0.999 is nearly always.  The chance is a hash of the element's place in the state, the
-// step and the seed: the same call gives the same bits.  Two rules keep the division harmless: a v that is not zero never gets
-// code 0, and a block whose largest size is below 2^-80 (whose root is far below any eps) is held as zeros.  A block that
-// holds a value that is not finite reads back as NaN throughout: a broken step does not hide.
+// step and the seed: the same call gives the same bits.  A v that is not zero never gets code 0, and a block whose largest size is
+// below 2^-80 is held as zeros.  A block that holds a value that is not finite reads back as NaN throughout: a broken step does not hide.
+//
+// What zeros for a small v cost.  At each step at most 2^-80 is dropped, which fades by b2 a step, so v lacks at most 2^-80 b2 / (1 - b2)
+// in all, and so much over (1 - b2) / (1 - b2^t) of that, never more, after the correction of its bias: the root lacks at most
+// r = 2^-40 / sqrt(1 - b2).  The quotient m / (root + eps) is then too large by r / eps of itself at most, whatever m is.  Where eps is
+// below 32 r (1.3e-10 at b2 = 0.95, 9.2e-10 at 0.999) 8-bit states are refused: with eps = 1e-15, gradients of 2e-12 that
+// stop would move a parameter by 1800 lr in one step.
 // The parameter is updated from the 32-bit m and v, before they are rounded.
 //
 // The products and sums that lead to a code are rounded one by one (no fused multiply-add): what a code is does not hang on what
@@ -379,7 +384,7 @@ __global__ void __launch_bounds__(kThreads, BITS8 ? 4 : 2) adamw_multi_kernel(co
     }
     // ---- the step
     const F2 keep = f2(1.f - a.lr * t.decay), rate = f2(-a.lr * a.bias1);
-    const bool tiny_eps = a.eps < 1e-15f;
+    const bool tiny_eps = !BITS8 && a.eps < 1e-15f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const F2 y = f2(g[2 * i], g[2 * i + 1]) * f2(gs);
@@ -502,6 +507,8 @@ cudaError_t launch_grad(const AdamMultiArgs& a, const AdamTensor* t, int count, 
 }
 
 }  // namespace
+
+double adamw_least_eps(double beta2) { return ldexp(1.0, -35) / sqrt(1.0 - beta2); }
 
 uint32_t adamw_noise_key(uint64_t seed, int64_t step) { return mix(mix((uint32_t)seed) + (uint32_t)step); }
 

@@ -31,6 +31,8 @@ struct AdamMultiArgs {
 
 enum AdamType : int { kAdamBf16 = 0, kAdamF16 = 1, kAdamF32 = 2 };
 
+// The smallest eps that 8-bit states take, 2^-35 / sqrt(1 - beta2): adamw_multi.cu has the reason.
+double adamw_least_eps(double beta2);
 uint32_t adamw_noise_key(uint64_t seed, int64_t step);
 cudaError_t launch_adamw_multi(const AdamMultiArgs& a, const AdamTensor* tensors, int count, int param_type, int grad_type, bool bits8,
                                int sm_count, cudaStream_t s);

@@ -69,6 +69,8 @@ void adamw_multi(const std::vector<at::Tensor>& params, const std::vector<at::Te
   TORCH_CHECK(step >= 1, "step counts from 1");
   TORCH_CHECK(std::isfinite(lr) && beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1 && eps >= 0 && std::isfinite(eps),
               "lr and eps must be finite, eps not negative, beta1 and beta2 in [0, 1)");
+  TORCH_CHECK(!(m_scale.has_value() || v_scale.has_value()) || eps >= adamw_least_eps(beta2), "8-bit states need an eps of at least ",
+              adamw_least_eps(beta2), " at this beta2: they hold second moments below 2^-80 as zeros");
   if (n == 0) return;
   const c10::Device device = params[0].device();
   const int pt = type_of(params[0], "a parameter"), gt = type_of(grads[0], "a gradient");
@@ -179,6 +181,7 @@ std::tuple<at::Tensor, at::Tensor> adamw_dequantize(const at::Tensor& m, const a
 
 void bind_adamw_multi(py::module_& m) {
   m.attr("adamw_block") = kAdamBlock;
+  m.def("adamw_least_eps", &adamw_least_eps, py::arg("beta2"), "the smallest eps that 8-bit states take");
   m.def("adamw_multi", &adamw_multi, py::arg("params"), py::arg("grads"), py::arg("masters"), py::arg("exp_avg"), py::arg("exp_avg_sq"),
         py::arg("exp_avg_scale"), py::arg("exp_avg_sq_scale"), py::arg("weight_decay"), py::arg("step"), py::arg("lr"), py::arg("beta1"),
         py::arg("beta2"), py::arg("eps"), py::arg("grad_scale") = 1.0, py::arg("max_grad_norm") = 0.0,

@@ -7,6 +7,8 @@ and 2/64 of a byte of scales per parameter instead of 8 (``optim_bits=8`` in the
 The states of a list are flat: each tensor's part starts on a multiple of 256 elements, in the order of the list.  With 8
 bits, 256 elements share a scale, and a value between two codes is rounded to one of them by chance so that its mean is
 kept; the chance is a function of ``seed``, ``step`` and the element's place, so the same call gives the same bits.
+Second moments of a block that are all below 2^-80 are held as zeros, so with 8 bits ``eps`` has to be large enough
+(``least_eps``) that their roots do not count beside it.
 """
 from __future__ import annotations
 
@@ -22,6 +24,12 @@ BLOCK = 256
 
 def _C():
     return build_kernels.load()
+
+
+def least_eps(beta2: float) -> float:
+    """The smallest ``eps`` that 8-bit states take: 2^-35 / sqrt(1 - beta2), 1.3e-10 at 0.95, 9.2e-10 at 0.999.  The update of an
+    element whose second moment is held as zero is then too large by 1/32 of itself at most."""
+    return _C().adamw_least_eps(beta2)
 
 
 def state_offsets(params: Sequence[torch.Tensor]) -> List[int]:

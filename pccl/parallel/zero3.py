@@ -128,6 +128,11 @@ class Zero3Engine:
         # both Adam moments in 32 bits, or in 8 with a scale for each 256 (pccl.ops.optim)
         if optim_bits not in (8, 32):
             raise ValueError("optim_bits must be 8 or 32")
+        if optim_bits == 8:
+            from ..ops.optim import least_eps
+
+            if self.optim.eps < least_eps(self.optim.beta2):
+                raise ValueError(f"optim_bits=8 needs an eps of at least {least_eps(self.optim.beta2):.3g} at beta2 = {self.optim.beta2}")
         self.optim_bits = optim_bits
         # parameter gathers by the GPU's copy engines instead of gather kernels (no SM is taken from
         # the GEMMs they overlap); needs symmetric parameter shards

@@ -298,3 +298,29 @@ def test_more_than_2_31_elements(bits):
         assert float(state.exp_avg_scale[:-8].abs().max()) == 0.0
     else:
         assert torch.equal(state.exp_avg[-2048:], own.exp_avg) and torch.equal(state.exp_avg_sq[-2048:], own.exp_avg_sq)
+
+
+@pytest.mark.parametrize("beta2", [0.95, 0.999])
+def test_second_moments_held_as_zeros_do_not_count(beta2):
+    """Gradients around the size whose square is held as zero, then none, at the smallest eps that is taken.  A block's gradients
+    are all alike, so its codes are its largest value and round nothing.  The root of v lacks at most eps / 32 (the kernel's head), so an
+    update lies between that of the 32-bit states and 33/32 of it; beside that, ten roundings of 2^-24 in the moments and a dozen of 2^-23
+    in the update (the hardware's root and reciprocal), and half a step of the parameter, which starts at zero."""
+    from pccl.ops.optim import adamw_state, adamw_step, least_eps
+
+    sizes = torch.logspace(-14, -8, 40, device=DEV)
+    sizes[0] = 2e-12
+    grad, none = sizes.repeat_interleave(256), torch.zeros(40 * 256, device=DEV)
+    hyper = dict(lr=1.0, beta1=0.9, beta2=beta2, eps=least_eps(beta2), weight_decay=0.0)
+    p8, p32 = none.clone(), none.clone()
+    s8, s32 = adamw_state([p8], 8), adamw_state([p32], 32)
+    for step in range(1, 250):
+        g = grad if step < 50 else none
+        for p, s in ((p8, s8), (p32, s32)):
+            p.zero_()
+            adamw_step([p], [g], s, step=step, **hyper)
+        # what m keeps below 2^-80 is held as zero too: 2^-80 over eps of an update
+        slack, least = 24 * 2.0 ** -23, 2.0 ** -80 / hyper["eps"] / (1 - 0.9) + 2.0 ** -126
+        a, b = -p8.double(), -p32.double()
+        assert torch.all(a >= b * (1 - slack * step) - least) and torch.all(a <= b * (33 / 32 + slack * step) + least), step
+    assert torch.all(s8.dequantize()[1] <= s32.exp_avg_sq * (1 + 2.0 ** -10))

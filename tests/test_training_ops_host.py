@@ -83,3 +83,22 @@ def test_positions_of_packed_documents():
 def test_what_the_attention_kernels_take():
     takes = lambda d: gpt.native_attention_takes(GPTConfig(1, 4 * d, 4, 64, vocab=8, seq_len=8))      # noqa: E731
     assert takes(8) and takes(64) and takes(80) and takes(128) and not takes(136) and not takes(12)
+
+
+def test_8_bit_states_refuse_a_small_eps():
+    from pccl.ops.optim import least_eps
+    from pccl.parallel.zero3 import OptimConfig, Zero3Engine
+
+    p, g = [torch.zeros(300)], [torch.zeros(300)]
+    for beta2 in (0.0, 0.95, 0.999, 0.99999):
+        least = 2.0 ** -35 / math.sqrt(1 - beta2)
+        assert abs(least_eps(beta2) / least - 1) < 1e-12
+        go = lambda eps, bits: adamw_step(p, g, adamw_state(p, bits), step=1, lr=1e-3, beta2=beta2, eps=eps)      # noqa: E731,B023
+        for eps in (0.0, 1e-15, least * 0.999):
+            with pytest.raises(RuntimeError, match="eps of at least"):
+                go(eps, 8)
+        for eps, bits in ((least * 1.001, 8), (1e-8, 8), (0.0, 32)):
+            with pytest.raises(RuntimeError, match="CUDA"):                        # taken, but for where the tensors lie
+                go(eps, bits)
+    with pytest.raises(ValueError, match="eps of at least"):
+        Zero3Engine(CFG, optim=OptimConfig(eps=1e-12), device=torch.device("cpu"), optim_bits=8)
