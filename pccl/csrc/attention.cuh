@@ -372,6 +372,13 @@ __device__ __forceinline__ void store32_f32(float* row, int col0, int D, const u
 __device__ __forceinline__ int64_t stat_row(const AttnArgs& a, int batch, int head) { return ((int64_t)batch * a.H + head) * a.Sq; }
 
 // ---- host
+// An early launch that is counted.
+template <typename K, typename... A>
+cudaError_t launch_counted(int64_t& kernels, K kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t stream, const A&... args) {
+  const cudaError_t e = launch_pdl(kernel, grid, block, smem, stream, args...);
+  if (e == cudaSuccess) ++kernels;
+  return e;
+}
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                               const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
                               CUtensorMapFloatOOBfill);

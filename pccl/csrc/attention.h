@@ -51,7 +51,8 @@ struct AttnScratch {
 };
 AttnScratch plan_attention_forward(AttnArgs& a, int sm_count);
 AttnScratch plan_attention_backward(AttnArgs& a, int sm_count);
-cudaError_t launch_attention_forward(const AttnArgs& a, cudaStream_t stream);
-cudaError_t launch_attention_backward(const AttnArgs& a, cudaStream_t stream);
+// kernels: goes up by one with each kernel launched.
+cudaError_t launch_attention_forward(const AttnArgs& a, cudaStream_t stream, int64_t& kernels);
+cudaError_t launch_attention_backward(const AttnArgs& a, cudaStream_t stream, int64_t& kernels);
 
 }  // namespace pccl

@@ -3,6 +3,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <atomic>
 #include <cmath>
 #include <cstring>
 #include <mutex>
@@ -38,6 +39,8 @@ volatile int* error_word(int device) {
   });
   return words + device;
 }
+
+std::atomic<int64_t> g_kernels{0};         // launched since the process began
 
 struct Shape {
   bool packed;
@@ -152,7 +155,10 @@ std::tuple<at::Tensor, at::Tensor> attention_forward(const at::Tensor& q, const 
     a.partial = partial.data_ptr<float>();
     a.partial_lse = partial_lse.data_ptr<float>();
   }
-  PCCL_CUDA(launch_attention_forward(a, at::cuda::getCurrentCUDAStream().stream()));
+  int64_t kernels = 0;
+  const cudaError_t e = launch_attention_forward(a, at::cuda::getCurrentCUDAStream().stream(), kernels);
+  g_kernels += kernels;
+  PCCL_CUDA(e);
   return {out, lse};
 }
 
@@ -194,7 +200,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_backward(const at::Tens
     partial = fresh({need.partial}, at::kFloat, q);
     a.partial = partial.data_ptr<float>();
   }
-  PCCL_CUDA(launch_attention_backward(a, at::cuda::getCurrentCUDAStream().stream()));
+  int64_t kernels = 0;
+  const cudaError_t e = launch_attention_backward(a, at::cuda::getCurrentCUDAStream().stream(), kernels);
+  g_kernels += kernels;
+  PCCL_CUDA(e);
   return {dq, dk, dv};
 }
 
@@ -208,6 +217,7 @@ void bind_attention(py::module_& m) {
         py::arg("causal") = true, py::arg("scale") = py::none(), py::arg("cu_seqlens_q") = py::none(),
         py::arg("cu_seqlens_k") = py::none(), py::arg("dq") = py::none(), py::arg("dk") = py::none(), py::arg("dv") = py::none(),
         "gradients of attention: returns (dq, dk, dv)");
+  m.def("attention_kernels_launched", [] { return g_kernels.load(); }, "kernels of attention launched since the process began");
   m.def("attention_error", [](int device) { return (int)*error_word(device); }, "0, or why a bounded wait of an attention kernel gave up");
   m.def("attention_reset_error", [](int device) { *error_word(device) = 0; });
 }

@@ -945,10 +945,11 @@ __global__ void __launch_bounds__(256) attention_sum_kernel(const float* partial
       make_uint4(pack2<BF16>(o[0], o[1]), pack2<BF16>(o[2], o[3]), pack2<BF16>(o[4], o[5]), pack2<BF16>(o[6], o[7]));
 }
 template <bool BF16>
-cudaError_t add_parts(const float* partial, int parts, const AttnTensor& dst, int B, int H, int S, int D, cudaStream_t stream) {
+cudaError_t add_parts(const float* partial, int parts, const AttnTensor& dst, int B, int H, int S, int D, cudaStream_t stream,
+                      int64_t& kernels) {
   const int64_t blocks = ((int64_t)B * H * S + 15) / 16;
   if (blocks > INT32_MAX) return cudaErrorInvalidValue;
-  return launch_pdl(attention_sum_kernel<BF16>, dim3((unsigned)blocks), dim3(256), 0, stream, partial, parts, dst, B, H, S, D);
+  return launch_counted(kernels, attention_sum_kernel<BF16>, dim3((unsigned)blocks), dim3(256), 0, stream, partial, parts, dst, B, H, S, D);
 }
 
 // The shared-memory limit is an attribute of the function on the current device.
@@ -966,29 +967,30 @@ cudaError_t allow_smem(uint32_t bytes) {
 
 template <int DP, bool BF16, bool SPLIT>
 cudaError_t launch_dkv(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mdo, const AttnArgs& a,
-                       cudaStream_t stream) {
+                       cudaStream_t stream, int64_t& kernels) {
   const cudaError_t e = allow_smem<attention_dkv_kernel<DP, BF16, SPLIT>>(Dkv<DP>::kSmem);
   if (e != cudaSuccess) return e;
   const int64_t tiles = a.cu_q != nullptr ? max_tiles(a.Sk, a.nseq, 128) : ((int64_t)a.Sk + 127) / 128;
   const int64_t ctas = tiles * a.Hk * a.B * a.parts_dkv;
   if (ctas > INT32_MAX) return cudaErrorInvalidValue;
-  return launch_pdl(attention_dkv_kernel<DP, BF16, SPLIT>, dim3((unsigned)ctas), dim3(kThreads), Dkv<DP>::kSmem, stream, mq, mk, mv, mdo, a);
+  return launch_counted(kernels, attention_dkv_kernel<DP, BF16, SPLIT>, dim3((unsigned)ctas), dim3(kThreads), Dkv<DP>::kSmem, stream, mq,
+                        mk, mv, mdo, a);
 }
 template <int DP, bool BF16, bool SPLIT>
 cudaError_t launch_dq(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mdo, const AttnArgs& a,
-                      cudaStream_t stream) {
+                      cudaStream_t stream, int64_t& kernels) {
   const cudaError_t e = allow_smem<attention_dq_kernel<DP, BF16, SPLIT>>(Dq<DP>::kSmem);
   if (e != cudaSuccess) return e;
   const int64_t tiles = a.cu_q != nullptr ? max_tiles(a.Sq, a.nseq, 128) : ((int64_t)a.Sq + 127) / 128;
   const int64_t ctas = tiles * a.H * a.B * a.parts_dq;
   if (ctas > INT32_MAX) return cudaErrorInvalidValue;
   const bool beside = a.Sk > 0 && a.parts_dkv == 1;          // the dk/dv kernel is right in front, and no part of its work is in this one's memory
-  return launch_pdl(attention_dq_kernel<DP, BF16, SPLIT>, dim3((unsigned)ctas), dim3(kThreads), Dq<DP>::kSmem, stream, mq, mk, mv, mdo, a,
-                    (int)tiles, beside);
+  return launch_counted(kernels, attention_dq_kernel<DP, BF16, SPLIT>, dim3((unsigned)ctas), dim3(kThreads), Dq<DP>::kSmem, stream, mq, mk,
+                        mv, mdo, a, (int)tiles, beside);
 }
 
 template <int DP, bool BF16>
-cudaError_t launch(const AttnArgs& a, cudaStream_t stream) {
+cudaError_t launch(const AttnArgs& a, cudaStream_t stream, int64_t& kernels) {
   const bool packed = a.cu_q != nullptr;
   CUtensorMap mq, mk, mv, mdo;
   if (a.Sq > 0 && (!make_map(&mq, a.q, BF16, a.D, a.H, a.Sq, a.B) || !make_map(&mdo, a.dout, BF16, a.D, a.H, a.Sq, a.B)))
@@ -998,28 +1000,31 @@ cudaError_t launch(const AttnArgs& a, cudaStream_t stream) {
   if (a.Sq == 0) mq = mdo = mk;                              // nothing of what is missing is ever loaded
   if (a.Sk == 0) mk = mv = mq;
   if (packed) {
-    const cudaError_t e = launch_pdl(attention_orders_kernel, dim3(2), dim3(1024), 0, stream, a);
+    const cudaError_t e = launch_counted(kernels, attention_orders_kernel, dim3(2), dim3(1024), 0, stream, a);
     if (e != cudaSuccess) return e;
   }
   if (a.Sq > 0) {
     if (a.B > 65535) return cudaErrorInvalidValue;
-    const cudaError_t e = launch_pdl(attention_delta_kernel<BF16>, dim3((unsigned)((a.Sq + 63) / 64), (unsigned)a.H, (unsigned)a.B), dim3(256), 0,
-                                     stream, a);
+    const cudaError_t e = launch_counted(kernels, attention_delta_kernel<BF16>,
+                                         dim3((unsigned)((a.Sq + 63) / 64), (unsigned)a.H, (unsigned)a.B), dim3(256), 0, stream, a);
     if (e != cudaSuccess) return e;
   }
   if (a.Sk > 0) {
-    cudaError_t e = a.parts_dkv > 1 ? launch_dkv<DP, BF16, true>(mq, mk, mv, mdo, a, stream) : launch_dkv<DP, BF16, false>(mq, mk, mv, mdo, a, stream);
+    cudaError_t e = a.parts_dkv > 1 ? launch_dkv<DP, BF16, true>(mq, mk, mv, mdo, a, stream, kernels)
+                                    : launch_dkv<DP, BF16, false>(mq, mk, mv, mdo, a, stream, kernels);
     if (e != cudaSuccess) return e;
     if (a.parts_dkv > 1) {
-      if ((e = add_parts<BF16>(a.partial, a.parts_dkv, a.dv, a.B, a.Hk, a.Sk, a.D, stream)) != cudaSuccess) return e;
+      if ((e = add_parts<BF16>(a.partial, a.parts_dkv, a.dv, a.B, a.Hk, a.Sk, a.D, stream, kernels)) != cudaSuccess) return e;
       const float* dk = a.partial + (int64_t)a.parts_dkv * a.B * a.Hk * a.Sk * a.D;
-      if ((e = add_parts<BF16>(dk, a.parts_dkv, a.dk, a.B, a.Hk, a.Sk, a.D, stream)) != cudaSuccess) return e;
+      if ((e = add_parts<BF16>(dk, a.parts_dkv, a.dk, a.B, a.Hk, a.Sk, a.D, stream, kernels)) != cudaSuccess) return e;
     }
   }
   if (a.Sq > 0) {
-    cudaError_t e = a.parts_dq > 1 ? launch_dq<DP, BF16, true>(mq, mk, mv, mdo, a, stream) : launch_dq<DP, BF16, false>(mq, mk, mv, mdo, a, stream);
+    cudaError_t e = a.parts_dq > 1 ? launch_dq<DP, BF16, true>(mq, mk, mv, mdo, a, stream, kernels)
+                                   : launch_dq<DP, BF16, false>(mq, mk, mv, mdo, a, stream, kernels);
     if (e != cudaSuccess) return e;
-    if (a.parts_dq > 1 && (e = add_parts<BF16>(a.partial, a.parts_dq, a.dq, a.B, a.H, a.Sq, a.D, stream)) != cudaSuccess) return e;
+    if (a.parts_dq > 1 && (e = add_parts<BF16>(a.partial, a.parts_dq, a.dq, a.B, a.H, a.Sq, a.D, stream, kernels)) != cudaSuccess)
+      return e;
   }
   return cudaSuccess;
 }
@@ -1056,12 +1061,12 @@ AttnScratch plan_attention_backward(AttnArgs& a, int sm_count) {
   return need;
 }
 
-cudaError_t launch_attention_backward(const AttnArgs& a, cudaStream_t stream) {
+cudaError_t launch_attention_backward(const AttnArgs& a, cudaStream_t stream, int64_t& kernels) {
   if (a.B <= 0 || a.H <= 0 || (a.Sq <= 0 && a.Sk <= 0)) return cudaSuccess;
   if (a.Hk <= 0 || a.H % a.Hk != 0 || a.D <= 0 || a.D % 8 != 0 || a.D > kAttnMaxDim || a.Sk < 0 || a.Sq < 0 || a.parts_dq < 1 || a.parts_dkv < 1)
     return cudaErrorInvalidValue;
-  if (a.D <= 64) return a.is_bf16 ? launch<64, true>(a, stream) : launch<64, false>(a, stream);
-  return a.is_bf16 ? launch<128, true>(a, stream) : launch<128, false>(a, stream);
+  if (a.D <= 64) return a.is_bf16 ? launch<64, true>(a, stream, kernels) : launch<64, false>(a, stream, kernels);
+  return a.is_bf16 ? launch<128, true>(a, stream, kernels) : launch<128, false>(a, stream, kernels);
 }
 
 }  // namespace pccl

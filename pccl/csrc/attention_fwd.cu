@@ -505,7 +505,7 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const __grid_consta
 }
 
 template <int DP, bool BF16, bool SPLIT>
-cudaError_t launch(const AttnArgs& a, cudaStream_t stream) {
+cudaError_t launch(const AttnArgs& a, cudaStream_t stream, int64_t& kernels) {
   using C = Fwd<DP>;
   CUtensorMap mq, mk, mv;
   if (!make_map(&mq, a.q, BF16, a.D, a.H, a.Sq, a.B)) return cudaErrorInvalidValue;
@@ -525,18 +525,18 @@ cudaError_t launch(const AttnArgs& a, cudaStream_t stream) {
   const int64_t ctas = tiles * a.H * a.B * a.parts_o;
   if (ctas > INT32_MAX) return cudaErrorInvalidValue;
   if (a.cu_q != nullptr) {
-    if ((e = launch_pdl(attention_order_kernel, dim3(1), dim3(1024), 0, stream, a)) != cudaSuccess) return e;
+    if ((e = launch_counted(kernels, attention_order_kernel, dim3(1), dim3(1024), 0, stream, a)) != cudaSuccess) return e;
   }
-  e = launch_pdl(kernel, dim3((unsigned)ctas), dim3(kThreads), C::kSmem, stream, mq, mk, mv, a, (int)tiles);
+  e = launch_counted(kernels, kernel, dim3((unsigned)ctas), dim3(kThreads), C::kSmem, stream, mq, mk, mv, a, (int)tiles);
   if (e != cudaSuccess || !SPLIT) return e;
   const int64_t blocks = ((int64_t)a.B * a.H * a.Sq + 15) / 16;
   if (blocks > INT32_MAX) return cudaErrorInvalidValue;
-  return launch_pdl(attention_join_kernel<BF16>, dim3((unsigned)blocks), dim3(256), 0, stream, a);
+  return launch_counted(kernels, attention_join_kernel<BF16>, dim3((unsigned)blocks), dim3(256), 0, stream, a);
 }
 
 template <int DP, bool BF16>
-cudaError_t launch_type(const AttnArgs& a, cudaStream_t stream) {
-  return a.parts_o > 1 ? launch<DP, BF16, true>(a, stream) : launch<DP, BF16, false>(a, stream);
+cudaError_t launch_type(const AttnArgs& a, cudaStream_t stream, int64_t& kernels) {
+  return a.parts_o > 1 ? launch<DP, BF16, true>(a, stream, kernels) : launch<DP, BF16, false>(a, stream, kernels);
 }
 
 }  // namespace
@@ -563,11 +563,11 @@ AttnScratch plan_attention_forward(AttnArgs& a, int sm_count) {
   return need;
 }
 
-cudaError_t launch_attention_forward(const AttnArgs& a, cudaStream_t stream) {
+cudaError_t launch_attention_forward(const AttnArgs& a, cudaStream_t stream, int64_t& kernels) {
   if (a.B <= 0 || a.H <= 0 || a.Sq <= 0) return cudaSuccess;
   if (a.Hk <= 0 || a.H % a.Hk != 0 || a.D <= 0 || a.D % 8 != 0 || a.D > kAttnMaxDim || a.Sk < 0 || a.parts_o < 1) return cudaErrorInvalidValue;
-  if (a.D <= 64) return a.is_bf16 ? launch_type<64, true>(a, stream) : launch_type<64, false>(a, stream);
-  return a.is_bf16 ? launch_type<128, true>(a, stream) : launch_type<128, false>(a, stream);
+  if (a.D <= 64) return a.is_bf16 ? launch_type<64, true>(a, stream, kernels) : launch_type<64, false>(a, stream, kernels);
+  return a.is_bf16 ? launch_type<128, true>(a, stream, kernels) : launch_type<128, false>(a, stream, kernels);
 }
 
 }  // namespace pccl

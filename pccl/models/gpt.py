@@ -349,10 +349,11 @@ def _attention(qkv: torch.Tensor, p: Dict[str, torch.Tensor], cfg: GPTConfig, ba
         global native_launches
         from ..ops.attention import attention_forward
 
-        native_launches += 1
+        before = _kernels().attention_kernels_launched()
         if cu is not None:
             q, k, v = (t.reshape(T, H, dh) if t.is_contiguous() else t.view(T, H, dh) for t in (q, k, v))
         out, lse = attention_forward(q, k, v, causal=True, cu_seqlens_q=cu)
+        native_launches += _kernels().attention_kernels_launched() - before
         return out.view(T, d), (qkv, q, k, v, out, lse)
     if cu is not None:
         raise ValueError("packed documents need native_attention")
@@ -382,7 +383,7 @@ def _attention_backward(da: torch.Tensor, saved, p: Dict[str, torch.Tensor], gr:
     else:
         from ..ops.attention import attention_backward
 
-        native_launches += 3
+        before = _kernels().attention_kernels_launched()
         dqkv = torch.empty_like(qkv)
         parts = dqkv.view(batch, S, 3, H, dh).unbind(2)
         grads = parts
@@ -391,6 +392,7 @@ def _attention_backward(da: torch.Tensor, saved, p: Dict[str, torch.Tensor], gr:
             dqkv.zero_()                            # tokens behind the last document have no gradient
         attention_backward(da.view(att.shape), q, k, v, att, lse, causal=True,
                            cu_seqlens_q=pos.cu_seqlens if pos is not None else None, dq=grads[0], dk=grads[1], dv=grads[2])
+        native_launches += _kernels().attention_kernels_launched() - before
         dq, dk = parts[0], parts[1]
     if cfg.qk_norm_rope:
         from ..ops.rotary import qk_norm_rope_backward

@@ -538,3 +538,65 @@ def test_row_sums_of_the_call_in_front_are_not_read(shape, packed):
         for a, b in zip(alone, got):
             assert all(torch.equal(x, y) for x, y in zip(a, b))
     check_errors()
+
+
+def _kernel_nodes(run):
+    """How many kernels a call launches: the kernel nodes of its captured graph."""
+    from cuda.bindings import runtime as rt
+
+    run()
+    g = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(g):
+        run()
+    raw = rt.cudaGraph_t(init_value=g.raw_cuda_graph())
+    err, _nodes, n = rt.cudaGraphGetNodes(raw)
+    assert err == rt.cudaError_t.cudaSuccess
+    err, nodes, n = rt.cudaGraphGetNodes(raw, n)
+    assert err == rt.cudaError_t.cudaSuccess
+    kinds = [rt.cudaGraphNodeGetType(x) for x in nodes[:n]]
+    assert all(e == rt.cudaError_t.cudaSuccess for e, _k in kinds)
+    return sum(k == rt.cudaGraphNodeType.cudaGraphNodeTypeKernel for _e, k in kinds)
+
+
+@pytest.mark.parametrize("shape,docs", [((1, 128, 2, 64), None), ((1, 1024, 4, 64), None), ((1, 2048, 2, 64), None), ((2, 160, 4, 64), [0, 1, 100, 320])],
+                         ids=str)
+def test_launches_are_counted(shape, docs):
+    """What is reported as launched is what a captured call holds: whole, split (with sums or a join behind), packed."""
+    from pccl import build_kernels
+    from pccl.models import gpt
+    from pccl.ops.attention import attention_backward, attention_forward
+
+    C, (B, S, H, D) = build_kernels.load(), shape
+    q, k, v, dout = _inputs(B, S, S, H, H, D, BF, 80)
+    cu = None
+    if docs:
+        cu = torch.tensor(docs, dtype=torch.int32, device=DEV)
+        q, k, v, dout = (t.reshape(B * S, H, D) for t in (q, k, v, dout))
+    out, lse = attention_forward(q, k, v, cu_seqlens_q=cu)
+    counts = []
+    for run in (lambda: attention_forward(q, k, v, cu_seqlens_q=cu), lambda: attention_backward(dout, q, k, v, out, lse, cu_seqlens_q=cu)):
+        before = C.attention_kernels_launched()
+        run()
+        counts.append(C.attention_kernels_launched() - before)
+        assert counts[-1] == _kernel_nodes(run)
+    assert tuple(counts) == {128: (1, 3), 1024: (2, 3), 2048: (2, 6), 160: (2, 4)}[S]
+    # the same through a block: one more for the column sums of the projection's gradient, and with rotation one forward and two backward
+    keep = gpt.native_attention
+    try:
+        gpt.native_attention = True
+        for rope in (False, True):
+            if docs and not rope:
+                continue
+            cfg = gpt.GPTConfig(1, H * D, H, 64, vocab=8, seq_len=S, qk_norm_rope=rope)
+            pos = gpt.positions_of(cfg, B, S, DEV, None, cu) if rope else None
+            w = {n: torch.ones(D, device=DEV, dtype=BF) for n in ("qn_w", "kn_w")}
+            grads = {**{n: torch.empty_like(t) for n, t in w.items()}, "qkv_b": torch.empty(3 * H * D, device=DEV, dtype=BF)}
+            qkv = torch.randn(B * S, 3 * H * D, device=DEV).to(BF)
+            before = gpt.native_launches
+            a, saved = gpt._attention(qkv, w, cfg, B, pos)
+            assert gpt.native_launches - before == counts[0] + rope
+            before = gpt.native_launches
+            gpt._attention_backward(torch.randn_like(a), saved, w, grads, cfg, B, pos)
+            assert gpt.native_launches - before == counts[1] + 2 * rope + 1
+    finally:
+        gpt.native_attention = keep
