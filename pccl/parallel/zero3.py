@@ -121,8 +121,8 @@ class Zero3Engine:
         # GELU backward as the epilogue of the data-gradient GEMM of FC2 (needs native_gemm)
         self.fused_gelu_bwd_gemm = bool(fused_gelu_bwd_gemm) and self.native_gemm
         # the attention core on the library's kernels instead of scaled_dot_product_attention
-        if cfg.qk_norm_rope and cfg.head_dim % 8 != 0:
-            raise ValueError("qk_norm_rope wants a head size that is a multiple of 8")
+        if cfg.qk_norm_rope and (cfg.head_dim % 8 != 0 or cfg.head_dim > 256):
+            raise ValueError("qk_norm_rope wants a head size that is a multiple of 8 up to 256")
         self.native_attention = bool(native_attention) and gpt.native_attention_takes(cfg)
         self._rope_tables = None
         # both Adam moments in 32 bits, or in 8 with a scale for each 256 (pccl.ops.optim)

@@ -102,3 +102,12 @@ def test_8_bit_states_refuse_a_small_eps():
                 go(eps, bits)
     with pytest.raises(ValueError, match="eps of at least"):
         Zero3Engine(CFG, optim=OptimConfig(eps=1e-12), device=torch.device("cpu"), optim_bits=8)
+
+
+def test_engine_refuses_head_sizes_that_the_rotation_does_not_take():
+    from pccl.parallel.zero3 import Zero3Engine
+
+    for d_model in (4 * 12, 4 * 264, 4 * 512):
+        cfg = GPTConfig(1, d_model, 4, 64, vocab=8, seq_len=8, qk_norm_rope=True)
+        with pytest.raises(ValueError, match="multiple of 8 up to 256"):
+            Zero3Engine(cfg, device=torch.device("cpu"))
