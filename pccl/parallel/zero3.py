@@ -327,6 +327,8 @@ class Zero3Engine:
         if cu_seqlens is not None and (cu_seqlens.device != self.device or cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1
                                        or cu_seqlens.numel() < 2 or not cu_seqlens.is_contiguous()):
             raise ValueError("cu_seqlens must be a contiguous 1-D int32 tensor of at least two starts on the engine's device")
+        if cfg.qk_norm_rope and cu_seqlens is None and tokens.shape[1] > cfg.seq_len:
+            raise ValueError(f"sequences of {tokens.shape[1]} tokens have positions that the table of {cfg.seq_len} does not hold")
         if tokens.device.type != "cuda":
             if self._tokens_dev is None or self._tokens_dev.shape != tokens.shape:
                 self._tokens_dev = torch.empty(tokens.shape, dtype=torch.int64, device=self.device)

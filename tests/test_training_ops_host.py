@@ -111,3 +111,14 @@ def test_engine_refuses_head_sizes_that_the_rotation_does_not_take():
         cfg = GPTConfig(1, d_model, 4, 64, vocab=8, seq_len=8, qk_norm_rope=True)
         with pytest.raises(ValueError, match="multiple of 8 up to 256"):
             Zero3Engine(cfg, device=torch.device("cpu"))
+
+
+def test_engine_refuses_long_sequences_before_the_step_begins():
+    """With nothing of the step begun: the engine here has no more than its configuration."""
+    from pccl.parallel.zero3 import Zero3Engine
+
+    eng = Zero3Engine.__new__(Zero3Engine)
+    eng.cfg, eng.C, eng.native_attention, eng.device = ROPE, None, True, torch.device("cpu")
+    tokens = torch.zeros(2, 17, dtype=torch.int64)
+    with pytest.raises(ValueError, match="17 tokens have positions"):
+        eng.train_step(tokens, tokens)
