@@ -23,6 +23,7 @@ AdamW kernel over the whole shard, with global-norm clipping computed on the dev
 """
 from __future__ import annotations
 
+import warnings
 from dataclasses import dataclass
 from typing import Callable, Dict, List, Optional
 
@@ -124,6 +125,8 @@ class Zero3Engine:
         if cfg.qk_norm_rope and (cfg.head_dim % 8 != 0 or cfg.head_dim > 256):
             raise ValueError("qk_norm_rope wants a head size that is a multiple of 8 up to 256")
         self.native_attention = bool(native_attention) and gpt.native_attention_takes(cfg)
+        if native_attention and not self.native_attention:
+            warnings.warn(f"native_attention does not take heads of {cfg.head_dim} columns: attention stays with scaled_dot_product_attention")
         self._rope_tables = None
         # both Adam moments in 32 bits, or in 8 with a scale for each 256 (pccl.ops.optim)
         if optim_bits not in (8, 32):

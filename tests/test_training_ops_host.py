@@ -1,6 +1,7 @@
 """What the training operators do on the host: layouts, tables, positions, parameters, refusals."""
 import dataclasses
 import math
+import warnings
 
 import pytest
 import torch
@@ -122,3 +123,21 @@ def test_engine_refuses_long_sequences_before_the_step_begins():
     tokens = torch.zeros(2, 17, dtype=torch.int64)
     with pytest.raises(ValueError, match="17 tokens have positions"):
         eng.train_step(tokens, tokens)
+
+
+def test_engine_says_where_native_attention_does_not_take_a_head_size():
+    from pccl.parallel.zero3 import Zero3Engine
+
+    def build(d):
+        try:
+            Zero3Engine(GPTConfig(1, 4 * d, 4, 64, vocab=8, seq_len=8), device=torch.device("cpu"), native_attention=True)
+        except Exception:           # noqa: BLE001  (the engine wants a GPU, later on)
+            pass
+
+    for d in (12, 136):
+        with pytest.warns(UserWarning, match=f"heads of {d} columns"):
+            build(d)
+    with warnings.catch_warnings(record=True) as said:
+        warnings.simplefilter("always")
+        build(64)
+    assert not [w for w in said if "native_attention" in str(w.message)]
