@@ -41,7 +41,7 @@ RotaryTensor view(const at::Tensor& t, const char* name, const at::Tensor& q, co
 }
 
 // An output: the caller's tensor, which may be exactly one of its own inputs (a row is read before it is written) but shares nothing
-// with those of the other heads, or a new one.
+// with those of the other heads nor with what every row reads (weights, tables, positions), or a new one.
 at::Tensor output(const std::optional<at::Tensor>& given, const at::Tensor& like, const char* name, std::initializer_list<at::Tensor> own,
                   std::initializer_list<at::Tensor> others) {
   if (!given.has_value()) return fresh(like.sizes(), like.scalar_type(), like);
@@ -49,6 +49,11 @@ at::Tensor output(const std::optional<at::Tensor>& given, const at::Tensor& like
   for (const at::Tensor& t : own) TORCH_CHECK(share(*given, t) != Share::kSome, name, " must not partly overlap an input");
   for (const at::Tensor& t : others) TORCH_CHECK(share(*given, t) == Share::kNone, name, " must not overlap an input of the other heads");
   return *given;
+}
+// The weights, tables and positions of a call beside an output that the caller gave.
+void check_apart(const at::Tensor& out, const char* name, std::initializer_list<at::Tensor> shared, const std::optional<at::Tensor>& positions) {
+  for (const at::Tensor& t : shared) TORCH_CHECK(share(out, t) == Share::kNone, name, " must not overlap the weights or the tables");
+  TORCH_CHECK(!positions.has_value() || share(out, *positions) == Share::kNone, name, " must not overlap the positions");
 }
 
 Shape fill(RotaryArgs& a, const at::Tensor& q, const at::Tensor& k, const at::Tensor& qw, const at::Tensor& kw, const at::Tensor& cos,
@@ -114,6 +119,8 @@ std::tuple<at::Tensor, at::Tensor> qk_norm_rope_forward(const at::Tensor& q, con
   c10::cuda::CUDAGuard guard(q.device());
   at::Tensor qo = output(q_out, q, "q_out", {q}, {k}), ko = output(k_out, k, "k_out", {k}, {q});
   TORCH_CHECK(share(qo, ko) == Share::kNone, "q_out and k_out must not overlap");
+  if (q_out.has_value()) check_apart(qo, "q_out", {qw, kw, cos, sin}, positions);
+  if (k_out.has_value()) check_apart(ko, "k_out", {qw, kw, cos, sin}, positions);
   a.y[0] = view(qo, "q_out", q, s, a.H[0]);
   a.y[1] = view(ko, "k_out", q, s, a.H[1]);
   if (s.B * s.S == 0 || a.H[0] + a.H[1] == 0) return {qo, ko};
@@ -133,6 +140,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> qk_norm_rope_backward
   a.dy[1] = view(dk, "dk", q, s, a.H[1]);
   at::Tensor qo = output(dq_in, q, "dq_in", {dq, q}, {dk, k}), ko = output(dk_in, k, "dk_in", {dk, k}, {dq, q});
   TORCH_CHECK(share(qo, ko) == Share::kNone, "dq_in and dk_in must not overlap");
+  if (dq_in.has_value()) check_apart(qo, "dq_in", {qw, kw, cos, sin}, positions);
+  if (dk_in.has_value()) check_apart(ko, "dk_in", {qw, kw, cos, sin}, positions);
   a.y[0] = view(qo, "dq_in", q, s, a.H[0]);
   a.y[1] = view(ko, "dk_in", q, s, a.H[1]);
   at::Tensor dqw = dqw_.has_value() ? *dqw_ : fresh(qw.sizes(), qw.scalar_type(), q), dkw = dkw_.has_value() ? *dkw_ : fresh(kw.sizes(), kw.scalar_type(), q);
@@ -141,6 +150,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> qk_norm_rope_backward
                     w->scalar_type() == qw.scalar_type(),
                 "dq_weight and dk_weight must look like the weights");
   TORCH_CHECK(share(dqw, dkw) == Share::kNone, "dq_weight and dk_weight must not overlap");
+  for (const at::Tensor* w : {&dqw, &dkw})
+    TORCH_CHECK(share(*w, qo) == Share::kNone && share(*w, ko) == Share::kNone, "dq_weight and dk_weight must not overlap dq_in or dk_in");
   a.dw[0] = dqw.data_ptr();
   a.dw[1] = dkw.data_ptr();
   if (s.B * s.S == 0 || a.H[0] + a.H[1] == 0) {

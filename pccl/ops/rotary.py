@@ -13,8 +13,9 @@ A pair is columns (i, i + rot / 2), or (2i, 2i + 1) with ``interleaved``; the re
 of a multiple of 8 up to 256 (views into a packed projection are read where they lie: 16-byte boundaries, strides that are
 multiples of 8 elements).  Weights are of that type or fp32.  ``cos`` and ``sin`` are fp32 tables, ``[positions, rot / 2]``
 (``rotary_table``).  ``positions``, one for each row, int32 or int64 on the device, says where in the table a row stands;
-without it that is the row's number.  A position that the table does not hold makes its row NaN.  These are plain functions
-like those of ``pccl.ops.gemm``: they record nothing for autograd.
+without it that is the row's number.  A position that the table does not hold makes its row NaN.  An output may be exactly the
+input that it comes from and overlaps nothing else of the call.  These are plain functions like those of ``pccl.ops.gemm``:
+they record nothing for autograd.
 """
 from __future__ import annotations
 

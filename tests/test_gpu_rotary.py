@@ -247,3 +247,33 @@ def test_offsets_beyond_32_bits():
     assert all(torch.equal(a, b) for a, b in zip(got, grad))
     got = qk_norm_rope_forward(cut(0), cut(128), w, w, *tab, q_out=cut(0), k_out=cut(128))
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_outputs_apart_from_weights_tables_and_positions():
+    """What every row reads must not be written by any: such calls are refused."""
+    from pccl.ops.rotary import qk_norm_rope_backward, qk_norm_rope_forward, rotary_table
+
+    S = 24
+    pool = torch.zeros(1 << 16, device=DEV, dtype=torch.uint8)
+    at = lambda i, n, dt: pool[i:i + n * dt.itemsize].view(dt)                              # noqa: E731
+    q, k = (torch.randn(S, 2, 64, device=DEV).to(BF) for _ in range(2))
+    w, (cos, sin) = torch.ones(64, device=DEV, dtype=BF), rotary_table(S, 64, device=DEV)
+    out = at(0, S * 2 * 64, BF).view(S, 2, 64)                                              # the pool's first 6144 bytes
+    pw, pc, pp = at(6016, 64, BF), at(3200, S * 32, torch.float32).view(S, 32), at(6080, S, torch.int64)
+    pw.fill_(1.0)
+    args = lambda **new: [{"qw": w, "kw": w, "cos": cos, "sin": sin, **new}[n] for n in ("qw", "kw", "cos", "sin")]  # noqa: E731
+    for name in ("q", "k"):
+        for new, pos in ((dict(qw=pw), None), (dict(kw=pw), None), (dict(cos=pc), None), (dict(sin=pc), None), ({}, pp)):
+            with pytest.raises(RuntimeError, match="overlap the"):
+                qk_norm_rope_forward(q, k, *args(**new), positions=pos, **{name + "_out": out})
+            with pytest.raises(RuntimeError, match="overlap the"):
+                qk_norm_rope_backward(q, k, q, k, *args(**new), positions=pos, **{f"d{name}_in": out})
+        for weight in ("dq_weight", "dk_weight"):
+            with pytest.raises(RuntimeError, match="overlap dq_in or dk_in"):
+                qk_norm_rope_backward(q, k, q, k, *args(), **{f"d{name}_in": out, weight: pw})
+    # beside the pool's first bytes all of that is taken, and a weight's gradient may take the weight's place
+    far = at(8192, 64, BF)
+    far.fill_(1.0)
+    want = qk_norm_rope_backward(q, k, q, k, *args())
+    got = qk_norm_rope_backward(q, k, q, k, *args(qw=far), dq_in=out, dq_weight=far)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
