@@ -125,10 +125,13 @@ Shape fill(AttnArgs& a, const at::Tensor& q, const at::Tensor& k, const at::Tens
 }
 
 // An output: the caller's tensor, or a new one.
-at::Tensor output(const std::optional<at::Tensor>& given, const at::Tensor& like, const char* name, std::initializer_list<at::Tensor> inputs) {
+at::Tensor output(const std::optional<at::Tensor>& given, const at::Tensor& like, const char* name, std::initializer_list<at::Tensor> inputs,
+                  const std::optional<at::Tensor>& cu_q, const std::optional<at::Tensor>& cu_k) {
   if (!given.has_value()) return fresh(like.sizes(), like.scalar_type(), like);
   TORCH_CHECK(distinct(*given), name, " must not overlap itself");
   for (const at::Tensor& t : inputs) TORCH_CHECK(share(*given, t) == Share::kNone, name, " must not overlap an input");
+  for (const std::optional<at::Tensor>* t : {&cu_q, &cu_k})
+    TORCH_CHECK(!t->has_value() || share(*given, **t) == Share::kNone, name, " must not overlap the starts of the sequences");
   return *given;
 }
 
@@ -138,7 +141,7 @@ std::tuple<at::Tensor, at::Tensor> attention_forward(const at::Tensor& q, const 
   AttnArgs a;
   const Shape s = fill(a, q, k, v, causal, scale, cu_q, cu_k);
   c10::cuda::CUDAGuard guard(q.device());
-  at::Tensor out = output(out_, q, "out", {q, k, v});
+  at::Tensor out = output(out_, q, "out", {q, k, v}, cu_q, cu_k);
   a.o = view(out, "out", q, s.B, s.Sq, s.H, s.D);
   at::Tensor lse = s.packed ? fresh({s.H, s.Sq}, at::kFloat, q) : fresh({s.B, s.H, s.Sq}, at::kFloat, q);
   a.lse = lse.data_ptr<float>();
@@ -178,7 +181,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_backward(const at::Tens
               "lse must be what the forward pass returned");
   TORCH_CHECK(dq_.has_value() == dk_.has_value() && dq_.has_value() == dv_.has_value(), "dq, dk and dv are given together or not at all");
   const std::initializer_list<at::Tensor> inputs = {dout, q, k, v, out, lse};
-  at::Tensor dq = output(dq_, q, "dq", inputs), dk = output(dk_, k, "dk", inputs), dv = output(dv_, v, "dv", inputs);
+  at::Tensor dq = output(dq_, q, "dq", inputs, cu_q, cu_k), dk = output(dk_, k, "dk", inputs, cu_q, cu_k),
+             dv = output(dv_, v, "dv", inputs, cu_q, cu_k);
   TORCH_CHECK(share(dq, dk) == Share::kNone && share(dq, dv) == Share::kNone && share(dk, dv) == Share::kNone,
               "dq, dk and dv must not overlap each other");
   TORCH_CHECK(s.B <= 65535, "the backward pass takes up to 65535 batch entries");

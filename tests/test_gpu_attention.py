@@ -600,3 +600,25 @@ def test_launches_are_counted(shape, docs):
             assert gpt.native_launches - before == counts[1] + 2 * rope + 1
     finally:
         gpt.native_attention = keep
+
+
+def test_outputs_apart_from_the_starts():
+    """Every block reads the starts, so none may write them: such calls are refused."""
+    from pccl.ops.attention import attention_backward, attention_forward
+
+    q, k, v, dout = (t[0] for t in _inputs(1, 40, 40, 2, 2, 64, BF, 90))
+    pool = torch.zeros(1 << 15, device=DEV, dtype=torch.uint8)
+    new = pool[:40 * 2 * 64 * 2].view(BF).view(40, 2, 64)
+    starts = pool[5120:5128].view(torch.int32)
+    starts.copy_(torch.tensor([0, 40]))
+    apart = starts.clone()
+    out, lse = attention_forward(q, k, v, cu_seqlens_q=apart)
+    for cu in (dict(cu_seqlens_q=starts), dict(cu_seqlens_q=apart, cu_seqlens_k=starts)):
+        with pytest.raises(RuntimeError, match="overlap the starts"):
+            attention_forward(q, k, v, out=new, **cu)
+        for which in range(3):
+            grads = [torch.empty_like(t) for t in (q, k, v)]
+            grads[which] = new
+            with pytest.raises(RuntimeError, match="overlap the starts"):
+                attention_backward(dout, q, k, v, out, lse, dq=grads[0], dk=grads[1], dv=grads[2], **cu)
+    assert torch.equal(attention_forward(q, k, v, cu_seqlens_q=apart, out=new)[0], out)
