@@ -69,6 +69,7 @@ void adamw_multi(const std::vector<at::Tensor>& params, const std::vector<at::Te
   TORCH_CHECK(step >= 1, "step counts from 1");
   TORCH_CHECK(std::isfinite(lr) && beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1 && eps >= 0 && std::isfinite(eps),
               "lr and eps must be finite, eps not negative, beta1 and beta2 in [0, 1)");
+  TORCH_CHECK(!std::isnan(max_grad_norm), "max_grad_norm must be a number: NaN would switch clipping off");
   TORCH_CHECK(!(m_scale.has_value() || v_scale.has_value()) || eps >= adamw_least_eps(beta2), "8-bit states need an eps of at least ",
               adamw_least_eps(beta2), " at this beta2: they hold second moments below 2^-80 as zeros");
   if (n == 0) return;

@@ -141,3 +141,13 @@ def test_engine_says_where_native_attention_does_not_take_a_head_size():
         warnings.simplefilter("always")
         build(64)
     assert not [w for w in said if "native_attention" in str(w.message)]
+
+
+def test_a_largest_norm_that_is_nan_is_refused():
+    p = [torch.zeros(300)]
+    go = lambda most: adamw_step(p, p, adamw_state(p), step=1, lr=1e-3, max_grad_norm=most, total_sq_norm=torch.zeros(1))      # noqa: E731
+    with pytest.raises(RuntimeError, match="max_grad_norm must be a number"):
+        go(math.nan)
+    for most in (-1.0, 0.0, 1.0, math.inf):
+        with pytest.raises(RuntimeError, match="CUDA"):                            # taken, but for where the tensors lie
+            go(most)
