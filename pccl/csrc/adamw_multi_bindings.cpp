@@ -82,7 +82,7 @@ void adamw_multi(const std::vector<at::Tensor>& params, const std::vector<at::Te
   std::vector<Range> ranges;
   table.reserve(n);
   blocks.reserve(n);
-  ranges.reserve(3 * n + 4);
+  ranges.reserve(3 * n + 5);
   uint64_t total = 0;
   for (size_t i = 0; i < n; ++i) {
     const at::Tensor &p = params[i], &g = grads[i];
@@ -114,7 +114,13 @@ void adamw_multi(const std::vector<at::Tensor>& params, const std::vector<at::Te
   }
   TORCH_CHECK(total * kAdamBlock == (uint64_t)m.numel(), "the states hold ", m.numel(), " elements, these parameters need ", total * kAdamBlock);
   TORCH_CHECK(total < ((uint64_t)1 << 32), "too many parameters for one call");
-  // two blocks of the grid that update the same memory would race
+  if (max_grad_norm > 0) {
+    TORCH_CHECK(total_sq_norm.has_value(), "max_grad_norm needs total_sq_norm");
+    TORCH_CHECK(total_sq_norm->device() == device && total_sq_norm->scalar_type() == at::kFloat && total_sq_norm->numel() == 1,
+                "total_sq_norm must hold one float32 on the device of the parameters");
+    add_range(ranges, *total_sq_norm, false);
+  }
+  // two blocks of the grid that update the same memory would race, and every block reads the norm
   for (const at::Tensor* t : {static_cast<const at::Tensor*>(&m), static_cast<const at::Tensor*>(&v)}) add_range(ranges, *t, true);
   if (bits8) {
     add_range(ranges, *m_scale, true);
@@ -143,13 +149,7 @@ void adamw_multi(const std::vector<at::Tensor>& params, const std::vector<at::Te
   a.bias2 = (float)(1.0 / (1.0 - std::pow(beta2, (double)step)));
   a.grad_scale = (float)grad_scale;
   a.max_grad_norm = (float)max_grad_norm;
-  a.total_sq_norm = nullptr;
-  if (max_grad_norm > 0) {
-    TORCH_CHECK(total_sq_norm.has_value(), "max_grad_norm needs total_sq_norm");
-    TORCH_CHECK(total_sq_norm->device() == device && total_sq_norm->scalar_type() == at::kFloat && total_sq_norm->numel() == 1,
-                "total_sq_norm must hold one float32 on the device of the parameters");
-    a.total_sq_norm = total_sq_norm->data_ptr<float>();
-  }
+  a.total_sq_norm = max_grad_norm > 0 ? total_sq_norm->data_ptr<float>() : nullptr;
   c10::cuda::CUDAGuard guard(device);
   const cudaStream_t stream = at::cuda::getCurrentCUDAStream().stream();
   const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;

@@ -324,3 +324,18 @@ def test_second_moments_held_as_zeros_do_not_count(beta2):
         a, b = -p8.double(), -p32.double()
         assert torch.all(a >= b * (1 - slack * step) - least) and torch.all(a <= b * (33 / 32 + slack * step) + least), step
     assert torch.all(s8.dequantize()[1] <= s32.exp_avg_sq * (1 + 2.0 ** -10))
+
+
+def test_a_norm_inside_what_the_step_writes_is_refused():
+    from pccl.ops.optim import adamw_state, adamw_step
+
+    p, g = torch.ones(300, device=DEV), torch.ones(300, device=DEV)
+    for bits in (8, 32):
+        st = adamw_state([p], bits)
+        inside = [p[7:8], st.exp_avg_scale[:1] if bits == 8 else st.exp_avg[255:256], st.exp_avg_sq_scale[1:] if bits == 8 else st.exp_avg_sq[-1:]]
+        for norm in inside:
+            with pytest.raises(RuntimeError, match="overlaps another one"):
+                adamw_step([p], [g], st, step=1, max_grad_norm=1.0, total_sq_norm=norm, **HYPER)
+            assert torch.all(p == 1)
+        adamw_step([p.clone()], [g], st, step=1, max_grad_norm=1.0, total_sq_norm=g[:1], **HYPER)       # a gradient is only read
+        adamw_step([p.clone()], [g], st, step=1, total_sq_norm=p[:1], **HYPER)                         # not read without clipping
