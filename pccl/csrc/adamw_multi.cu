@@ -510,7 +510,7 @@ cudaError_t launch_grad(const AdamMultiArgs& a, const AdamTensor* t, int count, 
 
 double adamw_least_eps(double beta2) { return ldexp(1.0, -35) / sqrt(1.0 - beta2); }
 
-uint32_t adamw_noise_key(uint64_t seed, int64_t step) { return mix(mix((uint32_t)seed) + (uint32_t)step); }
+uint32_t adamw_noise_key(uint64_t seed, int64_t step) { return mix(mix((uint32_t)seed ^ mix((uint32_t)(seed >> 32))) + (uint32_t)step); }
 
 cudaError_t launch_adamw_multi(const AdamMultiArgs& a, const AdamTensor* tensors, int count, int pt, int gt, bool bits8, int sm_count,
                                cudaStream_t s) {

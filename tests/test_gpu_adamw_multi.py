@@ -339,3 +339,15 @@ def test_a_norm_inside_what_the_step_writes_is_refused():
             assert torch.all(p == 1)
         adamw_step([p.clone()], [g], st, step=1, max_grad_norm=1.0, total_sq_norm=g[:1], **HYPER)       # a gradient is only read
         adamw_step([p.clone()], [g], st, step=1, total_sq_norm=p[:1], **HYPER)                         # not read without clipping
+
+
+def test_all_64_bits_of_the_seed_count():
+    from pccl.ops.optim import adamw_state, adamw_step
+
+    grad = torch.randn(256 * 40, device=DEV, generator=torch.Generator(device=DEV).manual_seed(9))
+    codes = []
+    for seed in (3, 3 + (1 << 32), 3 + (5 << 40), (1 << 64) - 1, (1 << 32) - 1):
+        state = adamw_state([grad], 8)
+        adamw_step([torch.zeros_like(grad)], [grad], state, step=1, seed=seed, **HYPER)
+        codes.append(torch.cat((state.exp_avg.int(), state.exp_avg_sq.int())))
+    assert all(not torch.equal(a, b) for i, a in enumerate(codes) for b in codes[:i])
