@@ -351,3 +351,30 @@ def test_all_64_bits_of_the_seed_count():
         adamw_step([torch.zeros_like(grad)], [grad], state, step=1, seed=seed, **HYPER)
         codes.append(torch.cat((state.exp_avg.int(), state.exp_avg_sq.int())))
     assert all(not torch.equal(a, b) for i, a in enumerate(codes) for b in codes[:i])
+
+
+def test_8_bit_lists_of_several_launches_against_32_bits():
+    """A list of more tensors than a launch takes, and one that needs the long table: scales are the block maxima of a 32-bit step from
+    the moments that the codes stood for, codes the neighbours of its moments, parameters its bits; the second step reads codes."""
+    from pccl.ops.optim import adamw_state, adamw_step
+
+    for sizes in ([257 + 3 * i for i in range(1700)], [1 + 5 * i for i in range(200)]):
+        params, grads, masters = _lists(sizes, BF, BF, 10)
+        decay = [0.01 * (i % 7) for i in range(len(sizes))]
+        state, full = adamw_state(params, 8), adamw_state(params, 32)
+        for step in (1, 2, 3):
+            for x, y in zip((full.exp_avg, full.exp_avg_sq), state.dequantize()):
+                x.copy_(y)
+            copies = [[t.clone() for t in x] for x in (params, masters)]
+            adamw_step(copies[0], grads, full, step=step, masters=copies[1], weight_decay=decay, **HYPER)
+            adamw_step(params, grads, state, step=step, masters=masters, weight_decay=decay, seed=step, **HYPER)
+            assert all(torch.equal(a, b) for x, y in zip((params, masters), copies) for a, b in zip(x, y))
+            for x, code, scale, top, power in ((full.exp_avg, state.exp_avg, state.exp_avg_scale, 127, 2),
+                                               (full.exp_avg_sq, state.exp_avg_sq, state.exp_avg_sq_scale, 255, 4)):
+                x, c = x.view(-1, 256).double(), code.view(-1, 256).double()
+                assert torch.equal(scale, x.abs().amax(1).float())
+                y = x.abs() / scale.double()[:, None].clamp(min=1e-300) * top ** power
+                # 1e-5: the 32-bit roundings of y
+                assert torch.all(c.abs() ** power <= ((y * (1 + 1e-5)) ** (1 / power) + 1) ** power)
+                assert torch.all((c.abs() + 1) ** power >= y * (1 - 1e-5))
+                assert torch.all((c == 0) | (torch.sign(c) == torch.sign(x)))

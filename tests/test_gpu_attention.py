@@ -622,3 +622,53 @@ def test_outputs_apart_from_the_starts():
             with pytest.raises(RuntimeError, match="overlap the starts"):
                 attention_backward(dout, q, k, v, out, lse, dq=grads[0], dk=grads[1], dv=grads[2], **cu)
     assert torch.equal(attention_forward(q, k, v, cu_seqlens_q=apart, out=new)[0], out)
+
+
+@pytest.mark.parametrize("poison", [0.0, math.nan])
+@pytest.mark.parametrize("case", PACKED, ids=str)
+def test_packed_sequences_in_fp16(case, poison, monkeypatch):
+    import sys
+
+    monkeypatch.setattr(sys.modules[__name__], "BF", FP)
+    test_packed_sequences_stay_apart(case, poison)
+
+
+@pytest.mark.parametrize("case", [([(2048, 2048)], 0, 16, 1, 64, True), ([(3, 2500), (129, 2200)], 5, 4, 1, 80, True), ([(1, 4000)], 0, 4, 2, 128, False)], ids=str)
+def test_packed_calls_of_shapes_that_are_split_when_they_are_not(case):
+    test_packed_sequences_stay_apart(case, 0.0)
+
+
+@pytest.mark.parametrize("case", [(1, 1500, 1100, 4, 1, 64, True, BF), (1, 2500, 2100, 2, 1, 64, True, FP), (2, 1300, 1024, 2, 2, 128, True, BF)], ids=str)
+def test_more_queries_than_keys_where_the_axes_are_split(case):
+    """The first queries see nothing, in any part."""
+    test_forward_matches_formula(case)
+    test_backward_matches_formula(case)
+
+
+def test_captured_packed_call_follows_the_starts():
+    """The starts are read on the device: a replay takes those that are there then."""
+    from pccl.ops.attention import attention_backward, attention_forward, check_errors
+
+    q, k, v, dout = (t[0].contiguous() for t in _inputs(1, 500, 500, 4, 2, 64, BF, 70))
+    cu = torch.tensor([0, 100, 300, 500], dtype=torch.int32, device=DEV)
+
+    def run():
+        out, lse = attention_forward(q, k, v, cu_seqlens_q=cu)
+        return out, lse, *attention_backward(dout, q, k, v, out, lse, cu_seqlens_q=cu)
+
+    run()
+    graphs = []
+    for _ in range(2):                  # two graphs that are replayed in turn share nothing
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got = run()
+        graphs.append((g, got))
+    for starts in ([0, 100, 300, 500], [0, 1, 1, 490], [0, 500, 500, 500], [0, 0, 0, 0], [0, 257, 258, 499]):
+        cu.copy_(torch.tensor(starts))
+        want = run()
+        for g, got in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for g, got in graphs:
+            assert all(torch.equal(a, b) for a, b in zip(want, got)), starts
+    check_errors()

@@ -663,3 +663,124 @@ def test_engine_with_8_bit_moments_steps_and_resumes():
     with pytest.raises(ValueError):
         Zero3Engine(GPTConfig(1, 256, 4, 512, vocab=512, seq_len=128), TorchBackend()).train_step(
             toks[0][:, :-1], toks[0][:, 1:], torch.tensor([0, 256], dtype=torch.int32, device=DEV))
+
+
+def _rope_engine(**kw):
+    from pccl.models.gpt import GPTConfig
+    from pccl.parallel.backend import TorchBackend
+    from pccl.parallel.zero3 import OptimConfig, Zero3Engine
+
+    cfg = GPTConfig(2, 256, 4, 512, vocab=512, seq_len=128, qk_norm_rope=True)
+    optim = OptimConfig(lr=1e-3, max_grad_norm=kw.pop("max_grad_norm", 1.0))
+    return Zero3Engine(cfg, TorchBackend(), optim, native_gemm=True, native_attention=True, **kw)
+
+
+def _distinct_tokens(seed):
+    """No token twice: each row of the embedding's gradient is added to once, so no order of additions can change its bits."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return torch.randperm(512, device=DEV, generator=g)[:256].view(2, 128), torch.randint(0, 512, (2, 128), device=DEV, generator=g)
+
+
+def test_engine_with_8_bit_moments_steps_by_the_formula():
+    """The first step is the 32-bit engine's; every later one is a 32-bit step from the moments that the codes stand for, bit for bit, and
+    the new codes are the neighbours of its moments."""
+    from pccl.ops.optim import adamw_state, adamw_step
+
+    a, full = _rope_engine(optim_bits=8), _rope_engine()
+    o = a.optim
+    for step in (1, 2, 3):
+        tokens, targets = _distinct_tokens(20 + step)
+        m, v = (x.clone() for x in a.adam8.dequantize())
+        start, param = a.master.clone(), a.param_shard.clone()
+        a.train_step(tokens, targets)
+        assert a.step_count == step and float((a.master - start).abs().max()) > 0.1 * o.lr
+        if step == 1:
+            full.train_step(tokens, targets)
+            assert torch.equal(a.grad_shard, full.grad_shard)
+            # Two kernels, two orders of rounding.  The update is lr at most.  Its factors differ by 1 - beta in 32 bits (2.4e-7: two steps
+            # of 2^-23 in m, one in the root), two dozen roundings, and the clip factor's sum of squares, whose order is free (16 in its root)
+            bound = 2.0 ** -22 * start.abs() + 48 * 2.0 ** -23 * o.lr
+            assert torch.all((a.master - full.master).abs() <= bound)
+        ref = adamw_state([start], 32)
+        ref.exp_avg.copy_(m)
+        ref.exp_avg_sq.copy_(v)
+        adamw_step([param], [a.grad_shard], ref, step=step, lr=o.lr, beta1=o.beta1, beta2=o.beta2, eps=o.eps, weight_decay=o.weight_decay,
+                   masters=[start], max_grad_norm=o.max_grad_norm, total_sq_norm=a.sq_norm)
+        assert torch.equal(a.master, start) and torch.equal(a.param_shard, param)
+        for x, code, scale, top, power in ((ref.exp_avg, a.adam8.exp_avg, a.adam8.exp_avg_scale, 127, 2),
+                                           (ref.exp_avg_sq, a.adam8.exp_avg_sq, a.adam8.exp_avg_sq_scale, 255, 4)):
+            x, c = x.view(-1, 256).double(), code.view(-1, 256).double()
+            most = x.abs().amax(1)
+            kept = most >= 2.0 ** -80
+            assert torch.equal(scale, torch.where(kept, most, 0.0).float())
+            y = (x.abs() / most[:, None].clamp(min=1e-300) * top ** power)[kept]
+            c, x = c[kept], x[kept]
+            # a code is the one below or above; 1e-5: the 32-bit roundings of y
+            assert torch.all(c.abs() ** power <= ((y * (1 + 1e-5)) ** (1 / power) + 1) ** power)
+            assert torch.all((c.abs() + 1) ** power >= y * (1 - 1e-5))
+            assert torch.all((c == 0) | (torch.sign(c) == torch.sign(x)))
+    a.check_errors()
+
+
+def test_engine_with_8_bit_moments_resumes_bit_for_bit():
+    # no clipping: the order of the norm's sum is free
+    a, b = (_rope_engine(optim_bits=8, max_grad_norm=0.0, seed=s) for s in (1, 2))
+    for i in range(2):
+        a.train_step(*_distinct_tokens(30 + i))
+    sd = {k: v.clone() for k, v in a.state_dict().items()}
+    assert not torch.equal(a.master, b.master)
+    b.load_state_dict(sd)
+    for i in range(3):
+        own, other = a.state_dict(), b.state_dict()
+        assert set(own) == {"master", "step", "world", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale"} == set(other)
+        for name in own:
+            assert torch.equal(own[name], other[name]), (i, name)
+        assert torch.equal(a.param_shard, b.param_shard) and int(own["step"]) == 2 + i
+        for e in (a, b):
+            e.train_step(*_distinct_tokens(40 + i))
+        assert torch.equal(a.grad_shard, b.grad_shard)
+
+
+def test_engine_with_tokens_behind_the_last_document(monkeypatch):
+    """Such tokens see nothing, their attention is zero; everything else of the model works on them.  Bounds as for the packed case above."""
+    from pccl.models.gpt import GPTConfig
+    from pccl.parallel.backend import TorchBackend
+    from pccl.parallel.zero3 import OptimConfig, Zero3Engine
+
+    cfg = GPTConfig(2, 256, 4, 512, vocab=512, seq_len=160, init_std=0.08, qk_norm_rope=True)
+    eng = Zero3Engine(cfg, TorchBackend(), OptimConfig(lr=0.0, max_grad_norm=0.0), native_gemm=True, native_attention=True)
+    g = torch.Generator(device=DEV).manual_seed(3)
+    tok = torch.randint(0, cfg.vocab, (2, 161), device=DEV, generator=g)
+    cu = torch.tensor([0, 1, 100, 100, 191], dtype=torch.int32, device=DEV)
+    i = torch.arange(320, device=DEV)
+    which = (i[:, None] >= cu[None, 1:]).sum(1)
+    place = (i - cu.long()[which]) % 160
+    which = which.double().masked_fill(which == 4, math.nan)                      # not even equal to itself: sees nothing
+    softmax = torch.softmax
+
+    def of_what_is_seen(s, dim):
+        any_ = (s > -math.inf).any(dim, keepdim=True)
+        return softmax(s.masked_fill(~any_, 0.0), dim) * any_
+
+    params = [{k: v.clone() for k, v in u[0].items()} for u in eng.pviews]
+    loss = eng.train_step(tok[:, :-1], tok[:, 1:], cu)
+    eng.check_errors()
+    monkeypatch.setattr(torch, "softmax", of_what_is_seen)
+    want, grads = _plain_step(cfg, params, tok[:, :-1], tok[:, 1:], (which, place))
+    assert abs(float(loss) - float(want)) <= 2e-2 * float(want)
+    for gv, ref in zip([eng.gviews0] + [u[0] for u in eng.gviews[1:]], grads):
+        for name, r in ref.items():
+            rel = float((gv[name].double() - r).norm() / r.norm().clamp(min=1e-12))
+            assert rel <= 0.04, (name, rel)
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_native_attention_beside_weight_gradients_on_a_second_stream(packed):
+    """The same bits as on one stream, over steps that reuse the memory."""
+    one, two = _rope_engine(max_grad_norm=0.0, optim_bits=8), _rope_engine(max_grad_norm=0.0, optim_bits=8, overlap_wgrad=True)
+    cu = torch.tensor([0, 1, 100, 230, 250], dtype=torch.int32, device=DEV) if packed else None
+    for i in range(4):
+        for e in (one, two):
+            e.train_step(*_distinct_tokens(50 + i), cu)
+        assert torch.equal(one.grad_shard, two.grad_shard) and torch.equal(one.master, two.master), i
+    two.check_errors()
