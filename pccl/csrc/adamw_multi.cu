@@ -10,7 +10,8 @@
 //
 // What bounds it.  308 million parameters: with states in 32 bits 1382 us, 6.24 TB/s (0.95 of the measured copy rate); tensors off
 // vector boundaries 1402.  With three blocks on an SM, more loads on their way, 1404; with four 1590.  In 8 bits 955 us, 5.16 TB/s: the
-// codes cost about 80 instructions for each element, and the issue slots are three quarters full; misaligned 1277.  Reading the
+// codes cost about 80 instructions for each element, and the issue slots are three quarters full; misaligned 1277: as full, DRAM at 42 %
+// instead of 57 %, a third more instructions for accesses of one element and the exchange between lanes.  Reading the
 // states back (adamw_dequantize) 458 us, 6.72 TB/s.
 //
 // 8-bit states.  A block keeps the size A of its largest value in 32 bits and a code c per element:

@@ -19,10 +19,10 @@
 // dq: S = Q K^T and dP = dO V^T as in the forward pass, dq += dS K; S is kept twice, so that its next tile is ready when the
 // exponentials of the last one are done.
 //
-// What bounds it.  4 x 2048 x 16 heads of 128 causal take 250 us, 687 TFLOP/s by the five products that the formulas need and 960
-// by the seven computed: row sums 10 us (6.4 TB/s), dk and dv 132, dq 103.  With the exponentials and conversions left out the
-// products alone take 110 and 87, 1330 and 1260 TFLOP/s, at heads of 64 81 instead of 110 for dk and dv; without the loads of query tiles
-// the whole takes 249.  A product of 128 x 128 x 16 takes 64.6 cycles, with 64 columns 32.5 (48.5 with both operands in shared memory),
+// What bounds it.  4 x 2048 x 16 heads of 128 causal take 250 us in runs of some 30 calls (302 on a card that has been busy for seconds,
+// whose clock is lower), 687 TFLOP/s by the five products that the formulas need and 960 by the seven computed: row sums 10 us (6.4 TB/s),
+// dk and dv 132, dq 103.  With the exponentials and conversions left out the products alone take 110 and 87, 1330 and 1260 TFLOP/s, at
+// heads of 64 81 instead of 110 for dk and dv; without the loads of query tiles the whole takes 249.  A product of 128 x 128 x 16 takes 64.6 cycles, with 64 columns 32.5 (48.5 with both operands in shared memory),
 // so the four of a step need 2070 cycles, at heads of 64 1040; with the conversions left out a step still takes 3200 and 2400.  So most
 // of the rest is the hand-over between warps at every tile, and the start and end of each walk, here of 8.5 steps on average.
 // Sixteen compute warps for eight: 253, at heads of 64 197 instead of 201; a second tile of scores at heads of 64: 199.  The

@@ -17,11 +17,13 @@
 // multiply-add units as a polynomial made it slower (928 us).  The chain product - maximum - exponentials - product is, and
 // the clock, which the power limit takes down to 1.69 GHz.
 // Shorter sequences pay for the start and the end of each tile: 4 x 2048 x 16 heads of 128 causal 82 us (838 TFLOP/s), 63
-// without softmax; heads of 64 69 us.  The grid's tiles are taken over at run time (attention.cuh), so that the loads of the next
+// without softmax; heads of 64 69 us.  These are runs of some 30 calls; on a card that has been busy for seconds, whose clock is lower, the
+// first takes 94 us (731 TFLOP/s).  The grid's tiles are taken over at run time (attention.cuh), so that the loads of the next
 // tile overlap the end of the last: one CTA per tile took a seventh longer, two passes over the scores in tensor memory a quarter.
 //
-// The running maximum only follows the true one when it has fallen behind by a factor of 2^8: sums and products are then at
-// most 2^8 times larger than with the true maximum, far inside fp32 and inside the range of 16-bit probabilities, and O, which
+// The running maximum and sum of a softmax in one pass are Milakov and Gimelshein's (2018); to let the maximum lag is a published idea for
+// this hardware, where reading O back costs more than headroom in the exponent.  It only follows the true one when it has fallen
+// behind by a factor of 2^8: sums and products are then at most 2^8 times larger than with the true maximum, far inside fp32 and inside the range of 16-bit probabilities, and O, which
 // would have to be read and written to be rescaled, is left alone for all but the first few tiles.  Probabilities are rounded
 // to 16 bits for the product (half a step of the inputs' own type); their sum is taken before that, in 32 bits.
 #include "attention.cuh"

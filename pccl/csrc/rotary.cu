@@ -7,8 +7,9 @@
 //
 // What bounds it.  8192 rows of 16 + 16 heads of 128, bf16: forward 26.9 us (5.0 TB/s: 0.76 of the measured copy rate), backward
 // 48.1 (4.2 TB/s); 32 + 32 heads 48.3 (5.6 TB/s) and 85.2 (4.7 TB/s).  A call of this length is never far from its start and its end;
-// behind that are the instructions: the issue slots are two thirds full in the forward pass, which is why the arithmetic is on
-// pairs of 32-bit numbers.
+// behind that are, in the forward pass, the instructions: its issue slots are two thirds full, which is why the arithmetic is on
+// pairs of 32-bit numbers.  In the backward pass neither they (52 %) nor DRAM (54 % of its nominal rate) are: four warps on a scheduler
+// load four heads and then compute on them, and the largest share of their waiting, a third, is for those loads.
 //
 // The backward pass computes the norms again (its x is read for the gradient anyway).  A group sums its share of a weight's
 // gradient in registers over all its rows, a block (of queries, or of keys) adds up its groups in order, and a second small

@@ -24,7 +24,8 @@ sequence to another.
 These are plain functions like those of ``pccl.ops.gemm``: they record nothing for autograd.  Results are the same bits from
 call to call (no atomic additions).  Outputs must not overlap inputs or each other (views that lie in each other's range are
 told apart where their strides are equal).  ``scale`` is positive.  Probabilities and score gradients are rounded to the
-inputs' type for the products that they enter: with fp16 a score gradient above 65504 becomes infinite, as it does in ``dout``.
+inputs' type for the products that they enter.  With fp16 that has a range: a score gradient above 65504 becomes infinite, as it does in
+``dout``; below 6e-5 it loses digits and below 3e-8 it vanishes, so a loss whose gradients are small is scaled up first.
 """
 from __future__ import annotations
 
